@@ -422,6 +422,124 @@ int pi05_normalize_rows(const float* x, int rows, int din, const float* a, const
 int pi05_unnormalize_rows(const float* x, int rows, int din, const float* a, const float* b, int nstat, int mode,
                           float* out, int dout, void* stream);
 
+/* ---- text decoding: rotary positions and a paged key-value cache ---------- */
+
+/* Element types of the ops below (activations and cache rows). */
+#define PI05_BF16 0
+#define PI05_FP16 1
+#define PI05_FP32 2 /* pi05_rope only */
+
+/* Rotary positions.  Pair i of a head turns by turns[i] / 2^64 of a full turn per
+ * position (fixed point, so that the angle of a far position loses nothing: the
+ * product with the position wraps modulo one turn in 64-bit integers), then is
+ * scaled by `magnitude`.  The pairs are the values (i, i + rotary_dim / 2) of a
+ * head, or with `interleaved` (2 i, 2 i + 1); values from rotary_dim on pass
+ * through.  fp32 math on each value, one rounding to the element type. */
+typedef struct Pi05Rotary {
+  const uint64_t* turns; /* device [rotary_dim / 2] */
+  int rotary_dim;        /* even, <= head_dim, <= 512 */
+  int interleaved;
+  float magnitude;
+} Pi05Rotary;
+
+/* out[t, h, :] = x[t, h, :] rotated by positions[t]; `transpose` turns backwards
+ * with the same magnitude, which is the gradient of the forward call.  Strides in
+ * elements, values of a head contiguous; out may be x itself (same strides), and
+ * must not overlap it otherwise.  positions: int32, or int64 with positions_i64;
+ * any sign.  tokens == 0 is a no-op.  Rotary embedding of modeling_gemma.py:151-216
+ * for any position, layout, rotated part and scaling. */
+int pi05_rope(const void* x, void* out, int dtype, int tokens, int heads, int head_dim, long long x_token_stride,
+              long long x_head_stride, long long out_token_stride, long long out_head_stride, const void* positions,
+              int positions_i64, const Pi05Rotary* rotary, int transpose, void* stream);
+
+/* A key-value cache in pages, shared by `batch` sequences.  Row r of sequence b is
+ * line r % page_size of page page_table[b, r / page_size].  Host struct of device
+ * pointers, owned by the caller.  Ops on one cache must be ordered on one stream.
+ * A page that an op writes (append, evict, attention with `track`) belongs to one
+ * sequence; pages that are only read may be shared.  A page number outside
+ * [0, num_pages) or a row beyond the table sets PI05_DEV_BAD_INDEX in the workspace
+ * status word; the row is then skipped (append), or counts as masked (attention, and
+ * eviction leaves the sequence as it is). */
+typedef struct Pi05PagedCache {
+  void* k_pages;             /* [num_pages, n_kv_heads, page_size, head_dim], strides below */
+  void* v_pages;             /* same strides */
+  long long page_stride;     /* elements, multiples of 8; values of a row contiguous */
+  long long head_stride;
+  long long row_stride;
+  float* weight;             /* [num_pages, n_kv_heads, page_size] accumulated attention weight, or NULL */
+  int32_t* pos;              /* same shape: position of the row's token, or NULL */
+  const int32_t* page_table; /* [batch, pages_per_seq], row pitch table_pitch */
+  int32_t* counts;           /* [2, batch]: rows held, tokens seen (the next token's position) */
+  int dtype;                 /* PI05_BF16 or PI05_FP16 */
+  int num_pages, page_size, n_kv_heads, head_dim; /* head_dim % 8 == 0, <= 256 */
+  int batch, pages_per_seq, table_pitch;          /* pages_per_seq * page_size < 2^31 - 2^20 */
+  void* workspace;           /* pi05_paged_workspace_bytes() bytes, 256-byte aligned, zero-filled once;
+                                status word as in pi05_workspace_bytes() workspaces */
+  size_t workspace_bytes;
+} Pi05PagedCache;
+
+/* Workspace bytes of a cache (0 for a struct that the ops refuse). */
+size_t pi05_paged_workspace_bytes(const Pi05PagedCache* cache);
+
+/* Appends `tokens` new rows and moves the counts on.  k, v [tokens, n_kv_heads,
+ * head_dim] with token and head strides in elements; token t is number
+ * t - cu_tokens[b] of sequence b's new tokens, for cu_tokens[b] <= t <
+ * cu_tokens[b + 1] (int32 device prefix sums [batch + 1] from 0); tokens from
+ * cu_tokens[batch] on are padding and leave everything as it was.  cu_tokens NULL:
+ * one token for each sequence (tokens == batch).  With `rotary`, k (and q, if given)
+ * is rotated to its position counts[1][b] + number first; q_out is dense [tokens,
+ * n_q_heads, head_dim].  The row's `pos` is that position and its `weight`
+ * new_weight[t, h], or 0.  A row beyond the sequence's pages is dropped. */
+typedef struct Pi05PagedAppend {
+  const void* k;
+  const void* v;
+  long long k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const void* q; /* or NULL */
+  void* q_out;
+  long long q_token_stride, q_head_stride;
+  int tokens, n_q_heads;
+  const int32_t* cu_tokens;
+  const float* new_weight;  /* [tokens, n_kv_heads] dense, or NULL */
+  const Pi05Rotary* rotary; /* or NULL: rows are stored as they are (q must be NULL) */
+} Pi05PagedAppend;
+int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* args, void* stream);
+
+/* Attention of one new token of each sequence over its rows:
+ * out[b, h] = sum_r softmax_r(scale * q[b, h] . k[r]) v[r] over the counts[0][b] rows
+ * of key-value head h / (n_q_heads / n_kv_heads), in the cache's type; statistics and
+ * sums in fp32.  key_valid [batch, valid_rows] bytes with a row pitch (0 = masked row), or
+ * NULL; rows from valid_rows on count.  What a masked row holds is not read.  A sequence with no row left gives
+ * out = 0, lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.  `track`
+ * adds each row's probability, summed over the query heads of its key-value head, to
+ * the cache's `weight`.  q with strides, out dense [batch, n_q_heads, head_dim].
+ * `scratch`: pi05_paged_attention_scratch_bytes() bytes, 16-byte aligned, any content.
+ * The result does not depend on the run: every sum has a fixed order. */
+typedef struct Pi05PagedAttention {
+  const void* q;
+  void* out;
+  float* lse;
+  const uint8_t* key_valid;
+  long long q_token_stride, q_head_stride, valid_pitch;
+  int valid_rows;
+  int n_q_heads;
+  float scale;
+  int track;
+  void* scratch;
+  size_t scratch_bytes;
+} Pi05PagedAttention;
+size_t pi05_paged_attention_scratch_bytes(const Pi05PagedCache* cache, int n_q_heads, int track);
+int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* args, void* stream);
+
+/* Cuts every sequence that holds more than `budget` rows down to `budget`, each
+ * key-value head on its own: the rows with the lowest accumulated weight go (ties:
+ * the lowest row first; NaN before everything), but rows of the `recent` newest
+ * positions (pos >= counts[1][b] - recent) and of positions below `sinks` only after
+ * all others.  Rows that stay and lie below the budget keep their place; the holes
+ * between them are filled, in order, by the ones that stay from above, with their
+ * weight and pos.  Rows from the budget on are left as they are.  Needs `weight` and
+ * `pos`; budget >= 1, recent and sinks >= 0, recent + sinks <= budget. */
+int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int sinks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,410 @@
+// The paged key-value cache: append (with the rotation of q and k) and eviction by
+// accumulated attention weight.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace pi05 {
+
+int paged_check(const Pi05PagedCache* c, const char* op, Pages* out) {
+  if (c == nullptr || c->k_pages == nullptr || c->v_pages == nullptr || c->page_table == nullptr ||
+      c->counts == nullptr) {
+    set_last_error("%s: null pointer", op);
+    return PI05_ERR_INVALID_ARG;
+  }
+  if (c->dtype != PI05_BF16 && c->dtype != PI05_FP16) {
+    set_last_error("%s: dtype %d is not bf16 or fp16", op, c->dtype);
+    return PI05_ERR_INVALID_ARG;
+  }
+  const long long capacity = (long long)c->pages_per_seq * c->page_size;
+  if (c->num_pages <= 0 || c->page_size <= 0 || c->n_kv_heads <= 0 || c->batch <= 0 || c->pages_per_seq <= 0 ||
+      c->table_pitch < c->pages_per_seq || c->head_dim <= 0 || c->head_dim % 8 || c->head_dim > 256 ||
+      capacity >= (1ll << 31) - (1 << 20) || (long long)c->batch * c->n_kv_heads >= (1 << 24)) {
+    set_last_error("%s: bad cache shape pages=%d x %d kv_heads=%d head_dim=%d batch=%d pages_per_seq=%d pitch=%d", op,
+                   c->num_pages, c->page_size, c->n_kv_heads, c->head_dim, c->batch, c->pages_per_seq, c->table_pitch);
+    return PI05_ERR_SHAPE;
+  }
+  if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || c->page_stride % 8 || c->head_stride % 8 ||
+      c->row_stride % 8) {
+    set_last_error("%s: cache rows must start on 16-byte boundaries", op);
+    return PI05_ERR_ALIGN;
+  }
+  if (c->workspace == nullptr || c->workspace_bytes < kWsAccumOffset + paged_moves_bytes(c)) {
+    set_last_error("%s: workspace missing or too small", op);
+    return PI05_ERR_WORKSPACE;
+  }
+  if ((reinterpret_cast<uintptr_t>(c->workspace) & 255) != 0) {
+    set_last_error("%s: workspace not 256-byte aligned", op);
+    return PI05_ERR_ALIGN;
+  }
+  char* ws = static_cast<char*>(c->workspace);
+  out->k = static_cast<char*>(c->k_pages);
+  out->v = static_cast<char*>(c->v_pages);
+  out->page_stride = c->page_stride * 2;
+  out->head_stride = c->head_stride * 2;
+  out->row_stride = c->row_stride * 2;
+  out->weight = c->weight;
+  out->pos = c->pos;
+  out->table = c->page_table;
+  out->counts = c->counts;
+  out->status = reinterpret_cast<int*>(ws + kWsStatusOffset);
+  out->ticket = reinterpret_cast<int*>(ws + kWsCounterOffset);
+  out->moves = reinterpret_cast<int32_t*>(ws + kWsAccumOffset);
+  out->page_div = FastDiv((uint32_t)c->page_size);
+  out->num_pages = c->num_pages;
+  out->page_size = c->page_size;
+  out->heads = c->n_kv_heads;
+  out->dim = c->head_dim;
+  out->batch = c->batch;
+  out->pitch = c->table_pitch;
+  out->capacity = (int)capacity;
+  return PI05_OK;
+}
+
+namespace {
+
+// ---- append ------------------------------------------------------------------
+// Memory bound: q, k and v read once; rotated q, and k and v at their rows, written
+// once.  One token at a time per CTA: its cos and sin are shared by its heads.
+constexpr int kAppendThreads = 256;
+
+struct AppendParams {
+  const void *k, *v, *q;
+  void* q_out;
+  long long kt, kh, vt, vh, qt, qh;  // strides, elements
+  const int32_t* cu;
+  const float* new_weight;
+  const uint64_t* turns;
+  int tokens, q_heads, rotary, interleaved;
+  float magnitude;
+};
+
+template <class T, int V>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(Pages c, AppendParams p) {
+  extern __shared__ float2 cs[];  // [rotary / 2]
+  __shared__ int last;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int d = c.dim;
+  const int turned = p.rotary > 0 ? rotary_units<V>(p.rotary, p.interleaved) : 0;
+  const int rot_units = turned + (d - p.rotary) / V, row_units = d / V;
+  const int total = p.cu != nullptr ? min(max(p.cu[c.batch], 0), p.tokens) : p.tokens;
+  for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    int b = t, off = 0;
+    if (p.cu != nullptr) {  // the sequence with cu[b] <= t < cu[b + 1]
+      int lo = 0, hi = c.batch;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        (p.cu[mid] <= t ? lo : hi) = mid;
+      }
+      b = lo;
+      off = t - p.cu[b];
+    }
+    const int held = c.counts[b], seen = c.counts[c.batch + b];
+    const long long r = (long long)held + off;
+    const int position = seen + off;
+    int line = 0, page = -1;
+    if (r >= 0 && r < c.capacity) page = c.page_of(b, (int)r, &line);
+    const bool ok = c.real(page);
+    if (!ok && threadIdx.x == 0) report_status(c.status, PI05_DEV_BAD_INDEX);
+    for (int i = threadIdx.x; i < p.rotary / 2; i += kAppendThreads)
+      cs[i] = rotation(position, p.turns[i], p.magnitude, false);
+    __syncthreads();
+    const int nq = p.q_heads * rot_units, nk = ok ? c.heads * rot_units : 0, nv = ok ? c.heads * row_units : 0;
+    for (int i = threadIdx.x; i < nq + nk + nv; i += kAppendThreads) {
+      const T* src;
+      T* dst;
+      int u, first = turned;
+      if (i < nq) {
+        const int h = i / rot_units;
+        u = i - h * rot_units;
+        src = static_cast<const T*>(p.q) + t * p.qt + h * p.qh;
+        dst = static_cast<T*>(p.q_out) + ((size_t)t * p.q_heads + h) * d;
+      } else if (i < nq + nk) {
+        const int h = (i - nq) / rot_units;
+        u = i - nq - h * rot_units;
+        src = static_cast<const T*>(p.k) + t * p.kt + h * p.kh;
+        dst = reinterpret_cast<T*>(c.k + c.row_at(page, h, line));
+      } else {
+        const int h = (i - nq - nk) / row_units;
+        u = i - nq - nk - h * row_units;
+        first = 0;
+        src = static_cast<const T*>(p.v) + t * p.vt + h * p.vh;
+        dst = reinterpret_cast<T*>(c.v + c.row_at(page, h, line));
+      }
+      if (u < first) {
+        rotate_unit<T, V>(src, dst, u, p.rotary, p.interleaved, cs);
+      } else {
+        Chunk<T, V> x;
+        const int at = (first > 0 ? p.rotary : 0) + (u - first) * V;
+        x.load(src + at);
+        x.store(dst + at);
+      }
+    }
+    if (ok) {
+      for (int h = threadIdx.x; h < c.heads; h += kAppendThreads) {
+        const size_t s = c.slot_at(page, h, line);
+        if (c.pos != nullptr) c.pos[s] = position;
+        if (c.weight != nullptr) c.weight[s] = p.new_weight != nullptr ? p.new_weight[(size_t)t * c.heads + h] : 0.f;
+      }
+    }
+    __syncthreads();  // the next token's cos and sin; and everyone has read the counts
+    if (p.cu == nullptr && threadIdx.x == 0) {  // this CTA alone has the sequence
+      c.counts[b] = max(held, min(held + 1, c.capacity));
+      c.counts[c.batch + b] = seen + 1;
+    }
+  }
+  if (p.cu == nullptr) return;
+  // Ragged: the CTA that finishes last moves the counts on, when all have read them.
+  if (threadIdx.x == 0) last = atom_add_acq_rel_gpu(c.ticket, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  for (int b = threadIdx.x; b < c.batch; b += kAppendThreads) {
+    const int n = max(min(p.cu[b + 1], p.tokens) - max(p.cu[b], 0), 0), held = c.counts[b];
+    c.counts[b] = max(held, (int)min((long long)held + n, (long long)c.capacity));
+    c.counts[c.batch + b] += n;
+  }
+  if (threadIdx.x == 0) *c.ticket = 0;
+}
+
+// ---- eviction ------------------------------------------------------------------
+// The rows of a (sequence, head) are ordered by a 32-bit key that sorts like the
+// weight; radix selection gives the key of the last row to go, and how many rows of
+// just that key go with it.
+constexpr int kSelectThreads = 1024;
+constexpr int kMoveThreads = 256;
+
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, long long recent_from, int sinks) {
+  if (pos >= recent_from || pos < sinks) return 0xffffffffu;
+  if (w != w) return 0u;
+  if (w == 0.f) return 0x80000000u;
+  const uint32_t u = __float_as_uint(w);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t key_of_row(const Pages& c, int b, int h, int r, long long recent_from, int sinks,
+                                               bool* bad) {
+  int line;
+  const int page = c.page_of(b, r, &line);
+  if (!c.real(page)) {
+    *bad = true;
+    return 0u;
+  }
+  const size_t s = c.slot_at(page, h, line);
+  return evict_key(c.weight[s], c.pos[s], recent_from, sinks);
+}
+
+// Moves of row list `moves`: [0] their number (-1: the sequence stays as it is), [1] the
+// rows left, then the holes, ascending, and from [2 + left] on the rows that fill them.
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(Pages c, int budget, int recent, int sinks) {
+  __shared__ int hist[256];
+  __shared__ int warp_sum[kSelectThreads / 32];
+  __shared__ uint32_t sh_prefix;
+  __shared__ int sh_want;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads, tid = threadIdx.x;
+  int32_t* moves = c.moves + (size_t)blockIdx.x * (c.capacity + 2);
+  const int len = c.rows(b);
+  const long long recent_from = (long long)c.counts[c.batch + b] - recent;
+  if (len <= budget) {
+    if (tid == 0) moves[0] = -1;
+    return;
+  }
+  bool bad = false;
+  uint32_t prefix = 0;
+  int want = len - budget;  // the want-th smallest of the keys that begin with `prefix`
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+    __syncthreads();
+    for (int r = tid; r < len; r += kSelectThreads) {
+      const uint32_t key = key_of_row(c, b, h, r, recent_from, sinks, &bad);
+      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+    }
+    if (__syncthreads_or(bad)) {
+      if (tid == 0) {
+        moves[0] = -1;
+        report_status(c.status, PI05_DEV_BAD_INDEX);
+      }
+      return;
+    }
+    if (tid == 0) {
+      int sum = 0, i = 0;
+      while (sum + hist[i] < want) sum += hist[i++];
+      sh_prefix = prefix | ((uint32_t)i << shift);
+      sh_want = want - sum;
+    }
+    __syncthreads();
+    prefix = sh_prefix;
+    want = sh_want;
+  }
+  // Rows in order: keys below `prefix` go, and the first `want` that equal it.
+  const int lane = tid & 31, w = tid >> 5;
+  int ties = 0, holes = 0, tails = 0;
+  for (int r0 = 0; r0 < len; r0 += kSelectThreads) {
+    const int r = r0 + tid;
+    const uint32_t key = r < len ? key_of_row(c, b, h, r, recent_from, sinks, &bad) : 0u;
+    const bool tie = r < len && key == prefix;
+    const uint32_t below = (1u << lane) - 1;
+    uint32_t m = __ballot_sync(~0u, tie);
+    __syncthreads();
+    if (lane == 0) warp_sum[w] = __popc(m);
+    __syncthreads();
+    int before = ties + __popc(m & below);
+    for (int i = 0; i < kSelectThreads / 32; ++i) {
+      if (i < w) before += warp_sum[i];
+      ties += warp_sum[i];
+    }
+    const bool gone = r < len && (key < prefix || (tie && before < want));
+    const bool hole = gone && r < budget, tail = r < len && !gone && r >= budget;
+    m = __ballot_sync(~0u, hole);
+    const uint32_t m2 = __ballot_sync(~0u, tail);
+    __syncthreads();
+    if (lane == 0) warp_sum[w] = __popc(m) | (__popc(m2) << 16);
+    __syncthreads();
+    int at_hole = holes + __popc(m & below), at_tail = tails + __popc(m2 & below);
+    for (int i = 0; i < kSelectThreads / 32; ++i) {
+      const int a = warp_sum[i] & 0xffff, t = warp_sum[i] >> 16;
+      if (i < w) at_hole += a, at_tail += t;
+      holes += a;
+      tails += t;
+    }
+    if (hole) moves[2 + at_hole] = r;
+    if (tail) moves[2 + budget + at_tail] = r;
+  }
+  if (tid == 0) {
+    moves[0] = holes;
+    moves[1] = budget;
+  }
+}
+
+// One warp per move.  Sources lie at or above the budget and targets below it, so no
+// move reads what another writes.
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(Pages c) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads;
+  const int32_t* moves = c.moves + (size_t)blockIdx.x * (c.capacity + 2);
+  const int n = moves[0];
+  if (n < 0) return;
+  const int left = moves[1], lane = threadIdx.x & 31;
+  for (int m = blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5); m < n; m += gridDim.y * (kMoveThreads / 32)) {
+    int from_line, to_line;
+    const int from = c.page_of(b, moves[2 + left + m], &from_line), to = c.page_of(b, moves[2 + m], &to_line);
+    const size_t src = c.row_at(from, h, from_line), dst = c.row_at(to, h, to_line);
+    if (lane < c.dim / 8) {
+      const uint4 k = reinterpret_cast<const uint4*>(c.k + src)[lane], v = reinterpret_cast<const uint4*>(c.v + src)[lane];
+      reinterpret_cast<uint4*>(c.k + dst)[lane] = k;
+      reinterpret_cast<uint4*>(c.v + dst)[lane] = v;
+    }
+    if (lane == 0) {
+      const size_t s = c.slot_at(from, h, from_line), t = c.slot_at(to, h, to_line);
+      c.weight[t] = c.weight[s];
+      c.pos[t] = c.pos[s];
+    }
+  }
+  if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) c.counts[b] = left;
+}
+
+template <class T>
+int append_run(const Pages& c, const AppendParams& p, cudaStream_t stream) {
+  const bool vec = aligned16(p.k) && aligned16(p.v) && p.kt % 8 == 0 && p.kh % 8 == 0 && p.vt % 8 == 0 &&
+                   p.vh % 8 == 0 &&
+                   (p.q == nullptr || (aligned16(p.q) && aligned16(p.q_out) && p.qt % 8 == 0 && p.qh % 8 == 0)) &&
+                   p.rotary % (p.interleaved ? 8 : 16) == 0;
+  const int grid = p.cu == nullptr ? p.tokens : std::min(p.tokens, kSMs * 8);
+  return launch_pdl(vec ? append_kernel<T, 8> : append_kernel<T, 1>, dim3(grid), dim3(kAppendThreads),
+                    (size_t)(p.rotary / 2) * sizeof(float2), stream, pdl_enabled(), c, p);
+}
+
+}  // namespace
+}  // namespace pi05
+
+using namespace pi05;
+
+extern "C" {
+
+size_t pi05_paged_workspace_bytes(const Pi05PagedCache* cache) {
+  if (cache == nullptr || cache->batch <= 0 || cache->n_kv_heads <= 0 || cache->pages_per_seq <= 0 ||
+      cache->page_size <= 0)
+    return 0;
+  return (kWsAccumOffset + paged_moves_bytes(cache) + 255) & ~size_t(255);
+}
+
+int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, void* stream) {
+  Pages c;
+  int rc = paged_check(cache, "paged_append", &c);
+  if (rc) return rc;
+  if (a == nullptr || (a->tokens > 0 && (a->k == nullptr || a->v == nullptr)) ||
+      (a->q != nullptr && a->q_out == nullptr)) {
+    set_last_error("paged_append: null pointer");
+    return PI05_ERR_INVALID_ARG;
+  }
+  const Pi05Rotary* rot = a->rotary;
+  if (rot == nullptr && a->q != nullptr) {
+    set_last_error("paged_append: q without rotary has nothing to do");
+    return PI05_ERR_INVALID_ARG;
+  }
+  if (rot != nullptr && (rot->turns == nullptr || rot->rotary_dim <= 0 || rot->rotary_dim % 2 ||
+                         rot->rotary_dim > c.dim)) {
+    set_last_error("paged_append: bad rotary_dim %d for head_dim %d", rot->rotary_dim, c.dim);
+    return PI05_ERR_SHAPE;
+  }
+  if (a->tokens < 0 || (a->q != nullptr && (a->n_q_heads <= 0 || (long long)a->n_q_heads * c.dim > (1 << 24))) ||
+      (a->cu_tokens == nullptr && a->tokens != c.batch)) {
+    set_last_error("paged_append: bad shape tokens=%d n_q_heads=%d batch=%d", a->tokens, a->n_q_heads, c.batch);
+    return PI05_ERR_SHAPE;
+  }
+  if (a->new_weight != nullptr && c.weight == nullptr) {
+    set_last_error("paged_append: the cache keeps no weights");
+    return PI05_ERR_INVALID_ARG;
+  }
+  if (a->tokens == 0) return PI05_OK;
+  AppendParams p;
+  p.k = a->k;
+  p.v = a->v;
+  p.q = a->q;
+  p.q_out = a->q_out;
+  p.kt = a->k_token_stride;
+  p.kh = a->k_head_stride;
+  p.vt = a->v_token_stride;
+  p.vh = a->v_head_stride;
+  p.qt = a->q_token_stride;
+  p.qh = a->q_head_stride;
+  p.cu = a->cu_tokens;
+  p.new_weight = a->new_weight;
+  p.turns = rot ? rot->turns : nullptr;
+  p.tokens = a->tokens;
+  p.q_heads = a->q != nullptr ? a->n_q_heads : 0;
+  p.rotary = rot ? rot->rotary_dim : 0;
+  p.interleaved = rot ? rot->interleaved : 0;
+  p.magnitude = rot ? rot->magnitude : 1.f;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return cache->dtype == PI05_BF16 ? append_run<__nv_bfloat16>(c, p, st) : append_run<__half>(c, p, st);
+}
+
+int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int sinks, void* stream) {
+  Pages c;
+  int rc = paged_check(cache, "paged_evict", &c);
+  if (rc) return rc;
+  if (c.weight == nullptr || c.pos == nullptr) {
+    set_last_error("paged_evict: the cache keeps no weights or positions");
+    return PI05_ERR_INVALID_ARG;
+  }
+  if (budget < 1 || recent < 0 || sinks < 0 || (long long)recent + sinks > budget) {
+    set_last_error("paged_evict: need budget >= 1 and 0 <= recent + sinks <= budget (budget=%d recent=%d sinks=%d)",
+                   budget, recent, sinks);
+    return PI05_ERR_SHAPE;
+  }
+  if (budget >= c.capacity) return PI05_OK;  // no sequence can hold more
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int rows = c.batch * c.heads;
+  rc = launch_pdl(evict_select_kernel, dim3(rows), dim3(kSelectThreads), 0, st, pdl_enabled(), c, budget, recent,
+                  sinks);
+  if (rc) return rc;
+  const int most = std::min(budget, c.capacity - budget);
+  const int chunks = std::min((most + kMoveThreads / 32 - 1) / (kMoveThreads / 32), std::max(1, kSMs * 16 / rows));
+  return launch_pdl(evict_move_kernel, dim3(rows, chunks), dim3(kMoveThreads), 0, st, pdl_enabled(), c);
+}
+
+}  // extern "C"

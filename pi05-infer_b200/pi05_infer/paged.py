@@ -1,0 +1,459 @@
+"""Text decoding on a paged key-value cache: rotary positions, append, single-token
+attention, and eviction by accumulated attention weight.
+
+The engine's own loop (``expert.py``) keeps one dense cache per observation; a program
+that decodes text next to it -- tokens one at a time, many sequences of different
+lengths, long contexts -- keeps its keys and values in pages::
+
+    freqs = RopeFrequencies(256, device="cuda")
+    cache = PagedKVCache.allocate(num_pages=512, page_size=64, n_kv_heads=1, head_dim=256, batch=4,
+                                  pages_per_seq=32, device="cuda")
+    cache.page_table.copy_(...)                     # which pages each sequence owns
+    cache.append(k, v, cu_tokens=cu, freqs=freqs)   # prompts, ragged
+    q = cache.append(k1, v1, q=q1, freqs=freqs)     # then one token of each sequence
+    out = cache.attend(q, track=True)
+    cache.evict(budget=1024, recent=128, sinks=4)
+
+Rotary embedding: the reference's ``modeling_gemma.py:151-216`` (half layout, no
+scaling); the cache has no counterpart there.  Calls run on the current stream of the
+tensors' device and never synchronise; calls on one cache are to be ordered on one
+stream (or by events).  Everything can be captured in a CUDA graph.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_P = ctypes.c_void_p
+_I = ctypes.c_int
+_L = ctypes.c_longlong
+_Z = ctypes.c_size_t
+_F = ctypes.c_float
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class Pi05Rotary(ctypes.Structure):
+    _fields_ = [("turns", _P), ("rotary_dim", _I), ("interleaved", _I), ("magnitude", _F)]
+
+
+class Pi05PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", _P), ("v_pages", _P), ("page_stride", _L), ("head_stride", _L), ("row_stride", _L),
+        ("weight", _P), ("pos", _P), ("page_table", _P), ("counts", _P),
+        ("dtype", _I), ("num_pages", _I), ("page_size", _I), ("n_kv_heads", _I), ("head_dim", _I),
+        ("batch", _I), ("pages_per_seq", _I), ("table_pitch", _I),
+        ("workspace", _P), ("workspace_bytes", _Z),
+    ]
+
+
+class Pi05PagedAppend(ctypes.Structure):
+    _fields_ = [
+        ("k", _P), ("v", _P), ("k_token_stride", _L), ("k_head_stride", _L), ("v_token_stride", _L),
+        ("v_head_stride", _L), ("q", _P), ("q_out", _P), ("q_token_stride", _L), ("q_head_stride", _L),
+        ("tokens", _I), ("n_q_heads", _I), ("cu_tokens", _P), ("new_weight", _P),
+        ("rotary", ctypes.POINTER(Pi05Rotary)),
+    ]
+
+
+class Pi05PagedAttention(ctypes.Structure):
+    _fields_ = [
+        ("q", _P), ("out", _P), ("lse", _P), ("key_valid", _P), ("q_token_stride", _L), ("q_head_stride", _L),
+        ("valid_pitch", _L), ("valid_rows", _I), ("n_q_heads", _I), ("scale", _F), ("track", _I), ("scratch", _P), ("scratch_bytes", _Z),
+    ]
+
+
+_CACHE = ctypes.POINTER(Pi05PagedCache)
+_lib.SIGNATURES.update({
+    "pi05_rope": (_I, [_P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _P, _I, ctypes.POINTER(Pi05Rotary), _I, _P]),
+    "pi05_paged_workspace_bytes": (_Z, [_CACHE]),
+    "pi05_paged_append": (_I, [_CACHE, ctypes.POINTER(Pi05PagedAppend), _P]),
+    "pi05_paged_attention_scratch_bytes": (_Z, [_CACHE, _I, _I]),
+    "pi05_paged_attention": (_I, [_CACHE, ctypes.POINTER(Pi05PagedAttention), _P]),
+    "pi05_paged_evict": (_I, [_CACHE, _I, _I, _I, _P]),
+})
+_fns = {}
+
+
+def _fn(name: str):
+    f = _fns.get(name)
+    if f is None:
+        f = getattr(_lib.lib(), name)
+        f.restype, f.argtypes = _lib.SIGNATURES[name]
+        _fns[name] = f
+    return f
+
+
+def _run(name: str, device: torch.device, *args) -> None:
+    """Calls the library on the current stream of ``device``, whichever device is current."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = _fn(name)(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        rc = _fn(name)(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc != _lib.PI05_OK:
+        raise _lib.Pi05Error(name, rc, _lib.last_error())
+
+
+def _cuda(device) -> torch.device:
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"expected a CUDA device, got {device} (pi05_infer has no CPU fallback)")
+    return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+
+def _pair_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast, beta_slow):
+    """Rad per position of each pair, and the factor on cos and sin."""
+    if scaling == "ntk":
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    inv_freq = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if scaling == "linear":
+        return [f / factor for f in inv_freq], 1.0
+    if scaling != "yarn":
+        return inv_freq, 1.0
+
+    def pair(turns):  # number (not whole) of the pair that turns so often within original_len
+        return rotary_dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
+    ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(rotary_dim // 2)]
+    return [f / factor * r + f * (1 - r) for f, r in zip(inv_freq, ramp)], 0.1 * math.log(factor) + 1.0
+
+
+def _turns(inv_freq):
+    """Fractions of a turn per position in units of 2^-64 (below one half: every frequency is at most 1 rad)."""
+    return [int(f / (2 * math.pi) * 2.0**64) for f in inv_freq]
+
+
+class RopeFrequencies:
+    """What each pair of a head turns by per position, as the kernels take it.
+
+    Pair ``i`` of the first ``rotary_dim`` values of a head turns by ``base ** (-2 i /
+    rotary_dim)`` rad per position.  ``layout``: ``"half"`` pairs value ``i`` with ``i +
+    rotary_dim / 2`` (``modeling_gemma.py:184-216``), ``"interleaved"`` ``2 i`` with ``2 i +
+    1``.  ``scaling`` for contexts longer than the trained ``original_len``, by ``factor``:
+
+    * ``"linear"``: every frequency divided by ``factor`` (position interpolation);
+    * ``"ntk"``: ``base * factor ** (rotary_dim / (rotary_dim - 2))``;
+    * ``"yarn"``: pairs that turn less than ``beta_slow`` times within ``original_len`` are
+      divided by ``factor``, those over ``beta_fast`` times are kept, a linear ramp over the pair
+      number between; cos and sin times ``0.1 ln(factor) + 1``.
+
+    The device table holds fractions of a turn in 64-bit fixed point, so an angle is as exact at
+    position 10^9 as at 1.
+    """
+
+    def __init__(self, rotary_dim: int, base: float = 10000.0, *, layout: str = "half", scaling: Optional[str] = None,
+                 factor: float = 1.0, original_len: Optional[int] = None, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, device="cuda"):
+        if rotary_dim <= 0 or rotary_dim % 2 or rotary_dim > 512:
+            raise ValueError(f"rotary_dim {rotary_dim} is not an even number of 2..512")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout {layout!r} is not 'half' or 'interleaved'")
+        if scaling not in (None, "linear", "ntk", "yarn"):
+            raise ValueError(f"scaling {scaling!r} is not None, 'linear', 'ntk' or 'yarn'")
+        if not base > 1 or not math.isfinite(base):
+            raise ValueError(f"base {base} is not above 1")
+        if scaling is not None and not (factor >= 1 and math.isfinite(factor)):
+            raise ValueError(f"factor {factor} is not 1 or more")
+        if scaling == "ntk" and rotary_dim == 2:
+            raise ValueError("'ntk' scaling needs rotary_dim > 2")
+        if scaling == "yarn" and (original_len is None or original_len <= 0 or not beta_fast > beta_slow > 0):
+            raise ValueError("'yarn' scaling needs original_len and beta_fast > beta_slow > 0")
+        self.rotary_dim, self.layout = rotary_dim, layout
+        self.inv_freq, self.magnitude = _pair_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast,
+                                                          beta_slow)
+        turns = _turns(self.inv_freq)
+        self.device = _cuda(device)
+        self.turns = torch.tensor(turns, dtype=torch.int64).to(self.device)
+        self.c = Pi05Rotary(self.turns.data_ptr(), rotary_dim, int(layout == "interleaved"), self.magnitude)
+        self._ref = ctypes.byref(self.c)
+
+
+def _rope(x, positions, freqs, out, transpose):
+    tokens, heads, dim = x.shape
+    _run("pi05_rope", x.device, x.data_ptr(), out.data_ptr(), _DTYPES[x.dtype], tokens, heads, dim, x.stride(0),
+         x.stride(1), out.stride(0), out.stride(1), positions.data_ptr(), positions.dtype == torch.int64, freqs._ref,
+         transpose)
+    return out
+
+
+class _Rope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, freqs, transpose):
+        ctx.save_for_backward(positions)
+        ctx.freqs, ctx.transpose = freqs, transpose
+        return _rope(x, positions, freqs, torch.empty(x.shape, dtype=x.dtype, device=x.device), transpose)
+
+    @staticmethod
+    def backward(ctx, g):
+        (positions,) = ctx.saved_tensors
+        g = g if g.stride(-1) == 1 else g.contiguous()
+        return _Rope.apply(g, positions, ctx.freqs, not ctx.transpose), None, None, None
+
+
+def _leaf_node(x: torch.Tensor):
+    """The node that accumulates leaf ``x``'s gradient, marked with the stream it was first seen on.
+
+    Torch makes it with the first graph that uses the leaf and keeps it as long as any lives; a backward
+    pass waits for its stream, which a capture on another stream cannot (torch then breaks the capture off
+    and leaves its random generator in it).  So a captured call is refused while such a graph is alive.
+    """
+    node = torch.autograd.graph.get_gradient_edge(x).node
+    stream = torch.cuda.current_stream(x.device).cuda_stream
+    first = node.metadata.setdefault("pi05_stream", stream)
+    if first != stream and torch.cuda.is_current_stream_capturing():
+        raise ValueError("x is a leaf that an earlier graph, made on another stream, still uses: drop that graph "
+                         "before capturing this call")
+    return node
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, transpose: bool = False,
+         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x`` ``[tokens, heads, dim]`` with the first ``freqs.rotary_dim`` values of each head rotated
+    to ``positions`` ``[tokens]`` (int32 or int64, any sign).
+
+    bf16, fp16 or fp32, fp32 math, one rounding.  Any token and head strides (a q|k|v row's q and k
+    heads in one call, say); values of a head contiguous.  ``out`` may be ``x`` (in place), but not
+    overlap it otherwise.  ``transpose`` turns backwards.  Differentiable in ``x`` when ``out`` is
+    not given; a captured call with a leaf ``x`` is refused while a graph of it from another stream
+    is alive.
+    """
+    if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda or x.stride(2) != 1:
+        raise ValueError("x must be a [tokens, heads, dim] CUDA tensor, bf16, fp16 or fp32, contiguous in dim")
+    if positions.shape != x.shape[:1] or positions.dtype not in (torch.int32, torch.int64) or \
+            positions.device != x.device or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int32 or int64 [tokens] on x's device")
+    if freqs.device != x.device:
+        raise ValueError(f"the frequencies are on {freqs.device}, x is on {x.device}")
+    if freqs.rotary_dim > x.shape[2]:
+        raise ValueError(f"rotary_dim {freqs.rotary_dim} is more than the head's {x.shape[2]} values")
+    grad = x.requires_grad and torch.is_grad_enabled()
+    if out is None:
+        if grad:
+            node = _leaf_node(x) if x.is_leaf else None  # alive until the new graph holds it
+            y = _Rope.apply(x, positions, freqs, bool(transpose))
+            del node
+            return y
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif grad:
+        raise ValueError("out= is not differentiable")
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
+        raise ValueError("out must have x's shape, type and device, contiguous in dim")
+    return _rope(x, positions, freqs, out, bool(transpose))
+
+
+# ---------------------------------------------------------------------------
+# the paged cache
+# ---------------------------------------------------------------------------
+
+
+class PagedKVCache:
+    """Keys and values of ``batch`` sequences in pages.
+
+    ``k_pages`` / ``v_pages`` ``[num_pages, n_kv_heads, page_size, head_dim]`` (bf16 or fp16, same
+    strides, rows on 16-byte boundaries), ``page_table`` ``[batch, pages_per_seq]`` int32, ``counts``
+    ``[2, batch]`` int32 (rows held; tokens seen, which is the next token's position), and for
+    eviction ``weight`` (fp32) and ``pos`` (int32) ``[num_pages, n_kv_heads, page_size]``.  Row ``r``
+    of sequence ``b`` is line ``r % page_size`` of page ``page_table[b, r // page_size]``.  The
+    tensors stay the caller's: who owns which page, and resetting or truncating a sequence (``counts``),
+    is done by writing to them.
+
+    The table is read on the device.  A page number outside the cache, or a row beyond the table,
+    is skipped or masked and sets ``PI05_DEV_BAD_INDEX`` (0x20) in :meth:`read_status`.  A page
+    that a call writes belongs to one sequence.
+    """
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, counts: torch.Tensor, *,
+                 weight: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None):
+        if k_pages.dim() != 4 or k_pages.dtype not in (torch.bfloat16, torch.float16) or not k_pages.is_cuda:
+            raise ValueError("k_pages must be a [pages, kv_heads, page_size, dim] CUDA tensor, bf16 or fp16")
+        device = k_pages.device
+        if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != device or \
+                v_pages.stride() != k_pages.stride() or k_pages.stride(3) != 1:
+            raise ValueError("v_pages must match k_pages (shape, type, device, strides; rows contiguous)")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device or \
+                page_table.stride(1) != 1:
+            raise ValueError("page_table must be int32 [batch, pages_per_seq] on the cache's device, rows contiguous")
+        if counts.shape != (2, page_table.shape[0]) or counts.dtype != torch.int32 or counts.device != device or \
+                not counts.is_contiguous():
+            raise ValueError("counts must be contiguous int32 [2, batch] on the cache's device")
+        for t, dt, name in ((weight, torch.float32, "weight"), (pos, torch.int32, "pos")):
+            if t is not None and (t.shape != k_pages.shape[:3] or t.dtype != dt or t.device != device or
+                                  not t.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous {dt} {list(k_pages.shape[:3])} on the cache's device")
+        self.k_pages, self.v_pages, self.page_table, self.counts = k_pages, v_pages, page_table, counts
+        self.weight, self.pos, self.device, self.dtype = weight, pos, device, k_pages.dtype
+        self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k_pages.shape
+        self.batch, self.pages_per_seq = page_table.shape
+
+        def p(t):
+            return None if t is None else t.data_ptr()
+
+        self._c = Pi05PagedCache(
+            p(k_pages), p(v_pages), *k_pages.stride()[:3], p(weight), p(pos), p(page_table), p(counts),
+            _DTYPES[self.dtype], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, self.batch,
+            self.pages_per_seq, page_table.stride(0), None, 0)
+        self._ref = ctypes.byref(self._c)
+        nbytes = _fn("pi05_paged_workspace_bytes")(self._ref)
+        # status word, ticket and the eviction's lists; zeroed once
+        self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self._c.workspace, self._c.workspace_bytes = self.workspace.data_ptr(), nbytes
+        self._scratch_bytes = {}
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, batch: int, pages_per_seq: int, *,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", track: bool = True) -> "PagedKVCache":
+        """A cache with zeroed tensors of its own; ``track``: with ``weight`` and ``pos``."""
+        device = _cuda(device)
+        shape = (num_pages, n_kv_heads, page_size)
+
+        def zeros(*size, dt):
+            return torch.zeros(size, dtype=dt, device=device)
+
+        return cls(zeros(*shape, head_dim, dt=dtype), zeros(*shape, head_dim, dt=dtype),
+                   zeros(batch, pages_per_seq, dt=torch.int32), zeros(2, batch, dt=torch.int32),
+                   weight=zeros(*shape, dt=torch.float32) if track else None,
+                   pos=zeros(*shape, dt=torch.int32) if track else None)
+
+    @property
+    def lens(self) -> torch.Tensor:
+        """Rows held by each sequence (a view of ``counts``)."""
+        return self.counts[0]
+
+    def _rows(self, t: torch.Tensor, name: str, heads: Optional[int]) -> None:
+        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or t.shape[2] != self.head_dim or \
+                t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
+                             f"{self.dtype} on {self.device}, contiguous in its last dimension")
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
+               freqs: Optional[RopeFrequencies] = None, cu_tokens: Optional[torch.Tensor] = None,
+               weight: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """Writes new rows behind each sequence's last and moves ``counts`` on.
+
+        ``k``, ``v`` ``[tokens, n_kv_heads, head_dim]``, any token and head strides.  One token of each
+        sequence (``tokens == batch``), or with ``cu_tokens`` (int32 ``[batch + 1]`` prefix sums
+        from 0, on the device) any number of each, none included; tokens behind the last sequence's are
+        padding and left out.  With ``freqs``, ``k`` and ``q`` ``[tokens, heads, head_dim]`` are
+        rotated to their positions; the rotated ``q`` is returned (rows of padding tokens as they were
+        in ``q_out``).  ``weight`` ``[tokens, n_kv_heads]`` fp32 is what the rows start with (0
+        otherwise), e.g. what the prompt's own attention gave them.
+        """
+        self._rows(k, "k", self.n_kv_heads)
+        self._rows(v, "v", self.n_kv_heads)
+        tokens = k.shape[0]
+        if v.shape[0] != tokens:
+            raise ValueError(f"k has {tokens} tokens, v has {v.shape[0]}")
+        a = Pi05PagedAppend(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        a.tokens = tokens
+        if q is not None:
+            self._rows(q, "q", None)
+            if freqs is None:
+                raise ValueError("q is only rotated: give freqs, or leave q out")
+            if q.shape[0] != tokens:
+                raise ValueError(f"k has {tokens} tokens, q has {q.shape[0]}")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device or \
+                    not q_out.is_contiguous():
+                raise ValueError("q_out must be contiguous, of q's shape, type and device")
+            a.q, a.q_out, a.q_token_stride, a.q_head_stride = q.data_ptr(), q_out.data_ptr(), q.stride(0), q.stride(1)
+            a.n_q_heads = q.shape[1]
+        if freqs is not None:
+            if freqs.device != self.device or freqs.rotary_dim > self.head_dim:
+                raise ValueError(f"freqs must be on {self.device} with rotary_dim <= {self.head_dim}")
+            a.rotary = ctypes.pointer(freqs.c)
+        if cu_tokens is not None:
+            if cu_tokens.shape != (self.batch + 1,) or cu_tokens.dtype != torch.int32 or \
+                    cu_tokens.device != self.device or not cu_tokens.is_contiguous():
+                raise ValueError(f"cu_tokens must be contiguous int32 [{self.batch + 1}] on {self.device}")
+            a.cu_tokens = cu_tokens.data_ptr()
+        elif tokens != self.batch:
+            raise ValueError(f"{tokens} tokens for {self.batch} sequences need cu_tokens")
+        if weight is not None:
+            if self.weight is None or weight.shape != (tokens, self.n_kv_heads) or weight.dtype != torch.float32 or \
+                    weight.device != self.device or not weight.is_contiguous():
+                raise ValueError(f"weight must be contiguous fp32 [{tokens}, {self.n_kv_heads}] on {self.device}, "
+                                 "for a cache that keeps weights")
+            a.new_weight = weight.data_ptr()
+        _run("pi05_paged_append", self.device, self._ref, ctypes.byref(a))
+        return q_out if q is not None else None
+
+    def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, key_valid: Optional[torch.Tensor] = None,
+               track: bool = False, out: Optional[torch.Tensor] = None, return_lse: bool = False):
+        """Attention of one token of each sequence over its rows: ``q`` ``[batch, heads, head_dim]``
+        (any token and head strides), ``heads`` a multiple of ``n_kv_heads``.
+
+        ``scale`` is ``head_dim ** -0.5`` if not given.  ``key_valid`` (bool or uint8 ``[batch, n]``):
+        rows that are False are left out, whatever they hold; rows from ``n`` on count (a prompt's
+        padding mask need not grow with the sequence).  ``track`` adds the probabilities
+        to the cache's ``weight``.  A sequence with no row gives zeros (lse ``-inf``).  Returns
+        ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32 natural-log sums
+        ``[batch, heads]``.
+        """
+        self._rows(q, "q", None)
+        batch, heads, dim = q.shape
+        if batch != self.batch or heads == 0 or heads % self.n_kv_heads:
+            raise ValueError(f"q must be [{self.batch}, a multiple of {self.n_kv_heads}, {dim}], got {list(q.shape)}")
+        if track and self.weight is None:
+            raise ValueError("this cache keeps no weights: build it with weight=")
+        if out is None:
+            out = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            raise ValueError("out must be contiguous, of q's shape, type and device")
+        lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        pitch = valid_rows = 0
+        if key_valid is not None:
+            if key_valid.dim() != 2 or key_valid.dtype not in (torch.bool, torch.uint8) or \
+                    key_valid.shape[0] != batch or key_valid.device != self.device or key_valid.stride(1) != 1:
+                raise ValueError("key_valid must be bool or uint8 [batch, rows] on the cache's device, rows contiguous")
+            pitch, valid_rows = key_valid.stride(0), key_valid.shape[1]
+        need = self._scratch_bytes.get((heads, track))
+        if need is None:
+            need = self._scratch_bytes[heads, track] = _fn("pi05_paged_attention_scratch_bytes")(
+                self._ref, heads, track)
+        # from torch's allocator, call by call: calls on different streams, and graphs, never share it
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a = Pi05PagedAttention(
+            q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+            None if key_valid is None else key_valid.data_ptr(), q.stride(0), q.stride(1), pitch, valid_rows, heads,
+            dim**-0.5 if scale is None else scale, track, scratch.data_ptr(), need)
+        _run("pi05_paged_attention", self.device, self._ref, ctypes.byref(a))
+        return (out, lse) if return_lse else out
+
+    def evict(self, budget: int, *, recent: int = 0, sinks: int = 0) -> None:
+        """Cuts every sequence with more than ``budget`` rows down to it.
+
+        Each key-value head on its own gives up the rows with the lowest accumulated ``weight``
+        (ties: the lowest row first; NaN first of all), those of the ``recent`` newest positions and
+        of the first ``sinks`` positions only after all others.  The holes below the budget are filled in
+        order by the rows that stay from above it, so the rows of a head are in no order of age
+        afterwards: ``pos`` says which token a row is.
+        """
+        if self.weight is None or self.pos is None:
+            raise ValueError("this cache keeps no weights and positions: build it with weight= and pos=")
+        if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+            raise ValueError(f"need budget >= 1 and 0 <= recent + sinks <= budget, got {budget}, {recent}, {sinks}")
+        _run("pi05_paged_evict", self.device, self._ref, budget, recent, sinks)
+
+    def read_status(self) -> int:
+        """Synchronise, read and clear the cache's device status word (0 = nothing went wrong)."""
+        v = ctypes.c_int(0)
+        rc = _lib.lib().pi05_read_device_status(self.workspace.data_ptr(), ctypes.byref(v),
+                                                torch.cuda.current_stream(self.device).cuda_stream)
+        if rc not in (_lib.PI05_OK, 7):
+            raise _lib.Pi05Error("pi05_read_device_status", rc, _lib.last_error())
+        return v.value
