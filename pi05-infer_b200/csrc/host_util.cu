@@ -72,6 +72,28 @@ int make_tmap_f32_2d(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t 
   return make_tmap_2d(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, rows, cols, ld, box_rows, box_cols, swizzle128);
 }
 
+int make_tmap_16bit_4d(CUtensorMap* tm, const void* base, const uint64_t* dims, const uint64_t* strides,
+                       uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) {
+    set_last_error("cuTensorMapEncodeTiled entry point unavailable");
+    return PI05_ERR_DRIVER;
+  }
+  cuuint32_t box[4] = {64, box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base),
+                  reinterpret_cast<const cuuint64_t*>(dims), reinterpret_cast<const cuuint64_t*>(strides), box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("cuTensorMapEncodeTiled failed (%d): %llu x %llu x %llu x %llu, strides %llu %llu %llu", (int)r,
+                   (unsigned long long)dims[0], (unsigned long long)dims[1], (unsigned long long)dims[2],
+                   (unsigned long long)dims[3], (unsigned long long)strides[0], (unsigned long long)strides[1],
+                   (unsigned long long)strides[2]);
+    return PI05_ERR_TMAP;
+  }
+  return PI05_OK;
+}
+
 static std::atomic<long long> g_launches{0};
 
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }

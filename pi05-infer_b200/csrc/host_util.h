@@ -67,6 +67,11 @@ int make_tmap_bf16_2d(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t
 int make_tmap_f32_2d(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                      uint32_t box_rows, uint32_t box_cols, bool swizzle128);
 
+// 4-D map of 16-bit elements, dims and byte strides innermost first (stride of dims[0]
+// implied); boxes of 64 columns x `box_rows` x 1 x 1, 128-byte swizzle, zeros outside.
+int make_tmap_16bit_4d(CUtensorMap* tm, const void* base, const uint64_t* dims, const uint64_t* strides,
+                       uint32_t box_rows);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Buffer set by pi05_debug_set_trace (per-CTA GEMM timestamps), or nullptr.

@@ -132,7 +132,7 @@ __device__ __forceinline__ void rotate_unit(const T* src, T* dst, int unit, int 
 // ---- division by a number known at launch (n < 2^31) ------------------------
 struct FastDiv {
   uint32_t mul, shift, d;
-  __host__ FastDiv() = default;
+  FastDiv() = default;
   __host__ explicit FastDiv(uint32_t div) : d(div) {
     shift = 0;
     while ((1ull << shift) < div) ++shift;

@@ -10,16 +10,21 @@
 // pairs, laid end to end, are dealt out in equal contiguous shares to a fixed grid, so
 // lengths may differ at will and the host need not know them.  A share that covers a
 // whole pair writes its result; pairs cut between CTAs leave fp32 partials (o, m, l)
-// that the finish kernel adds up in order.
+// that the join kernel adds up in order.
 //
-// A warp takes 16 rows at a time, in a cp.async ring of its own (no block barrier in
-// the loop).  The products run on the tensor cores with the rows as M:  S^T = K q^T
-// (16 rows x 8 heads), then O^T += V^T P^T, where the probabilities pass from one
-// fragment layout to the other by a matrix transpose in registers; with the heads as
-// N = 8, half as many products and accumulators as with 16 padded query rows.  The
-// probabilities enter the second product in the cache's 16-bit type (2^-9 relative for
-// bf16, the size of the output's own rounding); m, l and o stay fp32, l sums the
-// unrounded ones.
+// A warp takes 16 rows at a time, brought by TMA into a ring of its own (no block barrier
+// in the loop), and its copies run ahead of its products across the borders of pairs.  The
+// products run on the tensor cores with the rows as M:  S^T = K q^T (16 rows x 8 heads),
+// then O^T += V^T P^T, where the probabilities pass from one fragment layout to the other
+// by a matrix transpose in registers; with the heads as N = 8, half as many products and
+// accumulators as with 16 padded query rows.  The probabilities enter the second product
+// in the cache's 16-bit type (2^-9 relative for bf16, the size of the output's own
+// rounding); m, l and o stay fp32, l sums the unrounded ones.
+//
+// Measured: 2 x 131072 rows, 32 / 8 heads of 128: 157 us = 6.8 TB/s + 5 us for the join.
+// The same with 16-byte cp.async copies through registers' addresses: 190 us (430
+// instructions a tile, and 8 warps an SM are too few to hide them); with a bulk copy for
+// each row, issued one by one: 174 us with 12 warps, 206 us with 8.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -31,7 +36,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kWarpRows = 16;
 constexpr int kBlockRows = kWarps * kWarpRows;
-constexpr int kStages = 3;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 struct AttnParams {
@@ -44,28 +48,27 @@ struct AttnParams {
   int valid_rows;
   int q_heads, group, parts;  // query heads per key-value head, cut into `parts` of at most 8 NT heads
   float scale_log2;
-  int track, n_ctas;
+  int track, box_rows;
   // scratch
   float* part_o;    // [2 n_ctas][8 NT][dim]
   float2* part_ml;  // [2 n_ctas][8 NT]
   int2* row_info;   // [rows]: first partial slot (-1: done), last CTA
   float* row_lse;   // [rows][8 NT] log2 units, of the rows done in one piece
-  float* scores;    // [rows][capacity][8 NT], log2 units (track)
+  float* scores;    // [rows][capacity][score_pitch], log2 units (track)
+  int score_pitch;  // heads of a part, up to a power of two from 2 on
 };
 
 template <class T>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, const uint32_t* b);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, const uint32_t* a, const uint32_t* b) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 template <>
 __device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, const uint32_t* b) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
@@ -85,282 +88,140 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// 16 bytes through L2, or 16 zero bytes (nothing is read then).
-__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, int z,
+                                            int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
 }
 
-template <int DP>
+// A tile of 16 rows: boxes of 64 columns, 16 rows of 128 bytes each, whose 16-byte chunk
+// c of row r lies at chunk c ^ (r & 7) (the 128-byte swizzle): ldmatrix without conflicts.
+template <int DP, int NT>
 struct Tile {
-  static constexpr int kPitch = DP * 2 + 16;  // bytes; an odd number of 16-byte chunks: ldmatrix without conflicts
-  static constexpr int kBytes = kWarpRows * kPitch;
-  static constexpr int kChunks = DP / 8;                    // 16-byte chunks of a row
-  static constexpr int kRowsAtOnce = 32 / kChunks;          // rows one copy instruction of a warp covers
-  static constexpr int kSmem = kWarps * kStages * 2 * kBytes;
+  static constexpr int kBox = kWarpRows * 128;
+  static constexpr int kBytes = DP / 64 * kBox;
+  static constexpr int kStages = DP == 256 && NT == 1 ? 3 : 2;
+  static constexpr int kRing = kWarps * kStages * 2 * kBytes;
+  static constexpr int kSlot = (DP / 16 * NT * 4 + NT * 4) * 32 * 4;  // a warp's o, m and l, at a segment's end
+  static constexpr int kSmem = 1024 + kRing + 2 * kSlot;
+  // CTAs on an SM: as many as shared memory and the accumulators' registers leave room for.
+  static constexpr int kPerSM = DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 1;
+  static_assert(kPerSM * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
-// Where a warp's lane r (< 16) finds row r of a 16-row tile (line -1: the row does not
-// count), asked for ahead of time, so that the latency is not waited for.
-struct RowRef {
-  int page, line;
-};
-
-template <class T, int DP, int NT, bool FULL>
+// One contiguous run of blocks of one (sequence, key-value head, part of its query heads).
 struct Segment {
-  using L = Tile<DP>;
-  const AttnParams& p;
-  int b, kvh, heads;  // heads of this part
-  const char *k, *v;
-  int len, lane, w;
-  int d;
-  uint32_t ring;  // this warp's shared memory
+  int b, row, kvh, part, len, tile0, n;
+  bool whole;
+};
 
-  __device__ __forceinline__ RowRef look_up(int row0) const {
-    RowRef r{0, -1};
-    const int row = row0 + lane;
-    if (lane < kWarpRows && row < len) {
-      r.page = p.c.page_of(b, row, &r.line);
-      if (row < p.valid_rows && p.valid[b * p.valid_pitch + row] == 0) r.line = -1;
-    }
-    return r;
-  }
+// Walks through a CTA's share of the blocks, segment by segment.
+struct Walk {
+  int b;
+  long long base, at, end;  // first block of sequence b; the next block; the share's end
 
-  // Copies a tile's K and V, zeros in the place of rows that do not count; returns a
-  // bit for each row that does.
-  __device__ __forceinline__ uint32_t fetch(const RowRef& ref, int stage) const {
-    long long off = -1;
-    if (ref.line >= 0) {
-      if (p.c.real(ref.page)) off = (long long)p.c.row_at(ref.page, kvh, ref.line);
-      else report_status(p.c.status, PI05_DEV_BAD_INDEX);
+  __device__ __forceinline__ bool next(const AttnParams& p, Segment& s) {
+    if (at >= end) return false;
+    const int per = p.c.heads * p.parts;
+    int blocks;
+    while (true) {
+      s.len = p.c.rows(b);
+      blocks = (s.len + kBlockRows - 1) / kBlockRows;
+      if (at < base + (long long)blocks * per) break;
+      base += (long long)blocks * per;
+      ++b;
     }
-    const int chunk = lane % L::kChunks;
-    const int have = FULL ? DP / 8 : d / 8, used = FULL ? DP / 8 : ((d + 15) / 16) * 2;
-    const uint32_t dst = ring + stage * 2 * L::kBytes + chunk * 16;
-#pragma unroll
-    for (int i = 0; i < kWarpRows / L::kRowsAtOnce; ++i) {
-      const int row = i * L::kRowsAtOnce + lane / L::kChunks;
-      const long long o = __shfl_sync(~0u, off, row);
-      if (FULL || chunk < used) {
-        const bool read = o >= 0 && (FULL || chunk < have);
-        const long long at = read ? o + chunk * 16 : 0;
-        cp_async_16_or_zero(dst + row * L::kPitch, k + at, read);
-        cp_async_16_or_zero(dst + L::kBytes + row * L::kPitch, v + at, read);
-      }
-    }
-    return __ballot_sync(~0u, off >= 0);
+    const int pair = (int)((at - base) / blocks);
+    s.b = b;
+    s.row = b * per + pair;
+    s.kvh = pair / p.parts;
+    s.part = pair - s.kvh * p.parts;
+    s.tile0 = (int)((at - base) - (long long)pair * blocks);
+    s.n = (int)min((long long)(blocks - s.tile0), end - at);
+    s.whole = s.n == blocks;
+    at += s.n;
+    return true;
   }
 };
 
-// One contiguous run [tile0, tile1) of the blocks of one (sequence, head, part).
-template <class T, int DP, int NT, bool FULL>
-__device__ void run_segment(const AttnParams& p, char* smem, int b, int row, int kvh, int part, int len, int tile0,
-                            int tile1, int slot, bool whole) {
-  using L = Tile<DP>;
-  constexpr int H = 8 * NT;
-  constexpr int KS = DP / 16;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int d = FULL ? DP : p.c.dim, steps = FULL ? KS : (d + 15) / 16;
-  const int heads = min(H, p.group - part * H), head0 = kvh * p.group + part * H;
-  Segment<T, DP, NT, FULL> s{p, b, kvh, heads, p.c.k, p.c.v, len, lane, w, d,
-                             smem_u32(smem) + w * kStages * 2 * L::kBytes};
-  // This warp's tiles: row0 = (tile0 * 4 + w + 4 j) * 16.
-  const int n_tiles = tile1 - tile0;
-  auto row0_of = [&](int j) { return ((tile0 + j) * kWarps + w) * kWarpRows; };
+// A row of the cache as lane r < 16 of a warp knows row r of a tile; asked for one tile
+// ahead of its copy, so that the table's latency is not waited for.
+struct Ref {
+  int page, line, kvh;
+  bool tile, counts;  // there is a tile; this row counts
+};
 
-  uint32_t live[kStages];  // of the tiles in flight, the oldest first
-  RowRef ref = s.look_up(n_tiles > 0 ? row0_of(0) : len);
-#pragma unroll
-  for (int j = 0; j < kStages - 1; ++j) {
-    const RowRef now = ref;
-    ref = s.look_up(j + 1 < n_tiles ? row0_of(j + 1) : len);
-    live[j] = j < n_tiles ? s.fetch(now, j) : 0u;
-    cp_async_commit();
+__device__ __forceinline__ Ref look_up(const AttnParams& p, const Segment& s, int row0, int lane) {
+  Ref r{0, 0, s.kvh, true, false};
+  const int row = row0 + (lane & 15);
+  if (row < s.len) {
+    r.page = p.c.page_of(s.b, row, &r.line);
+    r.counts = row >= p.valid_rows || p.valid[s.b * p.valid_pitch + row] != 0;
   }
+  return r;
+}
 
-  // q^T fragments: lane holds head lane / 4, values 2 (lane % 4) + {0, 1, 8, 9} of each step.
-  uint32_t qf[KS][NT][2];
-  {
-    const int n = lane >> 2, c = 2 * (lane & 3);
+// Starts the copies of a tile's K and V by TMA, `p.box_rows` rows of 64 columns at a time
+// (the largest power of two that divides the page size, so that a box lies in one page);
+// a lane for each group of rows.  Returns a bit for each row that counts.
+template <int DP, int NT>
+__device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+                                          const Ref& ref, uint64_t* bar, uint32_t dst, int lane) {
+  using L = Tile<DP, NT>;
+  const bool real = p.c.real(ref.page);
+  if (ref.counts && !real) report_status(p.c.status, PI05_DEV_BAD_INDEX);
+  const uint32_t mask = __ballot_sync(~0u, ref.counts && real) & 0xffff;
+  const bool mine = lane < kWarpRows && (lane & (p.box_rows - 1)) == 0 && (mask >> lane & ((1u << p.box_rows) - 1)) != 0;
+  const int groups = __popc(__ballot_sync(~0u, mine));
+  if (lane == 0) mbar_arrive_expect_tx(bar, groups * p.box_rows * 128 * (DP / 64) * 2);
+  __syncwarp();
+  if (mine) {
+    const uint32_t to = dst + lane * 128, at = smem_u32(bar);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int h = nt * 8 + n;
-        const T* q = static_cast<const T*>(p.q) + b * p.qt + (long long)(head0 + h) * p.qh;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int at = ks * 16 + c + 8 * i;
-          qf[ks][nt][i] = h < heads && at < d ? *reinterpret_cast<const uint32_t*>(q + at) : 0u;
-        }
-      }
-  }
-
-  float o[KS][NT][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[ks][nt][i] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-
-  const uint32_t k_lane = (lane & 15) * L::kPitch + (lane >> 4) * 16;
-  const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * L::kPitch + ((lane >> 3) & 1) * 16;
-  for (int j = 0; j < n_tiles; ++j) {
-    const int row0 = row0_of(j);
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    {  // refill the slot read in the last turn
-      const RowRef now = ref;
-      const int next = j + kStages - 1;
-      ref = s.look_up(next + 1 < n_tiles ? row0_of(next + 1) : len);
-      live[kStages - 1] = next < n_tiles ? s.fetch(now, next % kStages) : 0u;
-      cp_async_commit();
-    }
-    // Which of this lane's two rows count (row lane / 4 and that plus 8).
-    const bool live0 = live[0] >> (lane >> 2) & 1, live1 = live[0] >> (lane >> 2) >> 8 & 1;
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) live[i] = live[i + 1];
-    const uint32_t k_at = s.ring + (j % kStages) * 2 * L::kBytes + k_lane;
-    const uint32_t v_at = s.ring + (j % kStages) * 2 * L::kBytes + L::kBytes + v_lane;
-    float x[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      if (FULL || ks < steps) {
-        uint32_t a[4];
-        ldsm4(a, k_at + ks * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<T>(x[nt], a, qf[ks][nt]);
-      }
-    }
-    const int r0 = row0 + (lane >> 2), r1 = r0 + 8;
-    uint32_t pf[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float* xs = x[nt];
-      xs[0] = live0 ? xs[0] * p.scale_log2 : -INFINITY;
-      xs[1] = live0 ? xs[1] * p.scale_log2 : -INFINITY;
-      xs[2] = live1 ? xs[2] * p.scale_log2 : -INFINITY;
-      xs[3] = live1 ? xs[3] * p.scale_log2 : -INFINITY;
-      if (p.track) {
-        const int h = nt * 8 + 2 * (lane & 3);
-        float* dst = p.scores + ((size_t)row * p.c.capacity) * H + h;
-        if (r0 < len) *reinterpret_cast<float2*>(dst + (size_t)r0 * H) = make_float2(xs[0], xs[1]);
-        if (r1 < len) *reinterpret_cast<float2*>(dst + (size_t)r1 * H) = make_float2(xs[2], xs[3]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float top = fmaxf(xs[i], xs[i + 2]);
-#pragma unroll
-        for (int sft = 4; sft < 32; sft <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, sft));
-        top = fmaxf(top, m[nt][i]);
-        const float base = top == -INFINITY ? 0.f : top;
-        const float keep = ex2_approx(m[nt][i] - base);
-        m[nt][i] = top;
-        xs[i] = ex2_approx(xs[i] - base);
-        xs[i + 2] = ex2_approx(xs[i + 2] - base);
-        l[nt][i] = l[nt][i] * keep + xs[i] + xs[i + 2];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          o[ks][nt][i] *= keep;
-          o[ks][nt][i + 2] *= keep;
-        }
-      }
-      pf[nt][0] = transpose8x8(pack2<T>(xs[0], xs[1]));
-      pf[nt][1] = transpose8x8(pack2<T>(xs[2], xs[3]));
-    }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      if (FULL || ks < steps) {
-        uint32_t a[4];
-        ldsm4_trans(a, v_at + ks * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[ks][nt], a, pf[nt]);
-      }
+    for (int i = 0; i < DP / 64; ++i) {
+      tma_load_4d(to + i * L::kBox, tm_k, at, i * 64, ref.line, ref.kvh, ref.page);
+      tma_load_4d(to + L::kBytes + i * L::kBox, tm_v, at, i * 64, ref.line, ref.kvh, ref.page);
     }
   }
-  cp_async_wait<0>();
-  __syncthreads();  // the rings are free: the warps' results meet there
-
-  float* so = reinterpret_cast<float*>(smem);                      // [kWarps][H][DP]
-  float2* sml = reinterpret_cast<float2*>(so + kWarps * H * DP);   // [kWarps][H]
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum = l[nt][i];
-#pragma unroll
-      for (int sft = 4; sft < 32; sft <<= 1) sum += __shfl_xor_sync(~0u, sum, sft);
-      const int h = nt * 8 + 2 * (lane & 3) + i;
-      if (lane < 4) sml[w * H + h] = make_float2(m[nt][i], sum);
-      float* dst = so + (w * H + h) * DP + (lane >> 2);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        dst[ks * 16] = o[ks][nt][i];
-        dst[ks * 16 + 8] = o[ks][nt][i + 2];
-      }
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * DP; i += kThreads) {
-    const int h = i / DP, x = i - h * DP;
-    float top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) top = fmaxf(top, sml[j * H + h].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) {
-      const float f = ex2_approx(sml[j * H + h].x - base);
-      sum += sml[j * H + h].y * f;
-      acc += so[(j * H + h) * DP + x] * f;
-    }
-    if (whole) {
-      // A sum of 0 has no row that counts; NaN stays NaN.
-      if (x < d)
-        static_cast<T*>(p.out)[((size_t)b * p.q_heads + head0 + h) * d + x] =
-            from_f32<T>(sum == 0.f ? 0.f : acc / sum);
-      if (x == 0) {
-        const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
-        if (p.lse != nullptr) p.lse[(size_t)b * p.q_heads + head0 + h] = lse2 * kLn2;
-        if (p.track) p.row_lse[(size_t)row * H + h] = lse2;
-      }
-    } else {
-      if (x < d) p.part_o[((size_t)slot * H + h) * d + x] = acc;
-      if (x == 0) p.part_ml[(size_t)slot * H + h] = make_float2(top, sum);
-    }
-  }
-  __syncthreads();  // before the rings fill again
+  return mask;
 }
 
 template <class T, int DP, int NT, bool FULL>
-__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnParams p) {
-  extern __shared__ __align__(16) char smem[];
-  __shared__ long long sh_sum[kThreads / 32];
+__global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
+    paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap tm_k,
+                           const __grid_constant__ CUtensorMap tm_v) {
+  using L = Tile<DP, NT>;
+  constexpr int H = 8 * NT, KS = DP / 16, S = L::kStages;
+  extern __shared__ char smem_raw[];
+  __shared__ long long sh_sum[kWarps];
   __shared__ long long sh_base;
   __shared__ int sh_b;
+  __shared__ uint64_t all_bars[kWarps * S];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (tid == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  if (tid < kWarps * S) mbar_init(&all_bars[tid], 1);
+  fence_mbar_init();
   pdl_wait();
   pdl_launch_dependents();
-  const int per_block = p.c.heads * p.parts, tid = threadIdx.x;
+
   // All blocks there are, then the sequence that this CTA's share begins in.
+  const int per_block = p.c.heads * p.parts;
   long long mine = 0;
   for (int b = tid; b < p.c.batch; b += kThreads) {
     mine += (p.c.rows(b) + kBlockRows - 1) / kBlockRows;
     if (blockIdx.x == 0 && p.c.rows(b) != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
   }
   for (int sft = 16; sft > 0; sft >>= 1) mine += __shfl_xor_sync(~0u, mine, sft);
-  if ((tid & 31) == 0) sh_sum[tid >> 5] = mine;
+  if (lane == 0) sh_sum[w] = mine;
   __syncthreads();
   long long total = 0;
-  for (int i = 0; i < kThreads / 32; ++i) total += sh_sum[i];
+  for (int i = 0; i < kWarps; ++i) total += sh_sum[i];
   total *= per_block;
   const long long n = min((long long)gridDim.x, total), cta = blockIdx.x;
   if (cta >= n) return;
@@ -372,14 +233,14 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnPar
     long long incl = own;
     for (int sft = 1; sft < 32; sft <<= 1) {
       const long long u = __shfl_up_sync(~0u, incl, sft);
-      if ((tid & 31) >= sft) incl += u;
+      if (lane >= sft) incl += u;
     }
     __syncthreads();
-    if ((tid & 31) == 31) sh_sum[tid >> 5] = incl;
+    if (lane == 31) sh_sum[w] = incl;
     __syncthreads();
-    for (int i = 0; i < (tid >> 5); ++i) incl += sh_sum[i];
+    for (int i = 0; i < w; ++i) incl += sh_sum[i];
     incl += before;
-    for (int i = 0; i < kThreads / 32; ++i) before += sh_sum[i];
+    for (int i = 0; i < kWarps; ++i) before += sh_sum[i];
     if (incl - own <= lo && lo < incl) {
       sh_b = b;
       sh_base = incl - own;
@@ -387,109 +248,421 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnPar
     if (before > lo) break;
   }
   __syncthreads();
-  int b = sh_b;
-  long long base = sh_base, at = lo;
-  while (at < hi) {
-    const int len = p.c.rows(b), blocks = (len + kBlockRows - 1) / kBlockRows;
-    if (at >= base + (long long)blocks * per_block) {
-      base += (long long)blocks * per_block;
-      ++b;
-      continue;
+
+  const uint32_t base_addr = (smem_u32(smem_raw) + 1023) & ~1023u;  // swizzled boxes start at multiples of 1024
+  const uint32_t ring = base_addr + w * S * 2 * L::kBytes;
+  float* slots = reinterpret_cast<float*>(smem_raw + (base_addr - smem_u32(smem_raw)) + L::kRing);
+  uint64_t* bars = all_bars + w * S;
+  const int d = FULL ? DP : p.c.dim, steps = FULL ? KS : (d + 15) / 16;
+
+  // The warp's copies run ahead of its products, across the segments' borders.
+  Walk ahead{sh_b, sh_base, lo, hi}, walk = ahead;
+  Segment fs;
+  bool more = ahead.next(p, fs);
+  int fj = 0;
+  auto next_ref = [&]() {
+    if (more && fj == fs.n) {
+      more = ahead.next(p, fs);
+      fj = 0;
     }
-    const int pair = (int)((at - base) / blocks);  // head, part
-    const int tile0 = (int)((at - base) - (long long)pair * blocks);
-    const int tile1 = (int)min((long long)blocks, tile0 + (hi - at));
-    const int row = b * per_block + pair;
-    const bool whole = tile0 == 0 && tile1 == blocks;
-    const int slot = 2 * (int)cta + (at == lo ? 0 : 1);
-    if (tile0 == 0 && tid == 0) {
-      const long long end = base + (long long)pair * blocks + blocks;  // the CTA that has the row's last block
-      p.row_info[row] = whole ? make_int2(-1, -1) : make_int2(slot, (int)((end * n - 1) / total));
+    if (!more) return Ref{0, 0, 0, false, false};
+    return look_up(p, fs, ((fs.tile0 + fj++) * kWarps + w) * kWarpRows, lane);
+  };
+  uint32_t live[S];  // rows that count of the tiles in flight, the oldest first
+  Ref ref = next_ref();
+#pragma unroll
+  for (int j = 0; j < S - 1; ++j) {
+    const Ref now = ref;
+    ref = next_ref();
+    live[j] = now.tile ? fetch<DP, NT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane) : 0u;
+  }
+  int stage = 0;
+  uint32_t phase = 0;
+  bool broken = false;  // a wait ran out: this warp reads no more
+
+  // Chunk 2 ks + c of row r lies at 128 r + 16 ((2 ks + c) ^ (r & 7)) of its box.
+  const uint32_t k_lane = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4) + L::kBytes;
+  auto step_at = [](uint32_t at, int ks) { return (at ^ ((ks & 3) << 5)) + (ks >> 2) * L::kBox; };
+
+  Segment s;
+  while (true) {
+    const bool first = walk.at == lo;
+    if (!walk.next(p, s)) break;
+    const int heads = min(H, p.group - s.part * H), head0 = s.kvh * p.group + s.part * H;
+    const int slot = 2 * (int)cta + (first ? 0 : 1);
+    if (s.tile0 == 0 && tid == 0) {
+      // the row's last block, and the CTA that has it
+      const long long end = walk.at - s.n + (s.len + kBlockRows - 1) / kBlockRows;
+      p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)((end * n - 1) / total));
     }
-    run_segment<T, DP, NT, FULL>(p, smem, b, row, pair / p.parts, pair % p.parts, len, tile0, tile1, slot, whole);
-    at += tile1 - tile0;
+    // q^T fragments: lane holds head lane / 4, values 2 (lane % 4) + {0, 1, 8, 9} of each step.
+    uint32_t qf[KS][NT][2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int h = nt * 8 + (lane >> 2);
+        const T* q = static_cast<const T*>(p.q) + s.b * p.qt + (long long)(head0 + h) * p.qh;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int at = ks * 16 + 2 * (lane & 3) + 8 * i;
+          qf[ks][nt][i] = h < heads && at < d ? *reinterpret_cast<const uint32_t*>(q + at) : 0u;
+        }
+      }
+
+    float o[KS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[ks][nt][i] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    for (int j = 0; j < s.n && !broken; ++j) {
+      if (__any_sync(~0u, !mbar_wait(bars + stage, phase))) {
+        report_status(p.c.status, PI05_DEV_TIMEOUT_PRODUCER);
+        broken = true;
+        break;
+      }
+      {  // refill the stage read in the last turn
+        const Ref now = ref;
+        ref = next_ref();
+        const int to = stage == 0 ? S - 1 : stage - 1;
+        live[S - 1] = now.tile ? fetch<DP, NT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane) : 0u;
+      }
+      const uint32_t tile = ring + stage * 2 * L::kBytes, rows = live[0];
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
+#pragma unroll
+      for (int i = 0; i < S - 1; ++i) live[i] = live[i + 1];
+      // Which of this lane's two rows count (row lane / 4 and that plus 8).
+      const bool live0 = rows >> (lane >> 2) & 1, live1 = rows >> (lane >> 2) >> 8 & 1;
+
+      // Fragments by the batch, ahead of the products that take them; two chains of sums.
+      // What a row that does not count holds may be anything, and 0 times that has to be 0:
+      // its values are cut out of the V fragments (two rows to a register).
+      const uint32_t r2 = rows >> (2 * (lane & 3));
+      const uint32_t cut0 = (r2 & 1 ? 0xffffu : 0u) | (r2 & 2 ? 0xffff0000u : 0u);
+      const uint32_t cut1 = (r2 & 0x100 ? 0xffffu : 0u) | (r2 & 0x200 ? 0xffff0000u : 0u);
+      auto load_v = [&](uint32_t* a, int ks) {
+        ldsm4_trans(a, step_at(tile + v_lane, ks));
+        if (rows != 0xffff) {
+          a[0] &= cut0;
+          a[1] &= cut0;
+          a[2] &= cut1;
+          a[3] &= cut1;
+        }
+      };
+      constexpr int B = KS < 8 ? KS : NT == 1 ? 8 : 4;
+      float x[NT][4], x2[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[nt][i] = x2[nt][i] = 0.f;
+#pragma unroll
+      for (int k0 = 0; k0 < KS; k0 += B) {
+        uint32_t a[B][4];
+#pragma unroll
+        for (int ks = 0; ks < B; ++ks)
+          if (FULL || k0 + ks < steps) ldsm4(a[ks], step_at(tile + k_lane, k0 + ks));
+#pragma unroll
+        for (int ks = 0; ks < B; ++ks)
+          if (FULL || k0 + ks < steps) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(ks & 1 ? x2[nt] : x[nt], a[ks], qf[k0 + ks][nt]);
+          }
+      }
+      uint32_t va[B][4];
+#pragma unroll
+      for (int ks = 0; ks < B; ++ks)
+        if (FULL || ks < steps) load_v(va[ks], ks);
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float* xs = x[nt];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xs[i] = (i < 2 ? live0 : live1) ? (xs[i] + x2[nt][i]) * p.scale_log2 : -INFINITY;
+        if (p.track) {
+          const int h = nt * 8 + 2 * (lane & 3), r0 = ((s.tile0 + j) * kWarps + w) * kWarpRows + (lane >> 2);
+          float* dst = p.scores + ((size_t)s.row * p.c.capacity + r0) * p.score_pitch + h;
+          if (r0 < s.len && h < heads) *reinterpret_cast<float2*>(dst) = make_float2(xs[0], xs[1]);
+          if (r0 + 8 < s.len && h < heads)
+            *reinterpret_cast<float2*>(dst + 8 * (size_t)p.score_pitch) = make_float2(xs[2], xs[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = fmaxf(xs[i], xs[i + 2]);
+#pragma unroll
+          for (int sft = 4; sft < 32; sft <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, sft));
+          top = fmaxf(top, m[nt][i]);
+          const float base = top == -INFINITY ? 0.f : top;
+          const float keep = ex2_approx(m[nt][i] - base);
+          m[nt][i] = top;
+          xs[i] = ex2_approx(xs[i] - base);
+          xs[i + 2] = ex2_approx(xs[i + 2] - base);
+          l[nt][i] = l[nt][i] * keep + xs[i] + xs[i + 2];
+          if (__any_sync(~0u, keep != 1.f)) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              o[ks][nt][i] *= keep;
+              o[ks][nt][i + 2] *= keep;
+            }
+          }
+        }
+        pf[nt][0] = transpose8x8(pack2<T>(xs[0], xs[1]));
+        pf[nt][1] = transpose8x8(pack2<T>(xs[2], xs[3]));
+      }
+#pragma unroll
+      for (int k0 = 0; k0 < KS; k0 += B) {
+        if (k0 > 0) {
+#pragma unroll
+          for (int ks = 0; ks < B; ++ks)
+            if (FULL || k0 + ks < steps) load_v(va[ks], k0 + ks);
+        }
+#pragma unroll
+        for (int ks = 0; ks < B; ++ks)
+          if (FULL || k0 + ks < steps) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[k0 + ks][nt], va[ks], pf[nt]);
+          }
+      }
+    }
+
+    // The four warps' results, joined two by two in a fixed order: warps 2 and 3 hand theirs
+    // to 0 and 1, then 1 to 0, fragment by fragment.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int sft = 4; sft < 32; sft <<= 1) l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], sft);
+    auto give = [&](int i_slot) {
+      float* to = slots + i_slot * (L::kSlot / 4) + lane;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          to[(nt * 4 + i) * 32] = m[nt][i];
+          to[(nt * 4 + 2 + i) * 32] = l[nt][i];
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[(NT * 4 + (ks * NT + nt) * 4 + i) * 32] = o[ks][nt][i];
+      }
+    };
+    auto take = [&](int i_slot) {
+      const float* from = slots + i_slot * (L::kSlot / 4) + lane;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float m2 = from[(nt * 4 + i) * 32], top = fmaxf(m[nt][i], m2), base = top == -INFINITY ? 0.f : top;
+          const float f = ex2_approx(m[nt][i] - base), f2 = ex2_approx(m2 - base);
+          m[nt][i] = top;
+          l[nt][i] = l[nt][i] * f + from[(nt * 4 + 2 + i) * 32] * f2;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int k = i; k < 4; k += 2)
+              o[ks][nt][k] = o[ks][nt][k] * f + from[(NT * 4 + (ks * NT + nt) * 4 + k) * 32] * f2;
+        }
+    };
+    __syncthreads();  // warp 0 is done with the last segment's
+    if (w >= 2) give(w - 2);
+    __syncthreads();
+    if (w < 2) take(w);
+    if (w == 1) give(1);
+    __syncthreads();
+    if (w == 0) {
+      take(1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int h = nt * 8 + 2 * (lane & 3) + i;
+          if (h >= heads) continue;
+          const float sum = l[nt][i];
+          // A sum of 0 has no row that counts; NaN stays NaN.
+          const float lse2 = sum == 0.f ? -INFINITY : m[nt][i] + log2f(sum), scale = sum == 0.f ? 0.f : 1.f / sum;
+          T* out = static_cast<T*>(p.out) + ((size_t)s.b * p.q_heads + head0 + h) * d;
+          float* part = p.part_o + ((size_t)slot * H + h) * d;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int x = ks * 16 + k * 8 + (lane >> 2);
+              if (!FULL && x >= d) continue;
+              const float v = o[ks][nt][i + 2 * k];
+              if (s.whole) out[x] = from_f32<T>(sum == 0.f ? 0.f : v * scale);
+              else part[x] = v;
+            }
+          if (lane < 4) {
+            if (!s.whole) {
+              p.part_ml[(size_t)slot * H + h] = make_float2(m[nt][i], sum);
+            } else {
+              if (p.lse != nullptr) p.lse[(size_t)s.b * p.q_heads + head0 + h] = lse2 * kLn2;
+              if (p.track) p.row_lse[(size_t)s.row * H + h] = lse2;
+            }
+          }
+        }
+    }
   }
 }
 
-// Joins the partials of a row (blockIdx.y == 0), and adds its probabilities to the
-// cache's weights (blockIdx.y > 0).
-constexpr int kFinishThreads = 256;
-constexpr int kTrackRows = 1024;  // of the longest sequence there can be, for each CTA
+// Joins what was cut, a CTA for each (sequence, query head).  Every warp works out the
+// head's maximum and sum from the partials' (m, l), a lane for each; the partial outputs
+// are added by groups of dim / 4 threads, each taking every n-th, and then in group order.
+// (One thread per value, walking all partials one after the other, took 40 us for 19
+// partials: two loads from L2 at a time.)
+constexpr int kFinishThreads = 128;
 
-// log2 of the row's sum over everything, from its partials.
+struct Total {
+  float top, sum;  // log2 units
+  __device__ __forceinline__ float lse2() const { return sum == 0.f ? -INFINITY : top + log2f(sum); }
+};
+
+// A row's partials are the first's slot and the even ones after it, up to the last CTA's.
+__device__ __forceinline__ int partials(int2 info) { return info.y - (info.x >> 1) + 1; }
+__device__ __forceinline__ int slot_of(int2 info, int i) { return i == 0 ? info.x : ((info.x >> 1) + i) * 2; }
+
+// All lanes of a warp together.
 template <int H>
-__device__ __forceinline__ float joined(const AttnParams& p, int2 info, int h, float* top_out, float* sum_out) {
+__device__ __forceinline__ Total total_of(const AttnParams& p, int2 info, int h) {
+  const int n = partials(info), lane = threadIdx.x & 31;
   float top = -INFINITY, sum = 0.f;
-  for (int slot = info.x; slot <= 2 * info.y; slot = (slot | 1) + 1) {
-    const float2 ml = p.part_ml[(size_t)slot * H + h];
-    const float t = fmaxf(top, ml.x), base = t == -INFINITY ? 0.f : t;
-    sum = sum * ex2_approx(top - base) + ml.y * ex2_approx(ml.x - base);
-    top = t;
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[(size_t)slot_of(info, i) * H + h].x);
+  for (int sft = 16; sft > 0; sft >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, sft));
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int i = lane; i < n; i += 32) {
+    const float2 ml = p.part_ml[(size_t)slot_of(info, i) * H + h];
+    sum += ml.y * ex2_approx(ml.x - base);
   }
-  *top_out = top;
-  *sum_out = sum;
-  return sum == 0.f ? -INFINITY : top + log2f(sum);
+  for (int sft = 16; sft > 0; sft >>= 1) sum += __shfl_xor_sync(~0u, sum, sft);
+  return {top, sum};
 }
 
 template <class T, int H>
-__global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const AttnParams p) {
-  __shared__ float sh_lse[H];
+__global__ void __launch_bounds__(kFinishThreads) paged_join_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ float4 acc_of[kFinishThreads];
   pdl_wait();
   pdl_launch_dependents();
-  const int row = blockIdx.x, per = p.c.heads * p.parts, b = row / per, pair = row - b * per;
-  const int kvh = pair / p.parts, part = pair - kvh * p.parts;
-  const int heads = min(H, p.group - part * H), head0 = kvh * p.group + part * H, d = p.c.dim;
-  const int len = p.c.rows(b);
-  if (blockIdx.y == 0) {
-    if (len > 0 && p.row_info[row].x < 0) return;
-    const int2 info = len > 0 ? p.row_info[row] : make_int2(1, 0);  // no partial at all
-    for (int i = threadIdx.x; i < heads * d; i += kFinishThreads) {
-      const int h = i / d, x = i - h * d;
-      float top, sum, acc = 0.f;
-      const float lse2 = joined<H>(p, info, h, &top, &sum);
-      const float base = top == -INFINITY ? 0.f : top;
-      for (int slot = info.x; slot <= 2 * info.y; slot = (slot | 1) + 1)
-        acc += p.part_o[((size_t)slot * H + h) * d + x] * ex2_approx(p.part_ml[(size_t)slot * H + h].x - base);
-      static_cast<T*>(p.out)[((size_t)b * p.q_heads + head0) * d + i] = from_f32<T>(sum == 0.f ? 0.f : acc / sum);
-      if (x == 0 && p.lse != nullptr) p.lse[(size_t)b * p.q_heads + head0 + h] = lse2 * kLn2;
-    }
+  const int b = blockIdx.x / p.q_heads, head = blockIdx.x - b * p.q_heads;
+  const int kvh = head / p.group, in_group = head - kvh * p.group, part = in_group / H, h = in_group - part * H;
+  const int row = (b * p.c.heads + kvh) * p.parts + part, d = p.c.dim, quads = d / 4;
+  T* out = static_cast<T*>(p.out) + ((size_t)b * p.q_heads + head) * d;
+  if (p.c.rows(b) == 0) {  // nothing to attend to
+    for (int i = threadIdx.x; i < d; i += kFinishThreads) out[i] = from_f32<T>(0.f);
+    if (threadIdx.x == 0 && p.lse != nullptr) p.lse[(size_t)b * p.q_heads + head] = -INFINITY;
     return;
   }
-  // The first part's CTAs add up all parts, so that a weight has one writer.
-  if (part != 0) return;
-  float* weight = p.c.weight;
-  const int first = (blockIdx.y - 1) * kFinishThreads, step = (gridDim.y - 1) * kFinishThreads;
-  for (int r0 = first; r0 < len; r0 += step) {
-    const int r = r0 + threadIdx.x;
-    float add = 0.f;
-    for (int q = 0; q < p.parts; ++q) {
-      const int2 info = p.row_info[row + q];
-      const int here = min(H, p.group - q * H);
-      __syncthreads();
-      if (threadIdx.x < here) {
-        float top, sum;
-        sh_lse[threadIdx.x] = info.x < 0 ? p.row_lse[(size_t)(row + q) * H + threadIdx.x]
-                                         : joined<H>(p, info, threadIdx.x, &top, &sum);
-      }
-      __syncthreads();
-      if (r < len) {
-        const float* s = p.scores + ((size_t)(row + q) * p.c.capacity + r) * H;
-        for (int h = 0; h < here; ++h) add += s[h] == -INFINITY ? 0.f : ex2_approx(s[h] - sh_lse[h]);
+  const int2 info = p.row_info[row];
+  if (info.x < 0) return;  // done in one piece
+  const Total t = total_of<H>(p, info, h);
+  const float base = t.top == -INFINITY ? 0.f : t.top;
+  const int n = partials(info), groups = kFinishThreads / quads, g = threadIdx.x / quads, at = threadIdx.x - g * quads;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (g < groups) {
+#pragma unroll 4
+    for (int i = g; i < n; i += groups) {
+      const size_t slot = (size_t)slot_of(info, i) * H + h;
+      const float f = ex2_approx(p.part_ml[slot].x - base);
+      const float4 o = *reinterpret_cast<const float4*>(p.part_o + slot * d + at * 4);
+      acc.x += o.x * f;
+      acc.y += o.y * f;
+      acc.z += o.z * f;
+      acc.w += o.w * f;
+    }
+  }
+  acc_of[threadIdx.x] = acc;
+  __syncthreads();
+  for (int i = threadIdx.x; i < d; i += kFinishThreads) {
+    const float* v = reinterpret_cast<const float*>(acc_of) + i;
+    float x = 0.f;
+    for (int j = 0; j < groups; ++j) x += v[j * d];
+    out[i] = from_f32<T>(t.sum == 0.f ? 0.f : x / t.sum);
+  }
+  if (threadIdx.x == 0) {
+    if (p.lse != nullptr) p.lse[(size_t)b * p.q_heads + head] = t.lse2() * kLn2;
+    if (p.track) p.row_lse[(size_t)row * H + h] = t.lse2();
+  }
+}
+
+// Adds the probabilities to the cache's weights: R rows a thread of one (sequence,
+// key-value head), a power of two P of scores for each, all loads before the first use.
+// A kernel of its own, behind the join: where its CTAs worked the sums out for themselves,
+// that was most of their instructions (33 us with 1024 rows a CTA, 52 us with the loads in
+// front but fewer CTAs on an SM; 64 sequences of 17 to 8192 rows, 8 key-value heads, 4
+// query heads each).
+template <int P, int H>
+__global__ void __launch_bounds__(kFinishThreads) paged_track_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int R = P == 16 ? 2 : 4;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int b = blockIdx.x / p.c.heads, kvh = blockIdx.x - b * p.c.heads, len = p.c.rows(b);
+  const long long step = R * kFinishThreads;
+  for (long long r0 = blockIdx.y * step; r0 < len; r0 += gridDim.y * step) {
+    float* weight[R];
+    float was[R], add[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const long long r = r0 + i * kFinishThreads + threadIdx.x;
+      int line = 0;
+      const int page = r < len ? p.c.page_of(b, (int)r, &line) : -1;
+      weight[i] = p.c.real(page) ? p.c.weight + p.c.slot_at(page, kvh, line) : nullptr;
+      was[i] = weight[i] != nullptr ? *weight[i] : 0.f;
+      add[i] = 0.f;
+    }
+    for (int part = 0; part < p.parts; ++part) {
+      const int row = (int)blockIdx.x * p.parts + part, heads = min(H, p.group - part * H);
+      const float* from = p.scores + ((size_t)row * p.c.capacity + r0 + threadIdx.x) * P;
+      __align__(16) float s[R][P];
+      float lse[P];
+#pragma unroll
+      for (int h = 0; h < P; ++h) lse[h] = h < heads ? p.row_lse[(size_t)row * H + h] : 0.f;
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (weight[i] != nullptr) {
+          if constexpr (P == 2) {
+            *reinterpret_cast<float2*>(s[i]) = *reinterpret_cast<const float2*>(from + i * kFinishThreads * P);
+          } else {
+#pragma unroll
+            for (int h = 0; h < P; h += 4)
+              *reinterpret_cast<float4*>(s[i] + h) = *reinterpret_cast<const float4*>(from + i * kFinishThreads * P + h);
+          }
+        }
+#pragma unroll
+      for (int h = 0; h < P; ++h) {
+        // A head with no row at all: every score is -inf, and so is what is left of it.
+        const float from_top = lse[h] == -INFINITY ? 0.f : lse[h];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (h < heads) add[i] += ex2_approx(s[i][h] - from_top);
       }
     }
-    if (r < len) {
-      int line;
-      const int page = p.c.page_of(b, r, &line);
-      if (p.c.real(page)) weight[p.c.slot_at(page, kvh, line)] += add;
-    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (weight[i] != nullptr) *weight[i] = was[i] + add[i];
   }
 }
 
 // ---- host ----------------------------------------------------------------------
 struct Plan {
-  int nt, parts, dp, ctas, rows;
+  int nt, parts, dp, ctas, rows, score_pitch;
   size_t part_o, part_ml, row_info, row_lse, scores, bytes;
 };
+
+int per_sm(int dp, int nt) {
+  if (dp == 64) return nt == 1 ? Tile<64, 1>::kPerSM : Tile<64, 2>::kPerSM;
+  if (dp == 128) return nt == 1 ? Tile<128, 1>::kPerSM : Tile<128, 2>::kPerSM;
+  return nt == 1 ? Tile<256, 1>::kPerSM : Tile<256, 2>::kPerSM;
+}
 
 Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   Plan s;
@@ -500,8 +673,7 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   s.rows = c->batch * c->n_kv_heads * s.parts;
   const long long capacity = (long long)c->pages_per_seq * c->page_size;
   const long long blocks = (capacity + kBlockRows - 1) / kBlockRows * s.rows;
-  const int per_sm = s.dp == 64 ? 4 : s.dp == 128 ? 2 : 1;
-  s.ctas = (int)std::min<long long>(blocks, (long long)kSMs * per_sm);
+  s.ctas = (int)std::min<long long>(blocks, (long long)kSMs * per_sm(s.dp, s.nt));
   const size_t h = 8 * s.nt;
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -513,15 +685,16 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   s.part_ml = take(2 * (size_t)s.ctas * h * 8);
   s.row_info = take((size_t)s.rows * 8);
   s.row_lse = take((size_t)s.rows * h * 4);
-  s.scores = take(track ? (size_t)s.rows * capacity * h * 4 : 0);
+  s.score_pitch = 2;
+  while (s.score_pitch < std::min((int)h, group)) s.score_pitch *= 2;
+  s.scores = take(track ? (size_t)s.rows * capacity * s.score_pitch * 4 : 0);
   s.bytes = at;
   return s;
 }
 
 template <class T, int DP, int NT, bool FULL>
-int launch(const AttnParams& p, const Plan& s, cudaStream_t st) {
-  constexpr int kJoin = kWarps * 8 * NT * (DP * 4 + 8);
-  constexpr int kSmem = Tile<DP>::kSmem > kJoin ? Tile<DP>::kSmem : kJoin;
+int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
+  constexpr int kSmem = Tile<DP, NT>::kSmem;
   static_assert(kSmem <= 227 * 1024, "shared memory");
   auto kernel = paged_attention_kernel<T, DP, NT, FULL>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
@@ -529,24 +702,32 @@ int launch(const AttnParams& p, const Plan& s, cudaStream_t st) {
     set_last_error("paged_attention: %s", cudaGetErrorString(e));
     return PI05_ERR_LAUNCH;
   }
-  int rc = launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), kSmem, st, pdl_enabled(), p);
+  int rc = launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), kSmem, st, pdl_enabled(), p, tm[0], tm[1]);
   if (rc) return rc;
-  const int chunks = p.track ? std::min((p.c.capacity + kTrackRows - 1) / kTrackRows, 1024) : 0;
-  return launch_pdl(paged_finish_kernel<T, 8 * NT>, dim3(s.rows, 1 + chunks), dim3(kFinishThreads), 0, st,
-                    pdl_enabled(), p);
+  rc = launch_pdl(paged_join_kernel<T, 8 * NT>, dim3(p.c.batch * p.q_heads), dim3(kFinishThreads), 0, st,
+                  pdl_enabled(), p);
+  if (rc || !p.track) return rc;
+  const int per_cta = (p.score_pitch == 16 ? 2 : 4) * kFinishThreads;
+  const dim3 grid(p.c.batch * p.c.heads, std::min((p.c.capacity + per_cta - 1) / per_cta, 65535));
+  if constexpr (NT == 2)
+    return launch_pdl(paged_track_kernel<16, 16>, grid, dim3(kFinishThreads), 0, st, pdl_enabled(), p);
+  else
+    return launch_pdl(p.score_pitch == 2   ? paged_track_kernel<2, 8>
+                      : p.score_pitch == 4 ? paged_track_kernel<4, 8>
+                                           : paged_track_kernel<8, 8>,
+                      grid, dim3(kFinishThreads), 0, st, pdl_enabled(), p);
 }
 
-template <class T, int DP, bool FULL>
-int launch_nt(const AttnParams& p, const Plan& s, cudaStream_t st) {
-  return s.nt == 1 ? launch<T, DP, 1, FULL>(p, s, st) : launch<T, DP, 2, FULL>(p, s, st);
+template <class T, int DP>
+int launch_dp(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
+  if (p.c.dim == DP) return s.nt == 1 ? launch<T, DP, 1, true>(p, s, tm, st) : launch<T, DP, 2, true>(p, s, tm, st);
+  return s.nt == 1 ? launch<T, DP, 1, false>(p, s, tm, st) : launch<T, DP, 2, false>(p, s, tm, st);
 }
 
 template <class T>
-int launch_type(const AttnParams& p, const Plan& s, cudaStream_t st) {
-  const int d = p.c.dim;
-  if (s.dp == 64) return d == 64 ? launch_nt<T, 64, true>(p, s, st) : launch_nt<T, 64, false>(p, s, st);
-  if (s.dp == 128) return d == 128 ? launch_nt<T, 128, true>(p, s, st) : launch_nt<T, 128, false>(p, s, st);
-  return d == 256 ? launch_nt<T, 256, true>(p, s, st) : launch_nt<T, 256, false>(p, s, st);
+int launch_type(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
+  if (s.dp == 64) return launch_dp<T, 64>(p, s, tm, st);
+  return s.dp == 128 ? launch_dp<T, 128>(p, s, tm, st) : launch_dp<T, 256>(p, s, tm, st);
 }
 
 bool plain_shape(const Pi05PagedCache* c, int q_heads) {
@@ -609,14 +790,23 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
   p.parts = s.parts;
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   p.track = a->track;
-  p.n_ctas = s.ctas;
   p.part_o = reinterpret_cast<float*>(sc + s.part_o);
   p.part_ml = reinterpret_cast<float2*>(sc + s.part_ml);
   p.row_info = reinterpret_cast<int2*>(sc + s.row_info);
   p.row_lse = reinterpret_cast<float*>(sc + s.row_lse);
   p.scores = reinterpret_cast<float*>(sc + s.scores);
+  p.score_pitch = s.score_pitch;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return cache->dtype == PI05_BF16 ? launch_type<__nv_bfloat16>(p, s, st) : launch_type<__half>(p, s, st);
+  p.box_rows = std::min(kWarpRows, cache->page_size & -cache->page_size);
+  const uint64_t dims[4] = {(uint64_t)cache->head_dim, (uint64_t)cache->page_size, (uint64_t)cache->n_kv_heads,
+                            (uint64_t)cache->num_pages};
+  const uint64_t strides[3] = {(uint64_t)p.c.row_stride, (uint64_t)p.c.head_stride, (uint64_t)p.c.page_stride};
+  CUtensorMap tm[2];
+  for (int i = 0; i < 2; ++i) {
+    rc = make_tmap_16bit_4d(&tm[i], i == 0 ? cache->k_pages : cache->v_pages, dims, strides, p.box_rows);
+    if (rc) return rc;
+  }
+  return cache->dtype == PI05_BF16 ? launch_type<__nv_bfloat16>(p, s, tm, st) : launch_type<__half>(p, s, tm, st);
 }
 
 }  // extern "C"
