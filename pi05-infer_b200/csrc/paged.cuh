@@ -48,31 +48,17 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// V consecutive elements, moved by 16-byte words (V = 8, aligned) or one by one.
-template <class T, int V>
-struct Chunk {
-  __align__(16) T e[V];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (V * sizeof(T) % 16 == 0) {
-#pragma unroll
-      for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i)
-        reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) e[i] = p[i];
-    }
-  }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (V * sizeof(T) % 16 == 0) {
-#pragma unroll
-      for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i)
-        reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) p[i] = e[i];
-    }
-  }
-};
+// Two 16-bit elements of a 32-bit word (lower half first).
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
 
 // ---- rotation --------------------------------------------------------------
 // The angle of a position is position * turns / 2^64 turns.  The product wraps at
@@ -87,47 +73,118 @@ __device__ __forceinline__ float2 rotation(long long position, uint64_t turns, f
   return make_float2(c * magnitude, (back ? -s : s) * magnitude);
 }
 
-// What one thread does at a time: V pairs of the half layout (two chunks of V), or
-// V / 2 pairs (one chunk; V = 1: one pair) of the interleaved one, or a chunk of
-// the values that pass through.
+// What one thread does at a time: V pairs of the half layout (two words of V elements),
+// or V / 2 pairs of the interleaved one, or a word of the values that pass through.  V = 1
+// takes single elements, a pair at a time.
 template <int V>
 __host__ __device__ __forceinline__ int rotary_units(int rotary, bool interleaved) {
-  return interleaved ? (V == 1 ? rotary / 2 : rotary / V) : rotary / (2 * V);
+  return rotary / (interleaved && V > 1 ? V : 2 * V);
 }
 
-// cs: cos, sin of each pair.
-template <class T, int V>
-__device__ __forceinline__ void rotate_unit(const T* src, T* dst, int unit, int rotary, bool interleaved,
-                                            const float2* cs) {
-  if (!interleaved) {
-    Chunk<T, V> a, b;
-    const int i = unit * V;
-    a.load(src + i);
-    b.load(src + rotary / 2 + i);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 r = cs[i + j];
-      const float x = to_f32(a.e[j]), y = to_f32(b.e[j]);
-      a.e[j] = from_f32<T>(x * r.x - y * r.y);
-      b.e[j] = from_f32<T>(y * r.x + x * r.y);
-    }
-    a.store(dst + i);
-    b.store(dst + rotary / 2 + i);
-  } else {
-    constexpr int W = V == 1 ? 2 : V;
-    Chunk<T, W> a;
-    const int i = unit * W;
-    a.load(src + i);
-#pragma unroll
-    for (int j = 0; j < W; j += 2) {
-      const float2 r = cs[(i + j) / 2];
-      const float x = to_f32(a.e[j]), y = to_f32(a.e[j + 1]);
-      a.e[j] = from_f32<T>(x * r.x - y * r.y);
-      a.e[j + 1] = from_f32<T>(y * r.x + x * r.y);
-    }
-    a.store(dst + i);
-  }
+// (a, b) -> (a c - b s, b c + a s)
+__device__ __forceinline__ void turn(float& a, float& b, float2 r) {
+  const float x = a;
+  a = x * r.x - b * r.y;
+  b = b * r.x + x * r.y;
 }
+
+// A unit in registers between its load and its store, so that a thread has several
+// loads on their way before it needs the first.  cs: cos and sin of each pair.
+template <class T, int V>
+struct Unit;
+
+template <class T>
+struct Unit<T, 1> {
+  T a, b;
+  __device__ __forceinline__ void load_row(const T* src, int u) { a = src[u]; }
+  __device__ __forceinline__ void store_row(T* dst, int u) const { dst[u] = a; }
+  __device__ __forceinline__ void load(const T* src, int u, int turned, int rotary, bool interleaved) {
+    if (u >= turned) {
+      a = src[rotary + u - turned];
+    } else {
+      a = src[interleaved ? 2 * u : u];
+      b = src[interleaved ? 2 * u + 1 : rotary / 2 + u];
+    }
+  }
+  __device__ __forceinline__ void store(T* dst, int u, int turned, int rotary, bool interleaved,
+                                        const float2* cs) const {
+    if (u >= turned) {
+      dst[rotary + u - turned] = a;
+    } else {
+      float x = to_f32(a), y = to_f32(b);
+      turn(x, y, cs[u]);
+      dst[interleaved ? 2 * u : u] = from_f32<T>(x);
+      dst[interleaved ? 2 * u + 1 : rotary / 2 + u] = from_f32<T>(y);
+    }
+  }
+};
+
+__device__ __forceinline__ uint4 ld16(const void* p) { return *static_cast<const uint4*>(p); }
+__device__ __forceinline__ void st16(void* p, const uint4& v) { *static_cast<uint4*>(p) = v; }
+
+// 16-byte words: V = 8 of the 16-bit types, 4 of fp32.
+template <class T, int V>
+struct Unit {
+  static_assert(V * sizeof(T) == 16, "a word");
+  uint4 a, b;
+  __device__ __forceinline__ void load_row(const T* src, int u) { a = ld16(src + u * V); }
+  __device__ __forceinline__ void store_row(T* dst, int u) const { st16(dst + u * V, a); }
+  __device__ __forceinline__ void load(const T* src, int u, int turned, int rotary, bool interleaved) {
+    a = ld16(src + (u < turned ? u * V : rotary + (u - turned) * V));
+    if (u < turned && !interleaved) b = ld16(src + rotary / 2 + u * V);
+  }
+  static __device__ __forceinline__ void turn_pair(uint32_t& x, const float2* cs) {  // interleaved, one word of 2
+    float2 v = unpack2<T>(x);
+    turn(v.x, v.y, *cs);
+    x = pack2<T>(v.x, v.y);
+  }
+  static __device__ __forceinline__ void turn_two(uint32_t& x, uint32_t& y, const float2* cs) {  // half layout
+    float2 v = unpack2<T>(x), w = unpack2<T>(y);
+    const float4 r = *reinterpret_cast<const float4*>(cs);
+    turn(v.x, w.x, make_float2(r.x, r.y));
+    turn(v.y, w.y, make_float2(r.z, r.w));
+    x = pack2<T>(v.x, v.y);
+    y = pack2<T>(w.x, w.y);
+  }
+  static __device__ __forceinline__ void turn_one(uint32_t& x, uint32_t& y, float2 r) {  // fp32
+    float v = __uint_as_float(x), w = __uint_as_float(y);
+    turn(v, w, r);
+    x = __float_as_uint(v);
+    y = __float_as_uint(w);
+  }
+  __device__ __forceinline__ void store(T* dst, int u, int turned, int rotary, bool interleaved, const float2* cs) {
+    if (u >= turned) {
+      st16(dst + rotary + (u - turned) * V, a);
+    } else if (interleaved) {
+      cs += u * (V / 2);
+      if constexpr (V == 8) {
+        turn_pair(a.x, cs);
+        turn_pair(a.y, cs + 1);
+        turn_pair(a.z, cs + 2);
+        turn_pair(a.w, cs + 3);
+      } else {
+        turn_one(a.x, a.y, cs[0]);
+        turn_one(a.z, a.w, cs[1]);
+      }
+      st16(dst + u * V, a);
+    } else {
+      cs += u * V;
+      if constexpr (V == 8) {
+        turn_two(a.x, b.x, cs);
+        turn_two(a.y, b.y, cs + 2);
+        turn_two(a.z, b.z, cs + 4);
+        turn_two(a.w, b.w, cs + 6);
+      } else {
+        turn_one(a.x, b.x, cs[0]);
+        turn_one(a.y, b.y, cs[1]);
+        turn_one(a.z, b.z, cs[2]);
+        turn_one(a.w, b.w, cs[3]);
+      }
+      st16(dst + u * V, a);
+      st16(dst + rotary / 2 + u * V, b);
+    }
+  }
+};
 
 // ---- division by a number known at launch (n < 2^31) ------------------------
 struct FastDiv {

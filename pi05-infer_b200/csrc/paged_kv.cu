@@ -65,7 +65,9 @@ namespace {
 
 // ---- append ------------------------------------------------------------------
 // Memory bound: q, k and v read once; rotated q, and k and v at their rows, written
-// once.  One token at a time per CTA: its cos and sin are shared by its heads.
+// once.  A CTA takes a few tokens: it asks for their values, finds their rows (sequence,
+// count, page: three loads one after the other) and cos and sin while those are on their
+// way, rotates and stores.
 constexpr int kAppendThreads = 256;
 
 struct AppendParams {
@@ -75,96 +77,130 @@ struct AppendParams {
   const int32_t* cu;
   const float* new_weight;
   const uint64_t* turns;
-  int tokens, q_heads, rotary, interleaved;
+  FastDiv by_units, by_rot, by_row, by_pairs, by_heads;
+  int tokens, q_heads, rotary, interleaved, per_cta;
+  int turned, rot_units, row_units, units;  // of a head rotated, of a head copied, of a token
   float magnitude;
 };
 
-template <class T, int V>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(Pages c, AppendParams p) {
-  extern __shared__ float2 cs[];  // [rotary / 2]
+struct __align__(16) TokenRow {
+  long long at;    // byte offset of the row in its head's lines, or -1
+  long long slot;  // the same of weight and pos
+  int position;
+};
+
+template <class T, int V, int J>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ Pages c,
+                                                                const __grid_constant__ AppendParams p) {
+  extern __shared__ __align__(16) char smem[];
+  TokenRow* row_of = reinterpret_cast<TokenRow*>(smem);             // [per_cta]
+  float2* cs = reinterpret_cast<float2*>(row_of + p.per_cta);       // [per_cta][rotary / 2]
   __shared__ int last;
   pdl_wait();
   pdl_launch_dependents();
-  const int d = c.dim;
-  const int turned = p.rotary > 0 ? rotary_units<V>(p.rotary, p.interleaved) : 0;
-  const int rot_units = turned + (d - p.rotary) / V, row_units = d / V;
-  const int total = p.cu != nullptr ? min(max(p.cu[c.batch], 0), p.tokens) : p.tokens;
-  for (int t = blockIdx.x; t < total; t += gridDim.x) {
-    int b = t, off = 0;
-    if (p.cu != nullptr) {  // the sequence with cu[b] <= t < cu[b + 1]
-      int lo = 0, hi = c.batch;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        (p.cu[mid] <= t ? lo : hi) = mid;
-      }
-      b = lo;
-      off = t - p.cu[b];
-    }
-    const int held = c.counts[b], seen = c.counts[c.batch + b];
-    const long long r = (long long)held + off;
-    const int position = seen + off;
-    int line = 0, page = -1;
-    if (r >= 0 && r < c.capacity) page = c.page_of(b, (int)r, &line);
-    const bool ok = c.real(page);
-    if (!ok && threadIdx.x == 0) report_status(c.status, PI05_DEV_BAD_INDEX);
-    for (int i = threadIdx.x; i < p.rotary / 2; i += kAppendThreads)
-      cs[i] = rotation(position, p.turns[i], p.magnitude, false);
-    __syncthreads();
-    const int nq = p.q_heads * rot_units, nk = ok ? c.heads * rot_units : 0, nv = ok ? c.heads * row_units : 0;
-    for (int i = threadIdx.x; i < nq + nk + nv; i += kAppendThreads) {
-      const T* src;
-      T* dst;
-      int u, first = turned;
-      if (i < nq) {
-        const int h = i / rot_units;
-        u = i - h * rot_units;
-        src = static_cast<const T*>(p.q) + t * p.qt + h * p.qh;
-        dst = static_cast<T*>(p.q_out) + ((size_t)t * p.q_heads + h) * d;
-      } else if (i < nq + nk) {
-        const int h = (i - nq) / rot_units;
-        u = i - nq - h * rot_units;
-        src = static_cast<const T*>(p.k) + t * p.kt + h * p.kh;
-        dst = reinterpret_cast<T*>(c.k + c.row_at(page, h, line));
-      } else {
-        const int h = (i - nq - nk) / row_units;
-        u = i - nq - nk - h * row_units;
-        first = 0;
-        src = static_cast<const T*>(p.v) + t * p.vt + h * p.vh;
-        dst = reinterpret_cast<T*>(c.v + c.row_at(page, h, line));
-      }
-      if (u < first) {
-        rotate_unit<T, V>(src, dst, u, p.rotary, p.interleaved, cs);
-      } else {
-        Chunk<T, V> x;
-        const int at = (first > 0 ? p.rotary : 0) + (u - first) * V;
-        x.load(src + at);
-        x.store(dst + at);
+  const int tid = threadIdx.x, d = c.dim, pairs = p.rotary / 2;
+  const int t0 = blockIdx.x * p.per_cta;
+  const int used = p.cu != nullptr ? min(max(p.cu[c.batch], 0), p.tokens) : p.tokens;
+  const int n = min(p.per_cta, used - t0), total = n * p.units;  // n < 1: padding alone
+  const int nq = p.q_heads * p.rot_units, nk = c.heads * p.rot_units;
+  for (int first = tid; first < total || first == tid; first += J * kAppendThreads) {
+    Unit<T, V> unit[J];
+    int token[J], head[J], u[J];  // head: query heads, then key heads, then value heads
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int i = first + j * kAppendThreads;
+      if (i < total) {
+        token[j] = p.by_units.div(i);
+        const int r = i - token[j] * p.units;
+        const long long t = t0 + token[j];
+        if (r < nq + nk) {
+          head[j] = p.by_rot.div(r);
+          u[j] = r - head[j] * p.rot_units;
+          const T* src = head[j] < p.q_heads ? static_cast<const T*>(p.q) + t * p.qt + head[j] * p.qh
+                                             : static_cast<const T*>(p.k) + t * p.kt + (head[j] - p.q_heads) * p.kh;
+          unit[j].load(src, u[j], p.turned, p.rotary, p.interleaved);
+        } else {
+          const int h = p.by_row.div(r - nq - nk);
+          u[j] = r - nq - nk - h * p.row_units;
+          head[j] = p.q_heads + c.heads + h;
+          unit[j].load_row(static_cast<const T*>(p.v) + t * p.vt + h * p.vh, u[j]);
+        }
       }
     }
-    if (ok) {
-      for (int h = threadIdx.x; h < c.heads; h += kAppendThreads) {
-        const size_t s = c.slot_at(page, h, line);
-        if (c.pos != nullptr) c.pos[s] = position;
-        if (c.weight != nullptr) c.weight[s] = p.new_weight != nullptr ? p.new_weight[(size_t)t * c.heads + h] : 0.f;
+    if (first == tid) {
+      for (int i = tid; i < n; i += kAppendThreads) {
+        const int t = t0 + i;
+        int b = t, off = 0;
+        if (p.cu != nullptr) {  // the sequence with cu[b] <= t < cu[b + 1]
+          int lo = 0, hi = c.batch;
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            (p.cu[mid] <= t ? lo : hi) = mid;
+          }
+          b = lo;
+          off = t - p.cu[b];
+        }
+        const int held = c.counts[b], seen = c.counts[c.batch + b];
+        const long long r = (long long)held + off;
+        int line = 0, page = -1;
+        if (r >= 0 && r < c.capacity) page = c.page_of(b, (int)r, &line);
+        TokenRow row{-1, -1, seen + off};
+        if (c.real(page)) {
+          row.at = (long long)c.row_at(page, 0, line);
+          row.slot = (long long)c.slot_at(page, 0, line);
+        } else {
+          report_status(c.status, PI05_DEV_BAD_INDEX);
+        }
+        row_of[i] = row;
+        if (p.cu == nullptr) {  // nobody else has the sequence
+          c.counts[b] = max(held, min(held + 1, c.capacity));
+          c.counts[c.batch + b] = seen + 1;
+        }
       }
+      __syncthreads();
+      for (int i = tid; i < n * pairs; i += kAppendThreads) {
+        const int t = p.by_pairs.div(i);
+        cs[i] = rotation(row_of[t].position, p.turns[i - t * pairs], p.magnitude, false);
+      }
+      for (int i = tid; i < n * c.heads; i += kAppendThreads) {
+        const int t = p.by_heads.div(i), h = i - t * c.heads;
+        if (row_of[t].at < 0) continue;
+        const size_t s = row_of[t].slot + (size_t)h * c.page_size;
+        if (c.pos != nullptr) c.pos[s] = row_of[t].position;
+        if (c.weight != nullptr)
+          c.weight[s] = p.new_weight != nullptr ? p.new_weight[(size_t)(t0 + t) * c.heads + h] : 0.f;
+      }
+      __syncthreads();
     }
-    __syncthreads();  // the next token's cos and sin; and everyone has read the counts
-    if (p.cu == nullptr && threadIdx.x == 0) {  // this CTA alone has the sequence
-      c.counts[b] = max(held, min(held + 1, c.capacity));
-      c.counts[c.batch + b] = seen + 1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (first + j * kAppendThreads >= total) continue;
+      const TokenRow row = row_of[token[j]];
+      const int h = head[j];
+      if (h < p.q_heads) {
+        unit[j].store(static_cast<T*>(p.q_out) + ((size_t)(t0 + token[j]) * p.q_heads + h) * d, u[j], p.turned,
+                      p.rotary, p.interleaved, cs + token[j] * pairs);
+      } else if (row.at >= 0) {
+        if (h < p.q_heads + c.heads)
+          unit[j].store(reinterpret_cast<T*>(c.k + row.at + (h - p.q_heads) * c.head_stride), u[j], p.turned, p.rotary,
+                        p.interleaved, cs + token[j] * pairs);
+        else
+          unit[j].store_row(reinterpret_cast<T*>(c.v + row.at + (h - p.q_heads - c.heads) * c.head_stride), u[j]);
+      }
     }
   }
   if (p.cu == nullptr) return;
   // Ragged: the CTA that finishes last moves the counts on, when all have read them.
-  if (threadIdx.x == 0) last = atom_add_acq_rel_gpu(c.ticket, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (tid == 0) last = atom_add_acq_rel_gpu(c.ticket, 1) == (int)gridDim.x - 1;
   __syncthreads();
   if (!last) return;
-  for (int b = threadIdx.x; b < c.batch; b += kAppendThreads) {
-    const int n = max(min(p.cu[b + 1], p.tokens) - max(p.cu[b], 0), 0), held = c.counts[b];
-    c.counts[b] = max(held, (int)min((long long)held + n, (long long)c.capacity));
-    c.counts[c.batch + b] += n;
+  for (int b = tid; b < c.batch; b += kAppendThreads) {
+    const int m = max(min(p.cu[b + 1], p.tokens) - max(p.cu[b], 0), 0), held = c.counts[b];
+    c.counts[b] = max(held, (int)min((long long)held + m, (long long)c.capacity));
+    c.counts[c.batch + b] += m;
   }
-  if (threadIdx.x == 0) *c.ticket = 0;
+  if (tid == 0) *c.ticket = 0;
 }
 
 // ---- eviction ------------------------------------------------------------------
@@ -306,15 +342,36 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(Pages c) {
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) c.counts[b] = left;
 }
 
+template <class T, int V>
+int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
+  constexpr int J = 4;
+  p.turned = p.rotary > 0 ? rotary_units<V>(p.rotary, p.interleaved) : 0;
+  p.rot_units = p.turned + (c.dim - p.rotary) / V;
+  p.row_units = c.dim / V;
+  p.units = (p.q_heads + c.heads) * p.rot_units + c.heads * p.row_units;
+  p.by_units = FastDiv(p.units);
+  p.by_rot = FastDiv(p.rot_units);
+  p.by_row = FastDiv(p.row_units);
+  p.by_pairs = FastDiv(std::max(1, p.rotary / 2));
+  p.by_heads = FastDiv(c.heads);
+  // Two batches of loads for a CTA, but for tokens enough to fill the SMs.
+  const int fill = std::max(1, std::min(64, 2 * J * kAppendThreads / p.units));
+  p.per_cta = std::max(1, std::min(fill, p.tokens / kSMs));
+  const size_t smem = p.per_cta * (sizeof(TokenRow) + (size_t)(p.rotary / 2) * sizeof(float2));  // 64 x 1 KB at most
+  static_assert(64 * (sizeof(TokenRow) + 128 * sizeof(float2)) <= 100 * 1024, "shared memory");
+  if (smem > 48 * 1024) p.per_cta = 32;
+  return launch_pdl(append_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kAppendThreads),
+                    p.per_cta * (sizeof(TokenRow) + (size_t)(p.rotary / 2) * sizeof(float2)), stream, pdl_enabled(), c,
+                    p);
+}
+
 template <class T>
-int append_run(const Pages& c, const AppendParams& p, cudaStream_t stream) {
+int append_type(const Pages& c, const AppendParams& p, cudaStream_t stream) {
   const bool vec = aligned16(p.k) && aligned16(p.v) && p.kt % 8 == 0 && p.kh % 8 == 0 && p.vt % 8 == 0 &&
                    p.vh % 8 == 0 &&
                    (p.q == nullptr || (aligned16(p.q) && aligned16(p.q_out) && p.qt % 8 == 0 && p.qh % 8 == 0)) &&
                    p.rotary % (p.interleaved ? 8 : 16) == 0;
-  const int grid = p.cu == nullptr ? p.tokens : std::min(p.tokens, kSMs * 8);
-  return launch_pdl(vec ? append_kernel<T, 8> : append_kernel<T, 1>, dim3(grid), dim3(kAppendThreads),
-                    (size_t)(p.rotary / 2) * sizeof(float2), stream, pdl_enabled(), c, p);
+  return vec ? append_run<T, 8>(c, p, stream) : append_run<T, 1>(c, p, stream);
 }
 
 }  // namespace
@@ -380,7 +437,7 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, voi
   p.interleaved = rot ? rot->interleaved : 0;
   p.magnitude = rot ? rot->magnitude : 1.f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return cache->dtype == PI05_BF16 ? append_run<__nv_bfloat16>(c, p, st) : append_run<__half>(c, p, st);
+  return cache->dtype == PI05_BF16 ? append_type<__nv_bfloat16>(c, p, st) : append_type<__half>(c, p, st);
 }
 
 int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int sinks, void* stream) {

@@ -2,8 +2,11 @@
 //
 //   (a, b) of a pair -> (a c - b s, b c + a s),  c + i s = magnitude * exp(i angle)
 //
-// Memory bound: x read once, out written once.  A token's cos and sin are worked out
-// once per CTA into shared memory and used for all its heads.
+// Memory bound: x read once, out written once.  A CTA takes a few tokens: it asks for its
+// values, works out the tokens' cos and sin into shared memory while they are on their way
+// (once for all heads), rotates and stores.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace pi05 {
@@ -15,56 +18,75 @@ struct RopeParams {
   long long xt, xh, ot, oh;  // strides, elements
   const void* positions;
   const uint64_t* turns;
-  int pos64, tokens, heads, dim, rotary, interleaved, back, per_cta;
+  FastDiv by_units, by_heads, by_pairs;
+  int pos64, tokens, heads, dim, rotary, interleaved, back, per_cta, units, turned;
   float magnitude;
 };
 
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const T* x, T* out, RopeParams p) {
-  extern __shared__ float2 cs[];  // [per_cta][rotary / 2]
+template <class T, int V, int J>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const T* x, T* out, const __grid_constant__ RopeParams p) {
+  extern __shared__ __align__(16) float2 cs[];  // [per_cta][rotary / 2]
   pdl_wait();
   pdl_launch_dependents();
   const int pairs = p.rotary / 2;
-  const int turned = rotary_units<V>(p.rotary, p.interleaved);
-  const int units = turned + (x == out ? 0 : (p.dim - p.rotary) / V);  // in place, the rest is there already
-  for (long long t0 = (long long)blockIdx.x * p.per_cta; t0 < p.tokens; t0 += (long long)gridDim.x * p.per_cta) {
-    const int n = min((long long)p.per_cta, p.tokens - t0);
-    for (int i = threadIdx.x; i < n * pairs; i += kThreads) {
-      const int t = i / pairs, f = i - t * pairs;
-      const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + t]
-                                    : static_cast<const int32_t*>(p.positions)[t0 + t];
-      cs[i] = rotation(pos, p.turns[f], p.magnitude, p.back);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * p.heads * units; i += kThreads) {
-      const int row = i / units, u = i - row * units, t = row / p.heads, h = row - t * p.heads;
-      const T* src = x + (t0 + t) * p.xt + h * p.xh;
-      T* dst = out + (t0 + t) * p.ot + h * p.oh;
-      if (u < turned) {
-        rotate_unit<T, V>(src, dst, u, p.rotary, p.interleaved, cs + t * pairs);
-      } else {
-        Chunk<T, V> c;
-        const int at = p.rotary + (u - turned) * V;
-        c.load(src + at);
-        c.store(dst + at);
+  const long long t0 = (long long)blockIdx.x * p.per_cta;
+  const int n = (int)min((long long)p.per_cta, p.tokens - t0), total = n * p.heads * p.units;
+  for (int first = threadIdx.x; first < total || first == (int)threadIdx.x; first += J * kThreads) {
+    Unit<T, V> unit[J];
+    int token[J], head[J], u[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int i = first + j * kThreads;
+      if (i < total) {
+        const int row = p.by_units.div(i);
+        token[j] = p.by_heads.div(row);
+        u[j] = i - row * p.units;
+        head[j] = row - token[j] * p.heads;
+        unit[j].load(x + (t0 + token[j]) * p.xt + head[j] * p.xh, u[j], p.turned, p.rotary, p.interleaved);
       }
     }
-    __syncthreads();
+    if (first == (int)threadIdx.x) {
+      for (int i = threadIdx.x; i < n * pairs; i += kThreads) {
+        const int t = p.by_pairs.div(i);
+        const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + t]
+                                      : static_cast<const int32_t*>(p.positions)[t0 + t];
+        cs[i] = rotation(pos, p.turns[i - t * pairs], p.magnitude, p.back);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (first + j * kThreads < total)
+        unit[j].store(out + (t0 + token[j]) * p.ot + head[j] * p.oh, u[j], p.turned, p.rotary, p.interleaved,
+                      cs + token[j] * pairs);
   }
 }
 
-template <class T>
+template <class T, int V>
 int rope_run(const void* x, void* out, RopeParams p, cudaStream_t stream) {
-  constexpr int kVec = 8;
-  const long long step = 16 / (long long)sizeof(T);
-  // 16-byte chunks need every row, and the partner half of a row, on a 16-byte boundary.
-  const bool vec = aligned16(x) && aligned16(out) && p.xt % step == 0 && p.xh % step == 0 && p.ot % step == 0 &&
-                   p.oh % step == 0 && p.dim % kVec == 0 && p.rotary % (p.interleaved ? kVec : 2 * kVec) == 0;
-  p.per_cta = 1;
+  constexpr int J = 4;
+  p.turned = rotary_units<V>(p.rotary, p.interleaved);
+  p.units = p.turned + (x == out ? 0 : (p.dim - p.rotary) / V);  // in place, the rest is there already
+  p.by_units = FastDiv(p.units);
+  p.by_heads = FastDiv(p.heads);
+  p.by_pairs = FastDiv(p.rotary / 2);
+  // One batch of loads for a CTA, but for tokens enough to fill the SMs.
+  const int fill = std::max(1, J * kThreads / (p.heads * p.units));
+  p.per_cta = std::max(1, std::min(fill, p.tokens / kSMs));
   const size_t smem = (size_t)p.per_cta * (p.rotary / 2) * sizeof(float2);
-  const int grid = (int)std::min<long long>((p.tokens + p.per_cta - 1) / p.per_cta, kSMs * 8);
-  return launch_pdl(vec ? rope_kernel<T, kVec> : rope_kernel<T, 1>, dim3(grid), dim3(kThreads), smem, stream,
-                    pdl_enabled(), static_cast<const T*>(x), static_cast<T*>(out), p);
+  if (smem > 48 * 1024) p.per_cta = 48 * 1024 / ((p.rotary / 2) * (int)sizeof(float2));
+  return launch_pdl(rope_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kThreads),
+                    (size_t)p.per_cta * (p.rotary / 2) * sizeof(float2), stream, pdl_enabled(),
+                    static_cast<const T*>(x), static_cast<T*>(out), p);
+}
+
+template <class T>
+int rope_type(const void* x, void* out, const RopeParams& p, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  // 16-byte chunks need every row, and the partner half of a row, on a 16-byte boundary.
+  const bool vec = aligned16(x) && aligned16(out) && p.xt % V == 0 && p.xh % V == 0 && p.ot % V == 0 && p.oh % V == 0 &&
+                   p.dim % V == 0 && p.rotary % (p.interleaved ? V : 2 * V) == 0;
+  return vec ? rope_run<T, V>(x, out, p, stream) : rope_run<T, 1>(x, out, p, stream);
 }
 
 }  // namespace
@@ -112,7 +134,7 @@ extern "C" int pi05_rope(const void* x, void* out, int dtype, int tokens, int he
   p.back = transpose;
   p.magnitude = rotary->magnitude;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == PI05_BF16) return rope_run<__nv_bfloat16>(x, out, p, st);
-  if (dtype == PI05_FP16) return rope_run<__half>(x, out, p, st);
-  return rope_run<float>(x, out, p, st);
+  if (dtype == PI05_BF16) return rope_type<__nv_bfloat16>(x, out, p, st);
+  if (dtype == PI05_FP16) return rope_type<__half>(x, out, p, st);
+  return rope_type<float>(x, out, p, st);
 }
