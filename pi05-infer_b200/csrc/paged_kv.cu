@@ -68,7 +68,7 @@ namespace {
 // once.  A CTA takes a few tokens: it asks for their values, finds their rows (sequence,
 // count, page: three loads one after the other) and cos and sin while those are on their
 // way, rotates and stores.
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 
 struct AppendParams {
   const void *k, *v, *q;
@@ -77,9 +77,10 @@ struct AppendParams {
   const int32_t* cu;
   const float* new_weight;
   const uint64_t* turns;
-  FastDiv by_units, by_rot, by_row, by_pairs, by_heads;
+  FastDiv by_qk, by_heads, by_pairs;
   int tokens, q_heads, rotary, interleaved, per_cta;
-  int turned, rot_units, row_units, units;  // of a head rotated, of a head copied, of a token
+  int turned, units, lanes;    // of a head of q or k
+  int row_units, row_lanes;    // of a head of v
   float magnitude;
 };
 
@@ -93,101 +94,134 @@ template <class T, int V, int J>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ Pages c,
                                                                 const __grid_constant__ AppendParams p) {
   extern __shared__ __align__(16) char smem[];
-  TokenRow* row_of = reinterpret_cast<TokenRow*>(smem);             // [per_cta]
-  float2* cs = reinterpret_cast<float2*>(row_of + p.per_cta);       // [per_cta][rotary / 2]
-  __shared__ int last;
+  TokenRow* row_of = reinterpret_cast<TokenRow*>(smem);        // [per_cta]
+  float2* cs = reinterpret_cast<float2*>(row_of + p.per_cta);  // [per_cta][rotary / 2]
+  __shared__ int last, cu_of[kAppendThreads], held_of[kAppendThreads], seen_of[kAppendThreads];
   pdl_wait();
   pdl_launch_dependents();
-  const int tid = threadIdx.x, d = c.dim, pairs = p.rotary / 2;
+  const int tid = threadIdx.x, pairs = p.rotary / 2;
   const int t0 = blockIdx.x * p.per_cta;
   const int used = p.cu != nullptr ? min(max(p.cu[c.batch], 0), p.tokens) : p.tokens;
-  const int n = min(p.per_cta, used - t0), total = n * p.units;  // n < 1: padding alone
-  const int nq = p.q_heads * p.rot_units, nk = c.heads * p.rot_units;
-  for (int first = tid; first < total || first == tid; first += J * kAppendThreads) {
-    Unit<T, V> unit[J];
-    int token[J], head[J], u[J];  // head: query heads, then key heads, then value heads
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int i = first + j * kAppendThreads;
-      if (i < total) {
-        token[j] = p.by_units.div(i);
-        const int r = i - token[j] * p.units;
-        const long long t = t0 + token[j];
-        if (r < nq + nk) {
-          head[j] = p.by_rot.div(r);
-          u[j] = r - head[j] * p.rot_units;
-          const T* src = head[j] < p.q_heads ? static_cast<const T*>(p.q) + t * p.qt + head[j] * p.qh
-                                             : static_cast<const T*>(p.k) + t * p.kt + (head[j] - p.q_heads) * p.kh;
-          unit[j].load(src, u[j], p.turned, p.rotary, p.interleaved);
-        } else {
-          const int h = p.by_row.div(r - nq - nk);
-          u[j] = r - nq - nk - h * p.row_units;
-          head[j] = p.q_heads + c.heads + h;
-          unit[j].load_row(static_cast<const T*>(p.v) + t * p.vt + h * p.vh, u[j]);
+  const int n = max(0, min(p.per_cta, used - t0));  // 0: padding alone
+
+  // Where the CTA's tokens go, and their cos and sin.
+  const bool few = p.cu != nullptr && c.batch <= kAppendThreads;
+  auto find_rows = [&]() {
+    if (few) {  // one load's latency instead of a search's
+      if (tid < c.batch) {
+        cu_of[tid] = p.cu[tid];
+        held_of[tid] = c.counts[tid];
+        seen_of[tid] = c.counts[c.batch + tid];
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < n; i += kAppendThreads) {
+      const int t = t0 + i;
+      int b = t, off = 0;
+      if (p.cu != nullptr) {  // the sequence with cu[b] <= t < cu[b + 1]
+        int lo = 0, hi = c.batch;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          ((few ? cu_of[mid] : p.cu[mid]) <= t ? lo : hi) = mid;
         }
+        b = lo;
+        off = t - (few ? cu_of[b] : p.cu[b]);
+      }
+      const int held = few ? held_of[b] : c.counts[b], seen = few ? seen_of[b] : c.counts[c.batch + b];
+      const long long r = (long long)held + off;
+      int line = 0, page = -1;
+      if (r >= 0 && r < c.capacity) page = c.page_of(b, (int)r, &line);
+      TokenRow row{-1, -1, seen + off};
+      if (c.real(page)) {
+        row.at = (long long)c.row_at(page, 0, line);
+        row.slot = (long long)c.slot_at(page, 0, line);
+      } else {
+        report_status(c.status, PI05_DEV_BAD_INDEX);
+      }
+      row_of[i] = row;
+      if (p.cu == nullptr) {  // nobody else has the sequence
+        c.counts[b] = max(held, min(held + 1, c.capacity));
+        c.counts[c.batch + b] = seen + 1;
       }
     }
-    if (first == tid) {
-      for (int i = tid; i < n; i += kAppendThreads) {
-        const int t = t0 + i;
-        int b = t, off = 0;
-        if (p.cu != nullptr) {  // the sequence with cu[b] <= t < cu[b + 1]
-          int lo = 0, hi = c.batch;
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            (p.cu[mid] <= t ? lo : hi) = mid;
+    __syncthreads();
+    for (int i = tid; i < n * pairs; i += kAppendThreads) {
+      const int t = p.by_pairs.div(i);
+      const int f = i - t * pairs;
+      cs[t * pairs + Unit<T, V>::place(f, p.turned, p.interleaved)] =
+          rotation(row_of[t].position, p.turns[f], p.magnitude, false);
+    }
+    for (int i = tid; i < n * c.heads; i += kAppendThreads) {
+      const int t = p.by_heads.div(i), h = i - t * c.heads;
+      if (row_of[t].at < 0) continue;
+      const size_t s = row_of[t].slot + (size_t)h * c.page_size;
+      if (c.pos != nullptr) c.pos[s] = row_of[t].position;
+      if (c.weight != nullptr)
+        c.weight[s] = p.new_weight != nullptr ? p.new_weight[(size_t)(t0 + t) * c.heads + h] : 0.f;
+    }
+    __syncthreads();
+  };
+
+  bool ready = false;
+  {  // q and k: `lanes` threads to a head's units, kAppendThreads / lanes heads at a time
+    const int heads = p.q_heads + c.heads, rows = n * heads;
+    const int row0 = tid / p.lanes, u0 = tid - row0 * p.lanes, step = kAppendThreads / p.lanes;
+    for (int u = u0; u < p.units || u == u0; u += p.lanes) {
+      const bool mine = u < p.units && row0 < step;
+      for (int r = row0; r < rows || !ready; r += J * step) {
+        Unit<T, V> unit[J];
+        int token[J], head[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int row = r + j * step;
+          token[j] = p.by_qk.div(row);
+          head[j] = row - token[j] * heads;
+          if (mine && row < rows)
+            unit[j].load(head[j] < p.q_heads
+                             ? static_cast<const T*>(p.q) + (t0 + token[j]) * p.qt + head[j] * p.qh
+                             : static_cast<const T*>(p.k) + (t0 + token[j]) * p.kt + (head[j] - p.q_heads) * p.kh,
+                         u, p.turned, p.rotary, p.interleaved);
+        }
+        if (!ready) find_rows();
+        ready = true;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (!mine || r + j * step >= rows) continue;
+          T* dst;
+          if (head[j] < p.q_heads) {
+            dst = static_cast<T*>(p.q_out) + ((size_t)(t0 + token[j]) * p.q_heads + head[j]) * c.dim;
+          } else {
+            const long long at = row_of[token[j]].at;
+            if (at < 0) continue;
+            dst = reinterpret_cast<T*>(c.k + at + (head[j] - p.q_heads) * c.head_stride);
           }
-          b = lo;
-          off = t - p.cu[b];
-        }
-        const int held = c.counts[b], seen = c.counts[c.batch + b];
-        const long long r = (long long)held + off;
-        int line = 0, page = -1;
-        if (r >= 0 && r < c.capacity) page = c.page_of(b, (int)r, &line);
-        TokenRow row{-1, -1, seen + off};
-        if (c.real(page)) {
-          row.at = (long long)c.row_at(page, 0, line);
-          row.slot = (long long)c.slot_at(page, 0, line);
-        } else {
-          report_status(c.status, PI05_DEV_BAD_INDEX);
-        }
-        row_of[i] = row;
-        if (p.cu == nullptr) {  // nobody else has the sequence
-          c.counts[b] = max(held, min(held + 1, c.capacity));
-          c.counts[c.batch + b] = seen + 1;
+          unit[j].store(dst, u, p.turned, p.rotary, p.interleaved, cs + token[j] * pairs);
         }
       }
-      __syncthreads();
-      for (int i = tid; i < n * pairs; i += kAppendThreads) {
-        const int t = p.by_pairs.div(i);
-        cs[i] = rotation(row_of[t].position, p.turns[i - t * pairs], p.magnitude, false);
-      }
-      for (int i = tid; i < n * c.heads; i += kAppendThreads) {
-        const int t = p.by_heads.div(i), h = i - t * c.heads;
-        if (row_of[t].at < 0) continue;
-        const size_t s = row_of[t].slot + (size_t)h * c.page_size;
-        if (c.pos != nullptr) c.pos[s] = row_of[t].position;
-        if (c.weight != nullptr)
-          c.weight[s] = p.new_weight != nullptr ? p.new_weight[(size_t)(t0 + t) * c.heads + h] : 0.f;
-      }
-      __syncthreads();
     }
+  }
+  {  // v
+    const int rows = n * c.heads;
+    const int row0 = tid / p.row_lanes, u0 = tid - row0 * p.row_lanes, step = kAppendThreads / p.row_lanes;
+    if (row0 < step)
+      for (int u = u0; u < p.row_units; u += p.row_lanes)
+        for (int r = row0; r < rows; r += J * step) {
+          Unit<T, V> unit[J];
+          int token[J], head[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      if (first + j * kAppendThreads >= total) continue;
-      const TokenRow row = row_of[token[j]];
-      const int h = head[j];
-      if (h < p.q_heads) {
-        unit[j].store(static_cast<T*>(p.q_out) + ((size_t)(t0 + token[j]) * p.q_heads + h) * d, u[j], p.turned,
-                      p.rotary, p.interleaved, cs + token[j] * pairs);
-      } else if (row.at >= 0) {
-        if (h < p.q_heads + c.heads)
-          unit[j].store(reinterpret_cast<T*>(c.k + row.at + (h - p.q_heads) * c.head_stride), u[j], p.turned, p.rotary,
-                        p.interleaved, cs + token[j] * pairs);
-        else
-          unit[j].store_row(reinterpret_cast<T*>(c.v + row.at + (h - p.q_heads - c.heads) * c.head_stride), u[j]);
-      }
-    }
+          for (int j = 0; j < J; ++j) {
+            const int row = r + j * step;
+            token[j] = p.by_heads.div(row);
+            head[j] = row - token[j] * c.heads;
+            if (row < rows) unit[j].load_row(static_cast<const T*>(p.v) + (t0 + token[j]) * p.vt + head[j] * p.vh, u);
+          }
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            if (r + j * step >= rows) continue;
+            const long long at = row_of[token[j]].at;
+            if (at >= 0) unit[j].store_row(reinterpret_cast<T*>(c.v + at + head[j] * c.head_stride), u);
+          }
+        }
   }
   if (p.cu == nullptr) return;
   // Ragged: the CTA that finishes last moves the counts on, when all have read them.
@@ -344,22 +378,18 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(Pages c) {
 
 template <class T, int V>
 int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
-  constexpr int J = 4;
+  constexpr int J = 2;
   p.turned = p.rotary > 0 ? rotary_units<V>(p.rotary, p.interleaved) : 0;
-  p.rot_units = p.turned + (c.dim - p.rotary) / V;
+  p.units = p.turned + (c.dim - p.rotary) / V;
+  p.lanes = std::min(p.units, kAppendThreads);
   p.row_units = c.dim / V;
-  p.units = (p.q_heads + c.heads) * p.rot_units + c.heads * p.row_units;
-  p.by_units = FastDiv(p.units);
-  p.by_rot = FastDiv(p.rot_units);
-  p.by_row = FastDiv(p.row_units);
-  p.by_pairs = FastDiv(std::max(1, p.rotary / 2));
+  p.row_lanes = std::min(p.row_units, kAppendThreads);
+  p.by_qk = FastDiv(p.q_heads + c.heads);
   p.by_heads = FastDiv(c.heads);
-  // Two batches of loads for a CTA, but for tokens enough to fill the SMs.
-  const int fill = std::max(1, std::min(64, 2 * J * kAppendThreads / p.units));
-  p.per_cta = std::max(1, std::min(fill, p.tokens / kSMs));
-  const size_t smem = p.per_cta * (sizeof(TokenRow) + (size_t)(p.rotary / 2) * sizeof(float2));  // 64 x 1 KB at most
-  static_assert(64 * (sizeof(TokenRow) + 128 * sizeof(float2)) <= 100 * 1024, "shared memory");
-  if (smem > 48 * 1024) p.per_cta = 32;
+  p.by_pairs = FastDiv(std::max(1, p.rotary / 2));
+  // A few batches of loads for a CTA, but for tokens enough to fill the SMs.
+  const int fill = 8 * J * (kAppendThreads / p.lanes) / (p.q_heads + c.heads);
+  p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 40}));  // 40 x (1 KB + 32) of shared memory at most
   return launch_pdl(append_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kAppendThreads),
                     p.per_cta * (sizeof(TokenRow) + (size_t)(p.rotary / 2) * sizeof(float2)), stream, pdl_enabled(), c,
                     p);

@@ -3,8 +3,10 @@
 //   (a, b) of a pair -> (a c - b s, b c + a s),  c + i s = magnitude * exp(i angle)
 //
 // Memory bound: x read once, out written once.  A CTA takes a few tokens: it asks for its
-// values, works out the tokens' cos and sin into shared memory while they are on their way
-// (once for all heads), rotates and stores.
+// first values, works out the tokens' cos and sin into shared memory while they are on
+// their way (once for all heads), then streams.  A thread keeps its place within a head
+// and goes from head to head: with the place worked out for every word, integer
+// arithmetic filled 76% of the issue slots at 5.6 TB/s.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -12,14 +14,14 @@
 namespace pi05 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct RopeParams {
   long long xt, xh, ot, oh;  // strides, elements
   const void* positions;
   const uint64_t* turns;
-  FastDiv by_units, by_heads, by_pairs;
-  int pos64, tokens, heads, dim, rotary, interleaved, back, per_cta, units, turned;
+  FastDiv by_heads, by_pairs;
+  int pos64, tokens, heads, dim, rotary, interleaved, back, per_cta, units, turned, lanes;
   float magnitude;
 };
 
@@ -28,37 +30,45 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const T* x, T* out, cons
   extern __shared__ __align__(16) float2 cs[];  // [per_cta][rotary / 2]
   pdl_wait();
   pdl_launch_dependents();
-  const int pairs = p.rotary / 2;
+  const int pairs = p.rotary / 2, tid = threadIdx.x;
   const long long t0 = (long long)blockIdx.x * p.per_cta;
-  const int n = (int)min((long long)p.per_cta, p.tokens - t0), total = n * p.heads * p.units;
-  for (int first = threadIdx.x; first < total || first == (int)threadIdx.x; first += J * kThreads) {
-    Unit<T, V> unit[J];
-    int token[J], head[J], u[J];
+  const int n = (int)min((long long)p.per_cta, p.tokens - t0), rows = n * p.heads;
+  x += t0 * p.xt;
+  out += t0 * p.ot;
+  // `lanes` threads to a head's units, kThreads / lanes heads at a time.
+  const int row0 = tid / p.lanes, u0 = tid - row0 * p.lanes, step = kThreads / p.lanes;
+  bool ready = false;
+  for (int u = u0; u < p.units || u == u0; u += p.lanes) {
+    const bool mine = u < p.units && row0 < step;
+    for (int r = row0; r < rows || !ready; r += J * step) {
+      Unit<T, V> unit[J];
+      int token[J], head[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int i = first + j * kThreads;
-      if (i < total) {
-        const int row = p.by_units.div(i);
+      for (int j = 0; j < J; ++j) {
+        const int row = r + j * step;
         token[j] = p.by_heads.div(row);
-        u[j] = i - row * p.units;
         head[j] = row - token[j] * p.heads;
-        unit[j].load(x + (t0 + token[j]) * p.xt + head[j] * p.xh, u[j], p.turned, p.rotary, p.interleaved);
+        if (mine && row < rows)
+          unit[j].load(x + token[j] * p.xt + head[j] * p.xh, u, p.turned, p.rotary, p.interleaved);
       }
-    }
-    if (first == (int)threadIdx.x) {
-      for (int i = threadIdx.x; i < n * pairs; i += kThreads) {
-        const int t = p.by_pairs.div(i);
-        const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + t]
-                                      : static_cast<const int32_t*>(p.positions)[t0 + t];
-        cs[i] = rotation(pos, p.turns[i - t * pairs], p.magnitude, p.back);
+      if (!ready) {
+        for (int i = tid; i < n * pairs; i += kThreads) {
+          const int t = p.by_pairs.div(i);
+          const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + t]
+                                        : static_cast<const int32_t*>(p.positions)[t0 + t];
+          const int f = i - t * pairs;
+          cs[t * pairs + Unit<T, V>::place(f, p.turned, p.interleaved)] =
+              rotation(pos, p.turns[f], p.magnitude, p.back);
+        }
+        __syncthreads();
+        ready = true;
       }
-      __syncthreads();
-    }
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (first + j * kThreads < total)
-        unit[j].store(out + (t0 + token[j]) * p.ot + head[j] * p.oh, u[j], p.turned, p.rotary, p.interleaved,
-                      cs + token[j] * pairs);
+      for (int j = 0; j < J; ++j)
+        if (mine && r + j * step < rows)
+          unit[j].store(out + token[j] * p.ot + head[j] * p.oh, u, p.turned, p.rotary, p.interleaved,
+                        cs + token[j] * pairs);
+    }
   }
 }
 
@@ -67,14 +77,12 @@ int rope_run(const void* x, void* out, RopeParams p, cudaStream_t stream) {
   constexpr int J = 4;
   p.turned = rotary_units<V>(p.rotary, p.interleaved);
   p.units = p.turned + (x == out ? 0 : (p.dim - p.rotary) / V);  // in place, the rest is there already
-  p.by_units = FastDiv(p.units);
+  p.lanes = std::min(p.units, kThreads);
   p.by_heads = FastDiv(p.heads);
   p.by_pairs = FastDiv(p.rotary / 2);
-  // One batch of loads for a CTA, but for tokens enough to fill the SMs.
-  const int fill = std::max(1, J * kThreads / (p.heads * p.units));
-  p.per_cta = std::max(1, std::min(fill, p.tokens / kSMs));
-  const size_t smem = (size_t)p.per_cta * (p.rotary / 2) * sizeof(float2);
-  if (smem > 48 * 1024) p.per_cta = 48 * 1024 / ((p.rotary / 2) * (int)sizeof(float2));
+  // A few batches of loads for a CTA, but for tokens enough to fill the SMs.
+  const int fill = std::max(1, 4 * J * (kThreads / p.lanes) / p.heads);
+  p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 48 * 1024 / (p.rotary / 2 * (int)sizeof(float2))}));
   return launch_pdl(rope_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kThreads),
                     (size_t)p.per_cta * (p.rotary / 2) * sizeof(float2), stream, pdl_enabled(),
                     static_cast<const T*>(x), static_cast<T*>(out), p);
