@@ -91,9 +91,7 @@ __device__ __forceinline__ void turn(float& a, float& b, float2 r) {
 // A unit in registers between its load and its store, so that a thread has several
 // loads on their way before it needs the first.  cs: cos and sin of the pairs, pair i at
 // place(i): two pairs to 16 bytes, and these of neighbouring units side by side, so that
-// the units of a warp read them without bank conflicts (in the pairs' own order, a unit's
-// 64 bytes beside the next one's, the reads kept shared memory 73% busy and the append of
-// 16384 tokens at 37 us).
+// the units of a warp read them without bank conflicts.
 template <class T, int V>
 struct Unit;
 
@@ -219,7 +217,8 @@ struct Pages {
   const int32_t* table;
   int32_t* counts;
   int* status;
-  int* ticket;
+  int* ticket;     // of an append
+  int* tickets;    // of an eviction's sequences
   int32_t* moves;  // eviction: per (sequence, head) two counts and a list of `capacity`
   FastDiv page_div;
   int num_pages, page_size, heads, dim, batch, pitch, capacity;
@@ -244,10 +243,10 @@ struct Pages {
 int paged_check(const Pi05PagedCache* c, const char* op, Pages* out);
 
 // Workspace of a cache: status word and ticket in the first 16640 bytes (as in the
-// engine's workspace, so that the same status call reads it), then the eviction's
-// move lists.
+// engine's workspace, so that the same status call reads it), then the eviction's tickets
+// and move lists.
 inline size_t paged_moves_bytes(const Pi05PagedCache* c) {
-  return (size_t)c->batch * c->n_kv_heads * ((size_t)c->pages_per_seq * c->page_size + 2) * sizeof(int32_t);
+  return (size_t)c->batch * (1 + c->n_kv_heads * ((size_t)c->pages_per_seq * c->page_size + 2)) * sizeof(int32_t);
 }
 
 }  // namespace pi05

@@ -49,7 +49,8 @@ int paged_check(const Pi05PagedCache* c, const char* op, Pages* out) {
   out->counts = c->counts;
   out->status = reinterpret_cast<int*>(ws + kWsStatusOffset);
   out->ticket = reinterpret_cast<int*>(ws + kWsCounterOffset);
-  out->moves = reinterpret_cast<int32_t*>(ws + kWsAccumOffset);
+  out->tickets = reinterpret_cast<int*>(ws + kWsAccumOffset);
+  out->moves = reinterpret_cast<int32_t*>(ws + kWsAccumOffset) + c->batch;
   out->page_div = FastDiv((uint32_t)c->page_size);
   out->num_pages = c->num_pages;
   out->page_size = c->page_size;
@@ -238,10 +239,19 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 }
 
 // ---- eviction ------------------------------------------------------------------
-// The rows of a (sequence, head) are ordered by a 32-bit key that sorts like the
-// weight; radix selection gives the key of the last row to go, and how many rows of
-// just that key go with it.
-constexpr int kSelectThreads = 1024;
+// A cluster of CTAs for each (sequence, head): each holds a run of the rows as 32-bit keys
+// that sort like the weight in shared memory, so that weights and positions are read from
+// memory once.  Radix selection, 11 bits a pass over all the cluster's histograms, gives
+// the key of the last row to go and how many rows of just that key go with it; then the
+// holes below the budget and the rows that fill them are counted, and listed in order.
+// Bound: latency (three passes and a count, each a cluster barrier).  One CTA that read
+// the weights from L2 in every pass took 100 us for 512 pairs of 2049 rows and 409 us for
+// 8 pairs of 65536.  With 8 bits a pass, 26 and 57 us: a weight's top 8 bits are its
+// sign and exponent but one bit, so that most rows of a pass add to the same few counters,
+// one after the other.  This form: EVICT_TOKEN and EVICT_LONG.
+constexpr int kFew = 4;  // rows to go that are looked for one by one
+constexpr int kBuckets = 2048;
+constexpr int kMaxKeys = 48 * 1024;  // that a CTA holds; later ones are worked out again
 constexpr int kMoveThreads = 256;
 
 __device__ __forceinline__ uint32_t evict_key(float w, int pos, long long recent_from, int sinks) {
@@ -252,127 +262,347 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, long long recent
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ uint32_t key_of_row(const Pages& c, int b, int h, int r, long long recent_from, int sinks,
-                                               bool* bad) {
-  int line;
-  const int page = c.page_of(b, r, &line);
-  if (!c.real(page)) {
-    *bad = true;
-    return 0u;
+__device__ __forceinline__ int4 ld_cluster4(const int4* p, uint32_t rank) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(mapa_shared(smem_u32(p), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster(const void* p, uint32_t rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+// Copies a row's key and value, weight and position; one warp.
+__device__ __forceinline__ void move_row(const Pages& c, int b, int h, int from_row, int to_row, int lane) {
+  int from_line, to_line;
+  const int from = c.page_of(b, from_row, &from_line), to = c.page_of(b, to_row, &to_line);
+  const size_t src = c.row_at(from, h, from_line), dst = c.row_at(to, h, to_line);
+  if (lane < c.dim / 8) {
+    const uint4 k = ld16(c.k + src + lane * 16), v = ld16(c.v + src + lane * 16);
+    st16(c.k + dst + lane * 16, k);
+    st16(c.v + dst + lane * 16, v);
   }
-  const size_t s = c.slot_at(page, h, line);
-  return evict_key(c.weight[s], c.pos[s], recent_from, sinks);
+  if (lane == 0) {
+    const size_t s = c.slot_at(from, h, from_line), t = c.slot_at(to, h, to_line);
+    c.weight[t] = c.weight[s];
+    c.pos[t] = c.pos[s];
+  }
+}
+
+// Sum of the first `n` (at most 32) of a warp's `x`.
+__device__ __forceinline__ int sum_before(const int* x, int n, int lane) {
+  return __reduce_add_sync(~0u, lane < n ? x[lane] : 0);
+}
+
+struct Victim {
+  uint32_t key;
+  int row;
+  __device__ __forceinline__ bool before(uint32_t k, int r) const { return key < k || (key == k && row < r); }
+};
+// The warp's least: lowest key, then lowest row.
+__device__ __forceinline__ Victim warp_least(Victim v) {
+  const uint32_t k = __reduce_min_sync(~0u, v.key);
+  return {k, (int)__reduce_min_sync(~0u, v.key == k ? (unsigned)v.row : 0x7fffffffu)};
 }
 
 // Moves of row list `moves`: [0] their number (-1: the sequence stays as it is), [1] the
 // rows left, then the holes, ascending, and from [2 + left] on the rows that fill them.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(Pages c, int budget, int recent, int sinks) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum[kSelectThreads / 32];
+// `move_here`: few enough to do them on the spot.  FIT: a CTA holds all its keys.
+template <int NT, bool FIT>
+__global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant__ Pages c, int budget, int recent,
+                                                          int sinks, int ctas, int held, int move_here) {
+  constexpr int NW = NT / 32;
+  extern __shared__ uint32_t keys[];  // [held]
+  __shared__ __align__(16) int hist[2][kBuckets];
+  __shared__ int warp_a[NW], warp_b[NW];
+  __shared__ int sh_bad, sh_counts[2];
   __shared__ uint32_t sh_prefix;
-  __shared__ int sh_want;
+  __shared__ int sh_want, sh_same;
+  __shared__ Victim warp_best[2][NW], cta_best[2];
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads, tid = threadIdx.x;
-  int32_t* moves = c.moves + (size_t)blockIdx.x * (c.capacity + 2);
+  const int pair = blockIdx.x / ctas, rank = blockIdx.x - pair * ctas;  // the grid is a line of clusters
+  const int b = pair / c.heads, h = pair - b * c.heads, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  int32_t* moves = c.moves + (size_t)pair * (c.capacity + 2);
   const int len = c.rows(b);
   const long long recent_from = (long long)c.counts[c.batch + b] - recent;
-  if (len <= budget) {
-    if (tid == 0) moves[0] = -1;
+  if (len <= budget) {  // the whole cluster alike
+    if (tid == 0 && rank == 0) moves[0] = -1;
     return;
   }
+  auto sync_all = [&]() {
+    if (ctas > 1) cluster_sync_all();
+    else __syncthreads();
+  };
+  auto peer = [&](const int* p, int r) { return ctas > 1 ? ld_cluster(p, r) : *p; };
+
+  // This CTA's rows, and a warp's among them: whole groups of 32 in order.
+  const int share = ((len + ctas - 1) / ctas + 31) & ~31, first = min(len, rank * share);
+  const int n = min(len - first, share);
   bool bad = false;
-  uint32_t prefix = 0;
-  int want = len - budget;  // the want-th smallest of the keys that begin with `prefix`
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    for (int r = tid; r < len; r += kSelectThreads) {
-      const uint32_t key = key_of_row(c, b, h, r, recent_from, sinks, &bad);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+  auto key_of = [&](int i) {
+    int line;
+    const int page = c.page_of(b, first + i, &line);
+    if (!c.real(page)) {
+      bad = true;
+      return 0u;
     }
-    if (__syncthreads_or(bad)) {
-      if (tid == 0) {
-        moves[0] = -1;
-        report_status(c.status, PI05_DEV_BAD_INDEX);
+    const size_t s = c.slot_at(page, h, line);
+    return evict_key(c.weight[s], c.pos[s], recent_from, sinks);
+  };
+  const int kept = FIT ? n : min(n, held);
+#pragma unroll 4
+  for (int i = tid; i < kept; i += NT) keys[i] = key_of(i);
+  for (int i = kept + tid; i < n; i += NT) key_of(i);  // for a bad page
+  auto key = [&](int i) { return FIT || i < held ? keys[i] : key_of(i); };
+  if (tid == 0) sh_bad = 0;
+  __syncthreads();
+  if (bad) sh_bad = 1;
+  sync_all();
+  int any_bad = 0;
+  for (int r = 0; r < ctas; ++r) any_bad |= peer(&sh_bad, r);
+  if (any_bad) {
+    if (tid == 0 && rank == 0) {
+      moves[0] = -1;
+      report_status(c.status, PI05_DEV_BAD_INDEX);
+    }
+    sync_all();  // nobody leaves while others look at its shared memory
+    return;
+  }
+  auto cut_count = [&]() {  // the head that is done last cuts the count, when all have read it
+    if (tid == 0 && rank == 0 && atom_add_acq_rel_gpu(&c.tickets[b], 1) == c.heads - 1) {
+      c.tickets[b] = 0;
+      c.counts[b] = budget;
+    }
+  };
+
+  // A few rows to go (one, in a program that evicts after every token): one by one, the
+  // least that comes after the last.
+  if (move_here && len - budget <= kFew) {
+    Victim gone[kFew];
+    const int few = len - budget;
+#pragma unroll
+    for (int v = 0; v < kFew; ++v) {
+      if (v >= few) break;
+      Victim best{0xffffffffu, 0x7fffffff};
+      for (int i = tid; i < n; i += NT) {
+        const uint32_t k = key(i);
+        if ((v == 0 || gone[v > 0 ? v - 1 : 0].before(k, first + i)) && !best.before(k, first + i)) best = {k, first + i};
       }
-      return;
+      best = warp_least(best);
+      if (lane == 0) warp_best[v & 1][w] = best;
+      __syncthreads();
+      best = warp_least(lane < NW ? warp_best[v & 1][lane] : Victim{0xffffffffu, 0x7fffffff});
+      if (ctas > 1) {
+        if (tid == 0) cta_best[v & 1] = best;
+        sync_all();
+        const int r = min(lane, ctas - 1);
+        best.key = (uint32_t)ld_cluster(&cta_best[v & 1].key, r);
+        best.row = ld_cluster(&cta_best[v & 1].row, r);
+        best = warp_least(best);
+      }
+      gone[v] = best;
     }
-    if (tid == 0) {
-      int sum = 0, i = 0;
-      while (sum + hist[i] < want) sum += hist[i++];
-      sh_prefix = prefix | ((uint32_t)i << shift);
-      sh_want = want - sum;
+    if (w == 0 && rank == 0) {
+      // Holes in order, and the rows from the budget on that stay, in order: lane v has the
+      // v-th victim and row budget + v.
+      int mine = 0x7fffffff;
+#pragma unroll
+      for (int v = 0; v < kFew; ++v)
+        if (v < few && lane == v) mine = gone[v].row;
+      bool stays = lane < few;
+      int at = 0;
+#pragma unroll
+      for (int v = 0; v < kFew; ++v) {
+        if (v < few && gone[v].row == budget + lane) stays = false;
+        if (v < few && gone[v].row < mine) ++at;
+      }
+      const uint32_t tails = __ballot_sync(~0u, stays);
+      for (int v = 0; v < __popc(tails); ++v) {
+        const int to = __shfl_sync(~0u, mine, __ffs(__ballot_sync(~0u, lane < few && at == v)) - 1);
+        move_row(c, b, h, budget + __fns(tails, 0, v + 1), to, lane);
+      }
+    }
+    if (ctas > 1) sync_all();  // nobody leaves while others look at its shared memory
+    cut_count();
+    return;
+  }
+
+  for (int i = tid; i < 2 * kBuckets; i += NT) (&hist[0][0])[i] = 0;
+  __syncthreads();
+  uint32_t prefix = 0;
+  int want = len - budget, same = 0;  // the want-th smallest of the keys that begin with `prefix`
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    int* mine = hist[pass & 1];
+    for (int g = w * 32; g < n; g += NT) {
+      const int i = g + lane;
+      const uint32_t k = i < n ? key(i) : 0u;
+      const bool in = i < n && (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits)));
+      // Rows of the same bucket as the warp's first (all protected, say, or all 0) in one go.
+      const uint32_t bucket = in ? (k >> shift) & ((1u << bits) - 1) : ~0u, lead = __shfl_sync(~0u, bucket, 0);
+      const uint32_t alike = __ballot_sync(~0u, in && bucket == lead);
+      if (lane == 0 && in) atomicAdd(&mine[bucket], __popc(alike));
+      else if (in && bucket != lead) atomicAdd(&mine[bucket], 1);
+    }
+    sync_all();
+    if (pass > 0)  // the buffer of the pass before: everybody has read it
+      for (int i = tid; i < kBuckets; i += NT) hist[1 - (pass & 1)][i] = 0;
+    // Four or eight buckets a thread, over all the cluster.
+    constexpr int Q = kBuckets / NT / 4;
+    int4 of[Q];
+    int sum = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int4* own = reinterpret_cast<const int4*>(mine) + tid * Q + q;
+      of[q] = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+      for (int r = 0; r < ctas; ++r) {
+        const int4 v = ctas > 1 ? ld_cluster4(own, r) : *own;
+        of[q].x += v.x;
+        of[q].y += v.y;
+        of[q].z += v.z;
+        of[q].w += v.w;
+      }
+      sum += of[q].x + of[q].y + of[q].z + of[q].w;
+    }
+    int incl = sum;
+    for (int sft = 1; sft < 32; sft <<= 1) {
+      const int u = __shfl_up_sync(~0u, incl, sft);
+      if (lane >= sft) incl += u;
+    }
+    if (lane == 31) warp_a[w] = incl;
+    __syncthreads();
+    incl += sum_before(warp_a, w, lane);
+    if (incl >= want && incl - sum < want) {
+      int before = incl - sum, bucket = tid * Q * 4;
+      bool found = false;
+      auto look = [&](int count) {
+        if (found) return;
+        if (before + count >= want) {
+          sh_prefix = prefix | ((uint32_t)bucket << shift);
+          sh_want = want - before;
+          sh_same = count;
+          found = true;
+        }
+        before += count;
+        ++bucket;
+      };
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        look(of[q].x);
+        look(of[q].y);
+        look(of[q].z);
+        look(of[q].w);
+      }
     }
     __syncthreads();
     prefix = sh_prefix;
     want = sh_want;
+    same = sh_same;
   }
-  // Rows in order: keys below `prefix` go, and the first `want` that equal it.
-  const int lane = tid & 31, w = tid >> 5;
-  int ties = 0, holes = 0, tails = 0;
-  for (int r0 = 0; r0 < len; r0 += kSelectThreads) {
-    const int r = r0 + tid;
-    const uint32_t key = r < len ? key_of_row(c, b, h, r, recent_from, sinks, &bad) : 0u;
-    const bool tie = r < len && key == prefix;
-    const uint32_t below = (1u << lane) - 1;
-    uint32_t m = __ballot_sync(~0u, tie);
-    __syncthreads();
-    if (lane == 0) warp_sum[w] = __popc(m);
-    __syncthreads();
-    int before = ties + __popc(m & below);
-    for (int i = 0; i < kSelectThreads / 32; ++i) {
-      if (i < w) before += warp_sum[i];
-      ties += warp_sum[i];
+
+  // Keys below `prefix` go, and the first `want` of those that equal it.  Warp w has the
+  // groups of 32 from w * per on.
+  const uint32_t below = (1u << lane) - 1;
+  const int per = (share / 32 + NW - 1) / NW, g0 = w * per;
+  int ties = 0;  // before this warp's rows
+  if (same > want) {
+    int count = 0;
+    for (int g = g0; g < g0 + per; ++g) {
+      const int i = g * 32 + lane;
+      count += __popc(__ballot_sync(~0u, i < n && key(i) == prefix));
     }
-    const bool gone = r < len && (key < prefix || (tie && before < want));
-    const bool hole = gone && r < budget, tail = r < len && !gone && r >= budget;
-    m = __ballot_sync(~0u, hole);
-    const uint32_t m2 = __ballot_sync(~0u, tail);
+    if (lane == 0) warp_a[w] = count;
     __syncthreads();
-    if (lane == 0) warp_sum[w] = __popc(m) | (__popc(m2) << 16);
-    __syncthreads();
-    int at_hole = holes + __popc(m & below), at_tail = tails + __popc(m2 & below);
-    for (int i = 0; i < kSelectThreads / 32; ++i) {
-      const int a = warp_sum[i] & 0xffff, t = warp_sum[i] >> 16;
-      if (i < w) at_hole += a, at_tail += t;
-      holes += a;
-      tails += t;
+    if (w == 0) {
+      const int sum = sum_before(warp_a, NW, lane);
+      if (lane == 0) sh_counts[0] = sum;
     }
-    if (hole) moves[2 + at_hole] = r;
-    if (tail) moves[2 + budget + at_tail] = r;
+    sync_all();
+    for (int r = 0; r < rank; ++r) ties += peer(&sh_counts[0], r);
+    ties += sum_before(warp_a, w, lane);
+    sync_all();  // before the counts are written anew
   }
-  if (tid == 0) {
-    moves[0] = holes;
+  auto classify = [&](int g, int& seen, bool& hole, bool& tail) {
+    const int i = g * 32 + lane, r = first + i;
+    const uint32_t k = i < n ? key(i) : ~0u;
+    bool gone = i < n && k < prefix;
+    const bool tie = i < n && k == prefix;
+    if (same > want) {
+      const uint32_t m = __ballot_sync(~0u, tie);
+      gone = gone || (tie && seen + __popc(m & below) < want);
+      seen += __popc(m);
+    } else {
+      gone = gone || tie;
+    }
+    hole = gone && r < budget;
+    tail = i < n && !gone && r >= budget;
+  };
+  int holes = 0, tails = 0, seen = ties;
+  for (int g = g0; g < g0 + per; ++g) {
+    bool hole, tail;
+    classify(g, seen, hole, tail);
+    holes += __popc(__ballot_sync(~0u, hole));
+    tails += __popc(__ballot_sync(~0u, tail));
+  }
+  if (lane == 0) {
+    warp_a[w] = holes;
+    warp_b[w] = tails;
+  }
+  __syncthreads();
+  if (w == 0) {
+    const int x = sum_before(warp_a, NW, lane), y = sum_before(warp_b, NW, lane);
+    if (lane == 0) sh_counts[0] = x, sh_counts[1] = y;
+  }
+  sync_all();
+  int all = 0, at_hole = 0, at_tail = 0;
+  for (int r = 0; r < ctas; ++r) {
+    const int x = peer(&sh_counts[0], r);
+    all += x;
+    if (r < rank) {
+      at_hole += x;
+      at_tail += peer(&sh_counts[1], r);
+    }
+  }
+  at_hole += sum_before(warp_a, w, lane);
+  at_tail += sum_before(warp_b, w, lane);
+  seen = ties;
+  for (int g = g0; g < g0 + per; ++g) {
+    bool hole, tail;
+    classify(g, seen, hole, tail);
+    const uint32_t m = __ballot_sync(~0u, hole), m2 = __ballot_sync(~0u, tail);
+    if (hole) moves[2 + at_hole + __popc(m & below)] = first + g * 32 + lane;
+    if (tail) moves[2 + budget + at_tail + __popc(m2 & below)] = first + g * 32 + lane;
+    at_hole += __popc(m);
+    at_tail += __popc(m2);
+  }
+  if (tid == 0 && rank == 0) {
+    moves[0] = all;
     moves[1] = budget;
   }
+  sync_all();  // the lists are written; and nobody leaves while others look at its shared memory
+  if (!move_here) return;
+  for (int m = rank * NW + w; m < all; m += ctas * NW) move_row(c, b, h, moves[2 + budget + m], moves[2 + m], lane);
+  cut_count();
 }
 
 // One warp per move.  Sources lie at or above the budget and targets below it, so no
 // move reads what another writes.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(Pages c) {
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ Pages c) {
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads;
   const int32_t* moves = c.moves + (size_t)blockIdx.x * (c.capacity + 2);
   const int n = moves[0];
   if (n < 0) return;
-  const int left = moves[1], lane = threadIdx.x & 31;
-  for (int m = blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5); m < n; m += gridDim.y * (kMoveThreads / 32)) {
-    int from_line, to_line;
-    const int from = c.page_of(b, moves[2 + left + m], &from_line), to = c.page_of(b, moves[2 + m], &to_line);
-    const size_t src = c.row_at(from, h, from_line), dst = c.row_at(to, h, to_line);
-    if (lane < c.dim / 8) {
-      const uint4 k = reinterpret_cast<const uint4*>(c.k + src)[lane], v = reinterpret_cast<const uint4*>(c.v + src)[lane];
-      reinterpret_cast<uint4*>(c.k + dst)[lane] = k;
-      reinterpret_cast<uint4*>(c.v + dst)[lane] = v;
-    }
-    if (lane == 0) {
-      const size_t s = c.slot_at(from, h, from_line), t = c.slot_at(to, h, to_line);
-      c.weight[t] = c.weight[s];
-      c.pos[t] = c.pos[s];
-    }
-  }
+  const int left = moves[1];
+  for (int m = blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5); m < n; m += gridDim.y * (kMoveThreads / 32))
+    move_row(c, b, h, moves[2 + left + m], moves[2 + m], threadIdx.x & 31);
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) c.counts[b] = left;
 }
 
@@ -485,13 +715,31 @@ int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int si
   }
   if (budget >= c.capacity) return PI05_OK;  // no sequence can hold more
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int rows = c.batch * c.heads;
-  rc = launch_pdl(evict_select_kernel, dim3(rows), dim3(kSelectThreads), 0, st, pdl_enabled(), c, budget, recent,
-                  sinks);
-  if (rc) return rc;
-  const int most = std::min(budget, c.capacity - budget);
-  const int chunks = std::min((most + kMoveThreads / 32 - 1) / (kMoveThreads / 32), std::max(1, kSMs * 16 / rows));
-  return launch_pdl(evict_move_kernel, dim3(rows, chunks), dim3(kMoveThreads), 0, st, pdl_enabled(), c);
+  const int pairs = c.batch * c.heads;
+  // CTAs of a pair: up to 8 while they hold 1024 rows each and find an SM of their own.
+  int ctas = 1;
+  while (ctas < 8 && pairs * ctas * 2 <= kSMs && c.capacity / (ctas * 2) >= 1024) ctas *= 2;
+  const int share = ((c.capacity + ctas - 1) / ctas + 31) & ~31, held = std::min(share, kMaxKeys);
+  const int most = std::min(budget, c.capacity - budget);  // moves of a pair
+  const int move_here = most <= 64 * ctas;
+  const size_t smem = (size_t)held * sizeof(uint32_t);
+  // More threads only for the rows that give each of them something to do: a pass over the
+  // buckets costs every thread the same.
+  const int threads = share <= 4096 ? 256 : 512;
+  auto kernel = held < share ? evict_select_kernel<512, false>
+                : threads == 256 ? evict_select_kernel<256, true> : evict_select_kernel<512, true>;
+  if (smem > 24 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
+    if (e != cudaSuccess) {
+      set_last_error("paged_evict: %s", cudaGetErrorString(e));
+      return PI05_ERR_LAUNCH;
+    }
+  }
+  rc = launch_pdl_cluster(kernel, dim3(pairs * ctas), dim3(threads), smem, st, pdl_enabled(), dim3(ctas), c, budget,
+                          recent, sinks, ctas, held, move_here);
+  if (rc || move_here) return rc;
+  const int chunks = std::min((most + kMoveThreads / 32 - 1) / (kMoveThreads / 32), std::max(1, kSMs * 16 / pairs));
+  return launch_pdl(evict_move_kernel, dim3(pairs, chunks), dim3(kMoveThreads), 0, st, pdl_enabled(), c);
 }
 
 }  // extern "C"
