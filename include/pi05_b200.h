@@ -448,9 +448,14 @@ typedef struct Pi05Rotary {
  * must not overlap it otherwise.  positions: int32, or int64 with positions_i64;
  * any sign.  tokens == 0 is a no-op.  Rotary embedding of modeling_gemma.py:151-216
  * for any position, layout, rotated part and scaling. */
-int pi05_rope(const void* x, void* out, int dtype, int tokens, int heads, int head_dim, long long x_token_stride,
-              long long x_head_stride, long long out_token_stride, long long out_head_stride, const void* positions,
-              int positions_i64, const Pi05Rotary* rotary, int transpose, void* stream);
+typedef struct Pi05RopeArgs {
+  const void* x;
+  void* out;
+  const void* positions; /* [tokens] */
+  long long x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  int dtype, tokens, heads, head_dim, positions_i64, transpose;
+} Pi05RopeArgs;
+int pi05_rope(const Pi05RopeArgs* args, const Pi05Rotary* rotary, void* stream);
 
 /* A key-value cache in pages, shared by `batch` sequences.  Row r of sequence b is
  * line r % page_size of page page_table[b, r / page_size].  Host struct of device

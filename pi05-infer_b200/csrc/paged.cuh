@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pi05_b200.h"
 #include "host_util.h"
 #include "ptx.cuh"
@@ -238,6 +240,23 @@ struct Pages {
     return ((size_t)page * heads + head) * page_size + line;
   }
 };
+
+// Lets a kernel have `bytes` of dynamic shared memory, once for each device (the call
+// costs a microsecond).  `done`: a static of the kernel's own.
+template <class K>
+int allow_smem(K kernel, int bytes, std::atomic<uint64_t>* done, const char* op) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (e == cudaSuccess && device < 64 && (done->load(std::memory_order_relaxed) & bit)) return PI05_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    set_last_error("%s: %s", op, cudaGetErrorString(e));
+    return PI05_ERR_LAUNCH;
+  }
+  done->fetch_or(bit, std::memory_order_relaxed);
+  return PI05_OK;
+}
 
 // Checks the struct and lays out its workspace.
 int paged_check(const Pi05PagedCache* c, const char* op, Pages* out);

@@ -697,12 +697,10 @@ int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream
   constexpr int kSmem = Tile<DP, NT>::kSmem;
   static_assert(kSmem <= 227 * 1024, "shared memory");
   auto kernel = paged_attention_kernel<T, DP, NT, FULL>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) {
-    set_last_error("paged_attention: %s", cudaGetErrorString(e));
-    return PI05_ERR_LAUNCH;
-  }
-  int rc = launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), kSmem, st, pdl_enabled(), p, tm[0], tm[1]);
+  static std::atomic<uint64_t> allowed{0};
+  int rc = allow_smem(kernel, kSmem, &allowed, "paged_attention");
+  if (rc) return rc;
+  rc = launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), kSmem, st, pdl_enabled(), p, tm[0], tm[1]);
   if (rc) return rc;
   rc = launch_pdl(paged_join_kernel<T, 8 * NT>, dim3(p.c.batch * p.q_heads), dim3(kFinishThreads), 0, st,
                   pdl_enabled(), p);

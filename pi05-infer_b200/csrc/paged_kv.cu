@@ -355,8 +355,24 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
     return evict_key(c.weight[s], c.pos[s], recent_from, sinks);
   };
   const int kept = FIT ? n : min(n, held);
-#pragma unroll 4
-  for (int i = tid; i < kept; i += NT) keys[i] = key_of(i);
+  constexpr int U = 8;  // rows of a thread whose table entries, then weights, are on their way at once
+  for (int i0 = tid; i0 < kept; i0 += U * NT) {
+    int page[U], line[U], pos[U];
+    float weight[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) page[j] = i0 + j * NT < kept ? c.page_of(b, first + i0 + j * NT, &line[j]) : -1;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const bool real = c.real(page[j]);
+      const size_t s = real ? c.slot_at(page[j], h, line[j]) : 0;
+      weight[j] = real ? c.weight[s] : 0.f;
+      pos[j] = real ? c.pos[s] : 0;
+      bad = bad || (!real && i0 + j * NT < kept);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (i0 + j * NT < kept) keys[i0 + j * NT] = evict_key(weight[j], pos[j], recent_from, sinks);
+  }
   for (int i = kept + tid; i < n; i += NT) key_of(i);  // for a bad page
   auto key = [&](int i) { return FIT || i < held ? keys[i] : key_of(i); };
   if (tid == 0) sh_bad = 0;
@@ -726,15 +742,12 @@ int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int si
   // More threads only for the rows that give each of them something to do: a pass over the
   // buckets costs every thread the same.
   const int threads = share <= 4096 ? 256 : 512;
-  auto kernel = held < share ? evict_select_kernel<512, false>
-                : threads == 256 ? evict_select_kernel<256, true> : evict_select_kernel<512, true>;
-  if (smem > 24 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
-    if (e != cudaSuccess) {
-      set_last_error("paged_evict: %s", cudaGetErrorString(e));
-      return PI05_ERR_LAUNCH;
-    }
-  }
+  const int which = held < share ? 2 : threads == 256 ? 0 : 1;
+  auto kernel = which == 2   ? evict_select_kernel<512, false>
+                : which == 0 ? evict_select_kernel<256, true>
+                             : evict_select_kernel<512, true>;
+  static std::atomic<uint64_t> allowed[3];
+  if (smem > 24 * 1024 && (rc = allow_smem(kernel, kMaxKeys * 4, &allowed[which], "paged_evict"))) return rc;
   rc = launch_pdl_cluster(kernel, dim3(pairs * ctas), dim3(threads), smem, st, pdl_enabled(), dim3(ctas), c, budget,
                           recent, sinks, ctas, held, move_here);
   if (rc || move_here) return rc;

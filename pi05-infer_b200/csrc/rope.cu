@@ -102,47 +102,44 @@ int rope_type(const void* x, void* out, const RopeParams& p, cudaStream_t stream
 
 using namespace pi05;
 
-extern "C" int pi05_rope(const void* x, void* out, int dtype, int tokens, int heads, int head_dim,
-                         long long x_token_stride, long long x_head_stride, long long out_token_stride,
-                         long long out_head_stride, const void* positions, int positions_i64, const Pi05Rotary* rotary,
-                         int transpose, void* stream) {
-  if (rotary == nullptr || (tokens > 0 && (x == nullptr || out == nullptr || positions == nullptr)) ||
-      rotary->turns == nullptr) {
+extern "C" int pi05_rope(const Pi05RopeArgs* a, const Pi05Rotary* rotary, void* stream) {
+  if (a == nullptr || rotary == nullptr || rotary->turns == nullptr ||
+      (a->tokens > 0 && (a->x == nullptr || a->out == nullptr || a->positions == nullptr))) {
     set_last_error("rope: null pointer");
     return PI05_ERR_INVALID_ARG;
   }
-  if (dtype != PI05_BF16 && dtype != PI05_FP16 && dtype != PI05_FP32) {
-    set_last_error("rope: dtype %d is not bf16, fp16 or fp32", dtype);
+  if (a->dtype != PI05_BF16 && a->dtype != PI05_FP16 && a->dtype != PI05_FP32) {
+    set_last_error("rope: dtype %d is not bf16, fp16 or fp32", a->dtype);
     return PI05_ERR_INVALID_ARG;
   }
   const int r = rotary->rotary_dim;
-  if (tokens < 0 || heads <= 0 || head_dim <= 0 || r <= 0 || r % 2 || r > head_dim || r > kMaxRotary ||
-      (long long)heads * head_dim > (1 << 24)) {
-    set_last_error("rope: bad shape tokens=%d heads=%d head_dim=%d rotary_dim=%d", tokens, heads, head_dim, r);
+  if (a->tokens < 0 || a->heads <= 0 || a->head_dim <= 0 || r <= 0 || r % 2 || r > a->head_dim || r > kMaxRotary ||
+      (long long)a->heads * a->head_dim > (1 << 24)) {
+    set_last_error("rope: bad shape tokens=%d heads=%d head_dim=%d rotary_dim=%d", a->tokens, a->heads, a->head_dim, r);
     return PI05_ERR_SHAPE;
   }
-  if (x == out && (x_token_stride != out_token_stride || x_head_stride != out_head_stride)) {
+  if (a->x == a->out && (a->x_token_stride != a->out_token_stride || a->x_head_stride != a->out_head_stride)) {
     set_last_error("rope: in place needs the same strides");
     return PI05_ERR_INVALID_ARG;
   }
-  if (tokens == 0) return PI05_OK;
+  if (a->tokens == 0) return PI05_OK;
   RopeParams p;
-  p.xt = x_token_stride;
-  p.xh = x_head_stride;
-  p.ot = out_token_stride;
-  p.oh = out_head_stride;
-  p.positions = positions;
+  p.xt = a->x_token_stride;
+  p.xh = a->x_head_stride;
+  p.ot = a->out_token_stride;
+  p.oh = a->out_head_stride;
+  p.positions = a->positions;
   p.turns = rotary->turns;
-  p.pos64 = positions_i64;
-  p.tokens = tokens;
-  p.heads = heads;
-  p.dim = head_dim;
+  p.pos64 = a->positions_i64;
+  p.tokens = a->tokens;
+  p.heads = a->heads;
+  p.dim = a->head_dim;
   p.rotary = r;
   p.interleaved = rotary->interleaved;
-  p.back = transpose;
+  p.back = a->transpose;
   p.magnitude = rotary->magnitude;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == PI05_BF16) return rope_type<__nv_bfloat16>(x, out, p, st);
-  if (dtype == PI05_FP16) return rope_type<__half>(x, out, p, st);
-  return rope_type<float>(x, out, p, st);
+  if (a->dtype == PI05_BF16) return rope_type<__nv_bfloat16>(a->x, a->out, p, st);
+  if (a->dtype == PI05_FP16) return rope_type<__half>(a->x, a->out, p, st);
+  return rope_type<float>(a->x, a->out, p, st);
 }

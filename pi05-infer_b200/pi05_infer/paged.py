@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -37,10 +38,19 @@ _Z = ctypes.c_size_t
 _F = ctypes.c_float
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POSITIONS = (torch.int32, torch.int64)
 
 
 class Pi05Rotary(ctypes.Structure):
     _fields_ = [("turns", _P), ("rotary_dim", _I), ("interleaved", _I), ("magnitude", _F)]
+
+
+class Pi05RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _P), ("out", _P), ("positions", _P), ("x_token_stride", _L), ("x_head_stride", _L),
+        ("out_token_stride", _L), ("out_head_stride", _L), ("dtype", _I), ("tokens", _I), ("heads", _I),
+        ("head_dim", _I), ("positions_i64", _I), ("transpose", _I),
+    ]
 
 
 class Pi05PagedCache(ctypes.Structure):
@@ -57,8 +67,7 @@ class Pi05PagedAppend(ctypes.Structure):
     _fields_ = [
         ("k", _P), ("v", _P), ("k_token_stride", _L), ("k_head_stride", _L), ("v_token_stride", _L),
         ("v_head_stride", _L), ("q", _P), ("q_out", _P), ("q_token_stride", _L), ("q_head_stride", _L),
-        ("tokens", _I), ("n_q_heads", _I), ("cu_tokens", _P), ("new_weight", _P),
-        ("rotary", ctypes.POINTER(Pi05Rotary)),
+        ("tokens", _I), ("n_q_heads", _I), ("cu_tokens", _P), ("new_weight", _P), ("rotary", _P),
     ]
 
 
@@ -69,14 +78,19 @@ class Pi05PagedAttention(ctypes.Structure):
     ]
 
 
-_CACHE = ctypes.POINTER(Pi05PagedCache)
+# The argument structs as bytes: packing one takes a fifth of the time that filling a ctypes
+# structure does, and these calls come once for every token.
+_ROPE_ARGS = struct.Struct("@3P4q6i")
+_APPEND_ARGS = struct.Struct("@2P4q2P2q2i3P")
+_ATTEND_ARGS = struct.Struct("@4P3q2ifiPN")
+
 _lib.SIGNATURES.update({
-    "pi05_rope": (_I, [_P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _P, _I, ctypes.POINTER(Pi05Rotary), _I, _P]),
-    "pi05_paged_workspace_bytes": (_Z, [_CACHE]),
-    "pi05_paged_append": (_I, [_CACHE, ctypes.POINTER(Pi05PagedAppend), _P]),
-    "pi05_paged_attention_scratch_bytes": (_Z, [_CACHE, _I, _I]),
-    "pi05_paged_attention": (_I, [_CACHE, ctypes.POINTER(Pi05PagedAttention), _P]),
-    "pi05_paged_evict": (_I, [_CACHE, _I, _I, _I, _P]),
+    "pi05_rope": (_I, [_P, _P, _P]),
+    "pi05_paged_workspace_bytes": (_Z, [_P]),
+    "pi05_paged_append": (_I, [_P, _P, _P]),
+    "pi05_paged_attention_scratch_bytes": (_Z, [_P, _I, _I]),
+    "pi05_paged_attention": (_I, [_P, _P, _P]),
+    "pi05_paged_evict": (_I, [_P, _I, _I, _I, _P]),
 })
 _fns = {}
 
@@ -90,14 +104,19 @@ def _fn(name: str):
     return f
 
 
-def _run(name: str, device: torch.device, *args) -> None:
-    """Calls the library on the current stream of ``device``, whichever device is current."""
-    index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            rc = _fn(name)(*args, torch.cuda.current_stream(index).cuda_stream)
+# The current stream's handle and the current device without the objects around them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _run(name: str, index: int, *args) -> None:
+    """Calls the library on the current stream of device ``index``, whichever device is current."""
+    if index == _raw_device():
+        rc = _fn(name)(*args, _raw_stream(index))
     else:
-        rc = _fn(name)(*args, torch.cuda.current_stream(index).cuda_stream)
+        with torch.cuda.device(index):
+            rc = _fn(name)(*args, _raw_stream(index))
     if rc != _lib.PI05_OK:
         raise _lib.Pi05Error(name, rc, _lib.last_error())
 
@@ -178,15 +197,18 @@ class RopeFrequencies:
         turns = _turns(self.inv_freq)
         self.device = _cuda(device)
         self.turns = torch.tensor(turns, dtype=torch.int64).to(self.device)
-        self.c = Pi05Rotary(self.turns.data_ptr(), rotary_dim, int(layout == "interleaved"), self.magnitude)
-        self._ref = ctypes.byref(self.c)
+        self._index = self.device.index
+        self._c = Pi05Rotary(self.turns.data_ptr(), rotary_dim, int(layout == "interleaved"), self.magnitude)
+        self._at = ctypes.addressof(self._c)
 
 
 def _rope(x, positions, freqs, out, transpose):
     tokens, heads, dim = x.shape
-    _run("pi05_rope", x.device, x.data_ptr(), out.data_ptr(), _DTYPES[x.dtype], tokens, heads, dim, x.stride(0),
-         x.stride(1), out.stride(0), out.stride(1), positions.data_ptr(), positions.dtype == torch.int64, freqs._ref,
-         transpose)
+    xt, xh, _ = x.stride()
+    ot, oh, _ = out.stride()
+    _run("pi05_rope", freqs._index, _ROPE_ARGS.pack(
+        x.data_ptr(), out.data_ptr(), positions.data_ptr(), xt, xh, ot, oh, _DTYPES[x.dtype], tokens, heads, dim,
+        positions.dtype == torch.int64, transpose), freqs._at)
     return out
 
 
@@ -195,7 +217,7 @@ class _Rope(torch.autograd.Function):
     def forward(ctx, x, positions, freqs, transpose):
         ctx.save_for_backward(positions)
         ctx.freqs, ctx.transpose = freqs, transpose
-        return _rope(x, positions, freqs, torch.empty(x.shape, dtype=x.dtype, device=x.device), transpose)
+        return _rope(x, positions, freqs, torch.empty_like(x), transpose)
 
     @staticmethod
     def backward(ctx, g):
@@ -233,10 +255,11 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
     """
     if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda or x.stride(2) != 1:
         raise ValueError("x must be a [tokens, heads, dim] CUDA tensor, bf16, fp16 or fp32, contiguous in dim")
-    if positions.shape != x.shape[:1] or positions.dtype not in (torch.int32, torch.int64) or \
-            positions.device != x.device or not positions.is_contiguous():
+    index = x.get_device()
+    if positions.shape != x.shape[:1] or positions.dtype not in _POSITIONS or positions.get_device() != index or \
+            not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32 or int64 [tokens] on x's device")
-    if freqs.device != x.device:
+    if freqs._index != index:
         raise ValueError(f"the frequencies are on {freqs.device}, x is on {x.device}")
     if freqs.rotary_dim > x.shape[2]:
         raise ValueError(f"rotary_dim {freqs.rotary_dim} is more than the head's {x.shape[2]} values")
@@ -247,10 +270,10 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
             y = _Rope.apply(x, positions, freqs, bool(transpose))
             del node
             return y
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x)
     elif grad:
         raise ValueError("out= is not differentiable")
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
+    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index or out.stride(2) != 1:
         raise ValueError("out must have x's shape, type and device, contiguous in dim")
     return _rope(x, positions, freqs, out, bool(transpose))
 
@@ -306,12 +329,12 @@ class PagedKVCache:
             p(k_pages), p(v_pages), *k_pages.stride()[:3], p(weight), p(pos), p(page_table), p(counts),
             _DTYPES[self.dtype], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, self.batch,
             self.pages_per_seq, page_table.stride(0), None, 0)
-        self._ref = ctypes.byref(self._c)
-        nbytes = _fn("pi05_paged_workspace_bytes")(self._ref)
+        self._at, self._index = ctypes.addressof(self._c), device.index
+        nbytes = _fn("pi05_paged_workspace_bytes")(self._at)
         # status word, ticket and the eviction's lists; zeroed once
         self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         self._c.workspace, self._c.workspace_bytes = self.workspace.data_ptr(), nbytes
-        self._scratch_bytes = {}
+        self._scratch = {}  # (heads, track): bytes, and a tensor of one byte that looks like so many
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, batch: int, pages_per_seq: int, *,
@@ -334,7 +357,7 @@ class PagedKVCache:
         return self.counts[0]
 
     def _rows(self, t: torch.Tensor, name: str, heads: Optional[int]) -> None:
-        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or t.shape[2] != self.head_dim or \
+        if t.dim() != 3 or t.dtype != self.dtype or t.get_device() != self._index or t.shape[2] != self.head_dim or \
                 t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
@@ -357,8 +380,7 @@ class PagedKVCache:
         tokens = k.shape[0]
         if v.shape[0] != tokens:
             raise ValueError(f"k has {tokens} tokens, v has {v.shape[0]}")
-        a = Pi05PagedAppend(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        a.tokens = tokens
+        q_at = q_out_at = q_token = q_head = n_q_heads = rotary = cu_at = weight_at = 0
         if q is not None:
             self._rows(q, "q", None)
             if freqs is None:
@@ -366,30 +388,34 @@ class PagedKVCache:
             if q.shape[0] != tokens:
                 raise ValueError(f"k has {tokens} tokens, q has {q.shape[0]}")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device or \
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.get_device() != self._index or \
                     not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous, of q's shape, type and device")
-            a.q, a.q_out, a.q_token_stride, a.q_head_stride = q.data_ptr(), q_out.data_ptr(), q.stride(0), q.stride(1)
-            a.n_q_heads = q.shape[1]
+            q_at, q_out_at, n_q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+            q_token, q_head, _ = q.stride()
         if freqs is not None:
-            if freqs.device != self.device or freqs.rotary_dim > self.head_dim:
+            if freqs._index != self._index or freqs.rotary_dim > self.head_dim:
                 raise ValueError(f"freqs must be on {self.device} with rotary_dim <= {self.head_dim}")
-            a.rotary = ctypes.pointer(freqs.c)
+            rotary = freqs._at
         if cu_tokens is not None:
             if cu_tokens.shape != (self.batch + 1,) or cu_tokens.dtype != torch.int32 or \
-                    cu_tokens.device != self.device or not cu_tokens.is_contiguous():
+                    cu_tokens.get_device() != self._index or not cu_tokens.is_contiguous():
                 raise ValueError(f"cu_tokens must be contiguous int32 [{self.batch + 1}] on {self.device}")
-            a.cu_tokens = cu_tokens.data_ptr()
+            cu_at = cu_tokens.data_ptr()
         elif tokens != self.batch:
             raise ValueError(f"{tokens} tokens for {self.batch} sequences need cu_tokens")
         if weight is not None:
             if self.weight is None or weight.shape != (tokens, self.n_kv_heads) or weight.dtype != torch.float32 or \
-                    weight.device != self.device or not weight.is_contiguous():
+                    weight.get_device() != self._index or not weight.is_contiguous():
                 raise ValueError(f"weight must be contiguous fp32 [{tokens}, {self.n_kv_heads}] on {self.device}, "
                                  "for a cache that keeps weights")
-            a.new_weight = weight.data_ptr()
-        _run("pi05_paged_append", self.device, self._ref, ctypes.byref(a))
+            weight_at = weight.data_ptr()
+        k_token, k_head, _ = k.stride()
+        v_token, v_head, _ = v.stride()
+        _run("pi05_paged_append", self._index, self._at, _APPEND_ARGS.pack(
+            k.data_ptr(), v.data_ptr(), k_token, k_head, v_token, v_head, q_at, q_out_at, q_token, q_head, tokens,
+            n_q_heads, cu_at, weight_at, rotary))
         return q_out if q is not None else None
 
     def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, key_valid: Optional[torch.Tensor] = None,
@@ -411,28 +437,31 @@ class PagedKVCache:
         if track and self.weight is None:
             raise ValueError("this cache keeps no weights: build it with weight=")
         if out is None:
-            out = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != self._index or \
+                not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape, type and device")
-        lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if return_lse else None
-        pitch = valid_rows = 0
+        lse = q.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
+        valid_at = pitch = valid_rows = 0
         if key_valid is not None:
             if key_valid.dim() != 2 or key_valid.dtype not in (torch.bool, torch.uint8) or \
-                    key_valid.shape[0] != batch or key_valid.device != self.device or key_valid.stride(1) != 1:
+                    key_valid.shape[0] != batch or key_valid.get_device() != self._index or key_valid.stride(1) != 1:
                 raise ValueError("key_valid must be bool or uint8 [batch, rows] on the cache's device, rows contiguous")
-            pitch, valid_rows = key_valid.stride(0), key_valid.shape[1]
-        need = self._scratch_bytes.get((heads, track))
-        if need is None:
-            need = self._scratch_bytes[heads, track] = _fn("pi05_paged_attention_scratch_bytes")(
-                self._ref, heads, track)
+            valid_at, pitch, valid_rows = key_valid.data_ptr(), key_valid.stride(0), key_valid.shape[1]
+        need, like = self._scratch.get((heads, track)) or self._need(heads, track)
         # from torch's allocator, call by call: calls on different streams, and graphs, never share it
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a = Pi05PagedAttention(
-            q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-            None if key_valid is None else key_valid.data_ptr(), q.stride(0), q.stride(1), pitch, valid_rows, heads,
-            dim**-0.5 if scale is None else scale, track, scratch.data_ptr(), need)
-        _run("pi05_paged_attention", self.device, self._ref, ctypes.byref(a))
+        scratch = torch.empty_like(like, memory_format=torch.contiguous_format)
+        q_token, q_head, _ = q.stride()
+        _run("pi05_paged_attention", self._index, self._at, _ATTEND_ARGS.pack(
+            q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), valid_at, q_token, q_head, pitch,
+            valid_rows, heads, dim**-0.5 if scale is None else scale, track, scratch.data_ptr(), need))
         return (out, lse) if return_lse else out
+
+    def _need(self, heads: int, track: bool):
+        need = _fn("pi05_paged_attention_scratch_bytes")(self._at, heads, track)
+        like = torch.empty(1, dtype=torch.uint8, device=self.device).expand(need)
+        self._scratch[heads, track] = need, like
+        return need, like
 
     def evict(self, budget: int, *, recent: int = 0, sinks: int = 0) -> None:
         """Cuts every sequence with more than ``budget`` rows down to it.
@@ -447,7 +476,7 @@ class PagedKVCache:
             raise ValueError("this cache keeps no weights and positions: build it with weight= and pos=")
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
             raise ValueError(f"need budget >= 1 and 0 <= recent + sinks <= budget, got {budget}, {recent}, {sinks}")
-        _run("pi05_paged_evict", self.device, self._ref, budget, recent, sinks)
+        _run("pi05_paged_evict", self._index, self._at, budget, recent, sinks)
 
     def read_status(self) -> int:
         """Synchronise, read and clear the cache's device status word (0 = nothing went wrong)."""

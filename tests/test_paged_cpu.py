@@ -59,7 +59,7 @@ def test_bad_arguments_are_refused():
         a = paged.Pi05PagedAppend(HERE, HERE, 128, 64, 128, 64)
         a.tokens = 3
         if rotary is not None:
-            a.rotary = ctypes.pointer(rotary)
+            a.rotary = ctypes.addressof(rotary)
         for n, v in kw.items():
             setattr(a, n, v)
         return call("pi05_paged_append", cache(weight=None) if "new_weight" in kw else cache(), ctypes.byref(a), None)[0]
@@ -96,8 +96,8 @@ def test_bad_arguments_are_refused():
     assert call("pi05_paged_evict", cache(), 64, 1, 1, None)[0] == 0  # 4 pages of 16: none can hold more
 
     def turn(x=HERE, out=HERE, dtype=0, tokens=2, heads=3, dim=64, xt=192, xh=64, ot=192, oh=64, pos=HERE, r=rot):
-        return call("pi05_rope", x, out, dtype, tokens, heads, dim, xt, xh, ot, oh, pos, 0,
-                    ctypes.byref(r) if r else None, 0, None)[0]
+        a = paged.Pi05RopeArgs(x, out, pos, xt, xh, ot, oh, dtype, tokens, heads, dim, 0, 0)
+        return call("pi05_rope", ctypes.byref(a), ctypes.byref(r) if r else None, None)[0]
 
     assert turn(x=None) == 1 and turn(out=None) == 1 and turn(pos=None) == 1 and turn(r=None) == 1
     assert turn(r=paged.Pi05Rotary(None, 64, 0, 1.0)) == 1 and turn(dtype=3) == 1
@@ -117,7 +117,7 @@ def test_sizes():
 
 
 def test_struct_layout_matches_header():
-    types = (paged.Pi05Rotary, paged.Pi05PagedCache, paged.Pi05PagedAppend, paged.Pi05PagedAttention)
+    types = (paged.Pi05Rotary, paged.Pi05RopeArgs, paged.Pi05PagedCache, paged.Pi05PagedAppend, paged.Pi05PagedAttention)
     src = "#include <stdio.h>\n#include <stddef.h>\n#include \"pi05_b200.h\"\nint main(void) {\n"
     for t in types:
         src += f'printf("{t.__name__} sizeof %zu\\n", sizeof({t.__name__}));\n'
@@ -131,6 +131,18 @@ def test_struct_layout_matches_header():
     for line in out.splitlines():
         t, f, n = line.split()
         assert (ctypes.sizeof(by[t]) if f == "sizeof" else getattr(by[t], f).offset) == int(n), line
+
+
+@pytest.mark.parametrize("packed,cls", [
+    (paged._ROPE_ARGS, paged.Pi05RopeArgs), (paged._APPEND_ARGS, paged.Pi05PagedAppend),
+    (paged._ATTEND_ARGS, paged.Pi05PagedAttention),
+])
+def test_packed_arguments_match_the_structs(packed, cls):
+    """Each field, packed with a value of its own, comes back under its name."""
+    values = list(range(1, len(cls._fields_) + 1))
+    a = cls.from_buffer_copy(packed.pack(*values))
+    assert packed.size == ctypes.sizeof(cls)
+    assert [getattr(a, f) for f, _ in cls._fields_] == values
 
 
 @pytest.mark.parametrize("rotary,base,scaling,factor,original", [
