@@ -26,6 +26,7 @@
 // instructions a tile, and 8 warps an SM are too few to hide them); with a bulk copy for
 // each row, issued one by one: 174 us with 12 warps, 206 us with 8.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -99,16 +100,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
 
 // A tile of 16 rows: boxes of 64 columns, 16 rows of 128 bytes each, whose 16-byte chunk
 // c of row r lies at chunk c ^ (r & 7) (the 128-byte swizzle): ldmatrix without conflicts.
-template <int DP, int NT>
+// KS: steps of 16 columns that the products take; what lies beyond a head is zeros.
+template <int KS, int NT>
 struct Tile {
+  static constexpr int kBoxes = (KS + 3) / 4;
   static constexpr int kBox = kWarpRows * 128;
-  static constexpr int kBytes = DP / 64 * kBox;
-  static constexpr int kStages = DP == 256 && NT == 1 ? 3 : 2;
+  static constexpr int kBytes = kBoxes * kBox;
+  static constexpr int kStages = kBoxes == 4 && NT == 1 ? 3 : 2;
   static constexpr int kRing = kWarps * kStages * 2 * kBytes;
-  static constexpr int kSlot = (DP / 16 * NT * 4 + NT * 4) * 32 * 4;  // a warp's o, m and l, at a segment's end
+  static constexpr int kSlot = (KS * NT * 4 + NT * 4) * 32 * 4;  // a warp's o, m and l, at a segment's end
   static constexpr int kSmem = 1024 + kRing + 2 * kSlot;
   // CTAs on an SM: as many as shared memory and the accumulators' registers leave room for.
-  static constexpr int kPerSM = DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 1;
+  static constexpr int kPerSM = kBoxes == 1 ? (NT == 1 ? 4 : 3) : kBoxes == 2 ? (NT == 1 ? 3 : 2) : kBoxes == 3 && NT == 1 ? 2 : 1;
   static_assert(kPerSM * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -167,21 +170,28 @@ __device__ __forceinline__ Ref look_up(const AttnParams& p, const Segment& s, in
 // Starts the copies of a tile's K and V by TMA, `p.box_rows` rows of 64 columns at a time
 // (the largest power of two that divides the page size, so that a box lies in one page);
 // a lane for each group of rows.  Returns a bit for each row that counts.
-template <int DP, int NT>
+template <int KS, int NT>
 __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
                                           const Ref& ref, uint64_t* bar, uint32_t dst, int lane) {
-  using L = Tile<DP, NT>;
+  using L = Tile<KS, NT>;
   const bool real = p.c.real(ref.page);
   if (ref.counts && !real) report_status(p.c.status, PI05_DEV_BAD_INDEX);
   const uint32_t mask = __ballot_sync(~0u, ref.counts && real) & 0xffff;
-  const bool mine = lane < kWarpRows && (lane & (p.box_rows - 1)) == 0 && (mask >> lane & ((1u << p.box_rows) - 1)) != 0;
-  const int groups = __popc(__ballot_sync(~0u, mine));
-  if (lane == 0) mbar_arrive_expect_tx(bar, groups * p.box_rows * 128 * (DP / 64) * 2);
-  __syncwarp();
+  constexpr uint32_t kRowBytes = 128 * L::kBoxes * 2;  // of a box row, over all boxes of K and V
+  bool mine;
+  if (p.box_rows == kWarpRows) {
+    mine = lane == 0 && mask != 0;
+    if (lane == 0) mbar_arrive_expect_tx(bar, mask != 0 ? kWarpRows * kRowBytes : 0);
+  } else {
+    mine = lane < kWarpRows && (lane & (p.box_rows - 1)) == 0 && (mask >> lane & ((1u << p.box_rows) - 1)) != 0;
+    const int groups = __popc(__ballot_sync(~0u, mine));
+    if (lane == 0) mbar_arrive_expect_tx(bar, groups * p.box_rows * kRowBytes);
+    __syncwarp();
+  }
   if (mine) {
     const uint32_t to = dst + lane * 128, at = smem_u32(bar);
 #pragma unroll
-    for (int i = 0; i < DP / 64; ++i) {
+    for (int i = 0; i < L::kBoxes; ++i) {
       tma_load_4d(to + i * L::kBox, tm_k, at, i * 64, ref.line, ref.kvh, ref.page);
       tma_load_4d(to + L::kBytes + i * L::kBox, tm_v, at, i * 64, ref.line, ref.kvh, ref.page);
     }
@@ -189,12 +199,12 @@ __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap
   return mask;
 }
 
-template <class T, int DP, int NT, bool FULL>
-__global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
+template <class T, int KS, int NT>
+__global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
     paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v) {
-  using L = Tile<DP, NT>;
-  constexpr int H = 8 * NT, KS = DP / 16, S = L::kStages;
+  using L = Tile<KS, NT>;
+  constexpr int H = 8 * NT, S = L::kStages;
   extern __shared__ char smem_raw[];
   __shared__ long long sh_sum[kWarps];
   __shared__ long long sh_base;
@@ -253,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
   const uint32_t ring = base_addr + w * S * 2 * L::kBytes;
   float* slots = reinterpret_cast<float*>(smem_raw + (base_addr - smem_u32(smem_raw)) + L::kRing);
   uint64_t* bars = all_bars + w * S;
-  const int d = FULL ? DP : p.c.dim, steps = FULL ? KS : (d + 15) / 16;
+  const int d = p.c.dim;
 
   // The warp's copies run ahead of its products, across the segments' borders.
   Walk ahead{sh_b, sh_base, lo, hi}, walk = ahead;
@@ -274,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
   for (int j = 0; j < S - 1; ++j) {
     const Ref now = ref;
     ref = next_ref();
-    live[j] = now.tile ? fetch<DP, NT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane) : 0u;
+    live[j] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane) : 0u;
   }
   int stage = 0;
   uint32_t phase = 0;
@@ -332,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
         const Ref now = ref;
         ref = next_ref();
         const int to = stage == 0 ? S - 1 : stage - 1;
-        live[S - 1] = now.tile ? fetch<DP, NT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane) : 0u;
+        live[S - 1] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane) : 0u;
       }
       const uint32_t tile = ring + stage * 2 * L::kBytes, rows = live[0];
       if (++stage == S) {
@@ -370,10 +380,10 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
         uint32_t a[B][4];
 #pragma unroll
         for (int ks = 0; ks < B; ++ks)
-          if (FULL || k0 + ks < steps) ldsm4(a[ks], step_at(tile + k_lane, k0 + ks));
+          if (k0 + ks < KS) ldsm4(a[ks], step_at(tile + k_lane, k0 + ks));
 #pragma unroll
         for (int ks = 0; ks < B; ++ks)
-          if (FULL || k0 + ks < steps) {
+          if (k0 + ks < KS) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816<T>(ks & 1 ? x2[nt] : x[nt], a[ks], qf[k0 + ks][nt]);
           }
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
       uint32_t va[B][4];
 #pragma unroll
       for (int ks = 0; ks < B; ++ks)
-        if (FULL || ks < steps) load_v(va[ks], ks);
+        load_v(va[ks], ks);
       uint32_t pf[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -423,11 +433,11 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
         if (k0 > 0) {
 #pragma unroll
           for (int ks = 0; ks < B; ++ks)
-            if (FULL || k0 + ks < steps) load_v(va[ks], k0 + ks);
+            if (k0 + ks < KS) load_v(va[ks], k0 + ks);
         }
 #pragma unroll
         for (int ks = 0; ks < B; ++ks)
-          if (FULL || k0 + ks < steps) {
+          if (k0 + ks < KS) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[k0 + ks][nt], va[ks], pf[nt]);
           }
@@ -498,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, Tile<DP, NT>::kPerSM)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int x = ks * 16 + k * 8 + (lane >> 2);
-              if (!FULL && x >= d) continue;
+              if (x >= d) continue;
               const float v = o[ks][nt][i + 2 * k];
               if (s.whole) out[x] = from_f32<T>(sum == 0.f ? 0.f : v * scale);
               else part[x] = v;
@@ -654,14 +664,32 @@ __global__ void __launch_bounds__(kFinishThreads) paged_track_kernel(const __gri
 
 // ---- host ----------------------------------------------------------------------
 struct Plan {
-  int nt, parts, dp, ctas, rows, score_pitch;
+  int nt, parts, ks, ctas, rows, score_pitch;
   size_t part_o, part_ml, row_info, row_lse, scores, bytes;
 };
 
-int per_sm(int dp, int nt) {
-  if (dp == 64) return nt == 1 ? Tile<64, 1>::kPerSM : Tile<64, 2>::kPerSM;
-  if (dp == 128) return nt == 1 ? Tile<128, 1>::kPerSM : Tile<128, 2>::kPerSM;
-  return nt == 1 ? Tile<256, 1>::kPerSM : Tile<256, 2>::kPerSM;
+// Steps of 16 columns that there are kernels for: every even size up to 12 and 5, which
+// heads of 72 and 80 need, then 16.
+int steps_for(int dim) {
+  const int need = (dim + 15) / 16;
+  return need <= 4 ? 4 : need <= 6 ? need : need <= 8 ? 8 : need <= 10 ? 10 : need <= 12 ? 12 : 16;
+}
+
+template <class F>
+auto with_steps(int ks, F f) {
+  switch (ks) {
+    case 4: return f(std::integral_constant<int, 4>());
+    case 5: return f(std::integral_constant<int, 5>());
+    case 6: return f(std::integral_constant<int, 6>());
+    case 8: return f(std::integral_constant<int, 8>());
+    case 10: return f(std::integral_constant<int, 10>());
+    case 12: return f(std::integral_constant<int, 12>());
+    default: return f(std::integral_constant<int, 16>());
+  }
+}
+
+int per_sm(int ks, int nt) {
+  return with_steps(ks, [&](auto k) { return nt == 1 ? Tile<k(), 1>::kPerSM : Tile<k(), 2>::kPerSM; });
 }
 
 Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
@@ -669,11 +697,11 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   const int group = q_heads / c->n_kv_heads;
   s.nt = group <= 8 ? 1 : 2;
   s.parts = (group + 8 * s.nt - 1) / (8 * s.nt);
-  s.dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  s.ks = steps_for(c->head_dim);
   s.rows = c->batch * c->n_kv_heads * s.parts;
   const long long capacity = (long long)c->pages_per_seq * c->page_size;
   const long long blocks = (capacity + kBlockRows - 1) / kBlockRows * s.rows;
-  s.ctas = (int)std::min<long long>(blocks, (long long)kSMs * per_sm(s.dp, s.nt));
+  s.ctas = (int)std::min<long long>(blocks, (long long)kSMs * per_sm(s.ks, s.nt));
   const size_t h = 8 * s.nt;
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -692,11 +720,11 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   return s;
 }
 
-template <class T, int DP, int NT, bool FULL>
+template <class T, int KS, int NT>
 int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
-  constexpr int kSmem = Tile<DP, NT>::kSmem;
+  constexpr int kSmem = Tile<KS, NT>::kSmem;
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  auto kernel = paged_attention_kernel<T, DP, NT, FULL>;
+  auto kernel = paged_attention_kernel<T, KS, NT>;
   static std::atomic<uint64_t> allowed{0};
   int rc = allow_smem(kernel, kSmem, &allowed, "paged_attention");
   if (rc) return rc;
@@ -716,16 +744,11 @@ int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream
                       grid, dim3(kFinishThreads), 0, st, pdl_enabled(), p);
 }
 
-template <class T, int DP>
-int launch_dp(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
-  if (p.c.dim == DP) return s.nt == 1 ? launch<T, DP, 1, true>(p, s, tm, st) : launch<T, DP, 2, true>(p, s, tm, st);
-  return s.nt == 1 ? launch<T, DP, 1, false>(p, s, tm, st) : launch<T, DP, 2, false>(p, s, tm, st);
-}
-
 template <class T>
 int launch_type(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
-  if (s.dp == 64) return launch_dp<T, 64>(p, s, tm, st);
-  return s.dp == 128 ? launch_dp<T, 128>(p, s, tm, st) : launch_dp<T, 256>(p, s, tm, st);
+  return with_steps(s.ks, [&](auto k) {
+    return s.nt == 1 ? launch<T, k(), 1>(p, s, tm, st) : launch<T, k(), 2>(p, s, tm, st);
+  });
 }
 
 bool plain_shape(const Pi05PagedCache* c, int q_heads) {

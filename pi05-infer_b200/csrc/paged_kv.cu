@@ -732,16 +732,19 @@ int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int si
   if (budget >= c.capacity) return PI05_OK;  // no sequence can hold more
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int pairs = c.batch * c.heads;
-  // CTAs of a pair: up to 8 while they hold 1024 rows each and find an SM of their own.
+  // CTAs of a pair: up to 8 while they hold 4096 rows each and find an SM of their own.  A
+  // cluster's barriers cost more than they share out for fewer: 8 pairs of 3712 rows take
+  // 11 us in one CTA each and 13 in four; 8 pairs of 65536 take 42 in four and 33 in eight.
   int ctas = 1;
-  while (ctas < 8 && pairs * ctas * 2 <= kSMs && c.capacity / (ctas * 2) >= 1024) ctas *= 2;
+  while (ctas < 8 && pairs * ctas * 2 <= kSMs && c.capacity / (ctas * 2) >= 4096) ctas *= 2;
   const int share = ((c.capacity + ctas - 1) / ctas + 31) & ~31, held = std::min(share, kMaxKeys);
   const int most = std::min(budget, c.capacity - budget);  // moves of a pair
   const int move_here = most <= 64 * ctas;
   const size_t smem = (size_t)held * sizeof(uint32_t);
-  // More threads only for the rows that give each of them something to do: a pass over the
-  // buckets costs every thread the same.
-  const int threads = share <= 4096 ? 256 : 512;
+  // A pass over the buckets costs every thread the same: 512 pairs of 2080 rows take 10 us
+  // with 256 threads each and 14 with 512; where the CTAs have an SM each, 8 pairs of 3712
+  // rows take 16 and 11.
+  const int threads = share <= 4096 && pairs * ctas > kSMs ? 256 : 512;
   const int which = held < share ? 2 : threads == 256 ? 0 : 1;
   auto kernel = which == 2   ? evict_select_kernel<512, false>
                 : which == 0 ? evict_select_kernel<256, true>
