@@ -121,6 +121,11 @@ struct Segment {
   bool whole;
 };
 
+// a / b; 32-bit division, a tenth of the 64-bit one's instructions, where it will do.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // Walks through a CTA's share of the blocks, segment by segment.
 struct Walk {
   int b;
@@ -137,7 +142,7 @@ struct Walk {
       base += (long long)blocks * per;
       ++b;
     }
-    const int pair = (int)((at - base) / blocks);
+    const int pair = (int)divide(at - base, blocks);
     s.b = b;
     s.row = b * per + pair;
     s.kvh = pair / p.parts;
@@ -220,37 +225,41 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
   pdl_wait();
   pdl_launch_dependents();
 
-  // All blocks there are, then the sequence that this CTA's share begins in.
+  // All blocks there are, then the sequence that this CTA's share begins in: one scan for
+  // up to kThreads sequences, else a sum and a scan of one part after the other.
   const int per_block = p.c.heads * p.parts;
-  long long mine = 0;
-  for (int b = tid; b < p.c.batch; b += kThreads) {
-    mine += (p.c.rows(b) + kBlockRows - 1) / kBlockRows;
-    if (blockIdx.x == 0 && p.c.rows(b) != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
-  }
-  for (int sft = 16; sft > 0; sft >>= 1) mine += __shfl_xor_sync(~0u, mine, sft);
-  if (lane == 0) sh_sum[w] = mine;
-  __syncthreads();
-  long long total = 0;
+  const bool few = p.c.batch <= kThreads;
+  auto scan = [&](long long own) {  // of the CTA's threads; inclusive
+    for (int sft = 1; sft < 32; sft <<= 1) {
+      const long long u = __shfl_up_sync(~0u, own, sft);
+      if (lane >= sft) own += u;
+    }
+    __syncthreads();
+    if (lane == 31) sh_sum[w] = own;
+    __syncthreads();
+    for (int i = 0; i < w; ++i) own += sh_sum[i];
+    return own;
+  };
+  auto blocks_of = [&](int b) {
+    const int len = p.c.rows(b);
+    if (blockIdx.x == 0 && len != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
+    return (long long)((len + kBlockRows - 1) / kBlockRows) * per_block;
+  };
+  long long own = 0;
+  for (int b = tid; b < p.c.batch; b += kThreads) own += blocks_of(b);
+  long long incl = scan(own), total = 0;
   for (int i = 0; i < kWarps; ++i) total += sh_sum[i];
-  total *= per_block;
   const long long n = min((long long)gridDim.x, total), cta = blockIdx.x;
   if (cta >= n) return;
-  const long long lo = cta * total / n, hi = (cta + 1) * total / n;
+  const long long lo = divide(cta * total, n), hi = divide((cta + 1) * total, n);
   long long before = 0;
   for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
     const int b = b0 + tid;
-    const long long own = b < p.c.batch ? (long long)((p.c.rows(b) + kBlockRows - 1) / kBlockRows) * per_block : 0;
-    long long incl = own;
-    for (int sft = 1; sft < 32; sft <<= 1) {
-      const long long u = __shfl_up_sync(~0u, incl, sft);
-      if (lane >= sft) incl += u;
+    if (!few) {
+      own = b < p.c.batch ? blocks_of(b) : 0;
+      incl = before + scan(own);
+      for (int i = 0; i < kWarps; ++i) before += sh_sum[i];
     }
-    __syncthreads();
-    if (lane == 31) sh_sum[w] = incl;
-    __syncthreads();
-    for (int i = 0; i < w; ++i) incl += sh_sum[i];
-    incl += before;
-    for (int i = 0; i < kWarps; ++i) before += sh_sum[i];
     if (incl - own <= lo && lo < incl) {
       sh_b = b;
       sh_base = incl - own;
@@ -295,19 +304,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
   const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4) + L::kBytes;
   auto step_at = [](uint32_t at, int ks) { return (at ^ ((ks & 3) << 5)) + (ks >> 2) * L::kBox; };
 
-  Segment s;
-  while (true) {
-    const bool first = walk.at == lo;
-    if (!walk.next(p, s)) break;
+  // q^T fragments: lane holds head lane / 4, values 2 (lane % 4) + {0, 1, 8, 9} of each step.
+  uint32_t qf[KS][NT][2];
+  auto load_q = [&](const Segment& s) {
     const int heads = min(H, p.group - s.part * H), head0 = s.kvh * p.group + s.part * H;
-    const int slot = 2 * (int)cta + (first ? 0 : 1);
-    if (s.tile0 == 0 && tid == 0) {
-      // the row's last block, and the CTA that has it
-      const long long end = walk.at - s.n + (s.len + kBlockRows - 1) / kBlockRows;
-      p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)((end * n - 1) / total));
-    }
-    // q^T fragments: lane holds head lane / 4, values 2 (lane % 4) + {0, 1, 8, 9} of each step.
-    uint32_t qf[KS][NT][2];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -320,7 +320,18 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
           qf[ks][nt][i] = h < heads && at < d ? *reinterpret_cast<const uint32_t*>(q + at) : 0u;
         }
       }
-
+  };
+  Segment next;
+  bool have = walk.next(p, next);
+  if (have) load_q(next);
+  for (int slot = 2 * (int)cta; have; slot |= 1) {
+    const Segment s = next;
+    const int heads = min(H, p.group - s.part * H), head0 = s.kvh * p.group + s.part * H;
+    if (s.tile0 == 0 && tid == 0) {
+      // the row's last block, and the CTA that has it
+      const long long end = walk.at - s.n + (s.len + kBlockRows - 1) / kBlockRows;
+      p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)divide(end * n - 1, total));
+    }
     float o[KS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -443,6 +454,9 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
           }
       }
     }
+
+    have = walk.next(p, next);
+    if (have) load_q(next);  // on its way while this segment is joined
 
     // The four warps' results, joined two by two in a fixed order: warps 2 and 3 hand theirs
     // to 0 and 1, then 1 to 0, fragment by fragment.

@@ -334,7 +334,8 @@ class PagedKVCache:
         # status word, ticket and the eviction's lists; zeroed once
         self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         self._c.workspace, self._c.workspace_bytes = self.workspace.data_ptr(), nbytes
-        self._scratch = {}  # (heads, track): bytes, and a tensor of one byte that looks like so many
+        # (heads, track): bytes of scratch, and one-element tensors with the shapes of scratch and lse
+        self._scratch = {}
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, batch: int, pages_per_seq: int, *,
@@ -441,14 +442,14 @@ class PagedKVCache:
         elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != self._index or \
                 not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape, type and device")
-        lse = q.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
+        need, like, like_lse = self._scratch.get((heads, track)) or self._need(heads, track)
+        lse = torch.empty_like(like_lse, memory_format=torch.contiguous_format) if return_lse else None
         valid_at = pitch = valid_rows = 0
         if key_valid is not None:
             if key_valid.dim() != 2 or key_valid.dtype not in (torch.bool, torch.uint8) or \
                     key_valid.shape[0] != batch or key_valid.get_device() != self._index or key_valid.stride(1) != 1:
                 raise ValueError("key_valid must be bool or uint8 [batch, rows] on the cache's device, rows contiguous")
             valid_at, pitch, valid_rows = key_valid.data_ptr(), key_valid.stride(0), key_valid.shape[1]
-        need, like = self._scratch.get((heads, track)) or self._need(heads, track)
         # from torch's allocator, call by call: calls on different streams, and graphs, never share it
         scratch = torch.empty_like(like, memory_format=torch.contiguous_format)
         q_token, q_head, _ = q.stride()
@@ -460,8 +461,9 @@ class PagedKVCache:
     def _need(self, heads: int, track: bool):
         need = _fn("pi05_paged_attention_scratch_bytes")(self._at, heads, track)
         like = torch.empty(1, dtype=torch.uint8, device=self.device).expand(need)
-        self._scratch[heads, track] = need, like
-        return need, like
+        like_lse = torch.empty(1, dtype=torch.float32, device=self.device).expand(self.batch, heads)
+        self._scratch[heads, track] = need, like, like_lse
+        return need, like, like_lse
 
     def evict(self, budget: int, *, recent: int = 0, sinks: int = 0) -> None:
         """Cuts every sequence with more than ``budget`` rows down to it.
