@@ -90,11 +90,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, int z,
-                                            int w) {
+                                            int w, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, "
+      "{%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
       : "memory");
 }
 
@@ -177,7 +177,8 @@ __device__ __forceinline__ Ref look_up(const AttnParams& p, const Segment& s, in
 // a lane for each group of rows.  Returns a bit for each row that counts.
 template <int KS, int NT>
 __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
-                                          const Ref& ref, uint64_t* bar, uint32_t dst, int lane) {
+                                          const Ref& ref, uint64_t* bar, uint32_t dst, int lane,
+                                          uint64_t policy) {
   using L = Tile<KS, NT>;
   const bool real = p.c.real(ref.page);
   if (ref.counts && !real) report_status(p.c.status, PI05_DEV_BAD_INDEX);
@@ -197,8 +198,8 @@ __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap
     const uint32_t to = dst + lane * 128, at = smem_u32(bar);
 #pragma unroll
     for (int i = 0; i < L::kBoxes; ++i) {
-      tma_load_4d(to + i * L::kBox, tm_k, at, i * 64, ref.line, ref.kvh, ref.page);
-      tma_load_4d(to + L::kBytes + i * L::kBox, tm_v, at, i * 64, ref.line, ref.kvh, ref.page);
+      tma_load_4d(to + i * L::kBox, tm_k, at, i * 64, ref.line, ref.kvh, ref.page, policy);
+      tma_load_4d(to + L::kBytes + i * L::kBox, tm_v, at, i * 64, ref.line, ref.kvh, ref.page, policy);
     }
   }
   return mask;
@@ -274,6 +275,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
   uint64_t* bars = all_bars + w * S;
   const int d = p.c.dim;
 
+  // K and V pass through L2 once, unless other parts of the query heads read them too; what
+  // is written for the kernels behind this one (scores: 34 of 1110 MB) should stay there.
+  const uint64_t policy = p.parts == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
+
   // The warp's copies run ahead of its products, across the segments' borders.
   Walk ahead{sh_b, sh_base, lo, hi}, walk = ahead;
   Segment fs;
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
   for (int j = 0; j < S - 1; ++j) {
     const Ref now = ref;
     ref = next_ref();
-    live[j] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane) : 0u;
+    live[j] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane, policy) : 0u;
   }
   int stage = 0;
   uint32_t phase = 0;
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
         const Ref now = ref;
         ref = next_ref();
         const int to = stage == 0 ? S - 1 : stage - 1;
-        live[S - 1] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane) : 0u;
+        live[S - 1] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane, policy) : 0u;
       }
       const uint32_t tile = ring + stage * 2 * L::kBytes, rows = live[0];
       if (++stage == S) {

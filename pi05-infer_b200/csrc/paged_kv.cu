@@ -91,7 +91,11 @@ struct __align__(16) TokenRow {
   int position;
 };
 
-template <class T, int V, int J>
+// ROT: with rotation.  Two kernels, since the registers of the one cost the other its
+// occupancy: with v's first batch held over the row search as well, the append of 16384
+// rotated tokens took 44 us instead of 37; without, that of 65536 plain ones 105 instead
+// of 93.
+template <class T, int V, bool ROT>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ Pages c,
                                                                 const __grid_constant__ AppendParams p) {
   extern __shared__ __align__(16) char smem[];
@@ -163,8 +167,48 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     __syncthreads();
   };
 
-  bool ready = false;
-  {  // q and k: `lanes` threads to a head's units, kAppendThreads / lanes heads at a time
+  // Rows that are stored as they are (v, and k without rotation): `row_lanes` threads to a
+  // row, C rows of a thread at once.  The first batches are asked for before the rows are
+  // looked for.
+  constexpr int C = ROT ? 2 : 4;
+  const int copy_rows = n * c.heads, copy0 = tid / p.row_lanes, copy_step = kAppendThreads / p.row_lanes;
+  const int copy_u = tid - copy0 * p.row_lanes;
+  auto copy_load = [&](Unit<T, V>* unit, const void* src, long long tt, long long hh, int r, int u) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int row = r + j * copy_step, t = p.by_heads.div(row), h = row - t * c.heads;
+      if (copy0 < copy_step && row < copy_rows && u < p.row_units)
+        unit[j].load_row(static_cast<const T*>(src) + (t0 + t) * tt + h * hh, u);
+    }
+  };
+  auto copy_store = [&](const Unit<T, V>* unit, char* pages, int r, int u) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int row = r + j * copy_step, t = p.by_heads.div(row), h = row - t * c.heads;
+      if (copy0 < copy_step && row < copy_rows && u < p.row_units && row_of[t].at >= 0)
+        unit[j].store_row(reinterpret_cast<T*>(pages + row_of[t].at + h * c.head_stride), u);
+    }
+  };
+  auto copy_rest = [&](const void* src, long long tt, long long hh, char* pages, bool all) {
+    for (int u = copy_u; u < p.row_units; u += p.row_lanes)
+      for (int r = copy0 + (u == copy_u && !all ? C * copy_step : 0); r < copy_rows; r += C * copy_step) {
+        Unit<T, V> unit[C];
+        copy_load(unit, src, tt, hh, r, u);
+        copy_store(unit, pages, r, u);
+      }
+  };
+
+  if constexpr (!ROT) {
+    Unit<T, V> k_first[C], v_first[C];
+    copy_load(k_first, p.k, p.kt, p.kh, copy0, copy_u);
+    copy_load(v_first, p.v, p.vt, p.vh, copy0, copy_u);
+    find_rows();
+    copy_store(k_first, c.k, copy0, copy_u);
+    copy_store(v_first, c.v, copy0, copy_u);
+    copy_rest(p.k, p.kt, p.kh, c.k, false);
+  } else {  // q and k: `lanes` threads to a head's units, kAppendThreads / lanes heads at a time
+    constexpr int J = 2;
+    bool ready = false;
     const int heads = p.q_heads + c.heads, rows = n * heads;
     const int row0 = tid / p.lanes, u0 = tid - row0 * p.lanes, step = kAppendThreads / p.lanes;
     for (int u = u0; u < p.units || u == u0; u += p.lanes) {
@@ -201,29 +245,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       }
     }
   }
-  {  // v
-    const int rows = n * c.heads;
-    const int row0 = tid / p.row_lanes, u0 = tid - row0 * p.row_lanes, step = kAppendThreads / p.row_lanes;
-    if (row0 < step)
-      for (int u = u0; u < p.row_units; u += p.row_lanes)
-        for (int r = row0; r < rows; r += J * step) {
-          Unit<T, V> unit[J];
-          int token[J], head[J];
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            const int row = r + j * step;
-            token[j] = p.by_heads.div(row);
-            head[j] = row - token[j] * c.heads;
-            if (row < rows) unit[j].load_row(static_cast<const T*>(p.v) + (t0 + token[j]) * p.vt + head[j] * p.vh, u);
-          }
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            if (r + j * step >= rows) continue;
-            const long long at = row_of[token[j]].at;
-            if (at >= 0) unit[j].store_row(reinterpret_cast<T*>(c.v + at + head[j] * c.head_stride), u);
-          }
-        }
-  }
+  copy_rest(p.v, p.vt, p.vh, c.v, ROT);
   if (p.cu == nullptr) return;
   // Ragged: the CTA that finishes last moves the counts on, when all have read them.
   __syncthreads();
@@ -624,7 +646,6 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 
 template <class T, int V>
 int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
-  constexpr int J = 2;
   p.turned = p.rotary > 0 ? rotary_units<V>(p.rotary, p.interleaved) : 0;
   p.units = p.turned + (c.dim - p.rotary) / V;
   p.lanes = std::min(p.units, kAppendThreads);
@@ -634,9 +655,9 @@ int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
   p.by_heads = FastDiv(c.heads);
   p.by_pairs = FastDiv(std::max(1, p.rotary / 2));
   // A few batches of loads for a CTA, but for tokens enough to fill the SMs.
-  const int fill = 8 * J * (kAppendThreads / p.lanes) / (p.q_heads + c.heads);
+  const int fill = 16 * (kAppendThreads / p.lanes) / (p.q_heads + c.heads);
   p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 40}));  // 40 x (1 KB + 32) of shared memory at most
-  return launch_pdl(append_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kAppendThreads),
+  return launch_pdl(p.turned > 0 ? append_kernel<T, V, true> : append_kernel<T, V, false>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kAppendThreads),
                     p.per_cta * (sizeof(TokenRow) + (size_t)(p.rotary / 2) * sizeof(float2)), stream, pdl_enabled(), c,
                     p);
 }
