@@ -401,9 +401,10 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   __syncthreads();
   if (bad) sh_bad = 1;
   sync_all();
-  int any_bad = 0;
-  for (int r = 0; r < ctas; ++r) any_bad |= peer(&sh_bad, r);
-  if (any_bad) {
+  // Others' values: a lane for each CTA, all on their way at once (one after the other, the
+  // eight of a cluster took 2 us each time).
+  auto of_all = [&](const int* x) { return lane < ctas ? peer(x, lane) : 0; };
+  if (__any_sync(~0u, of_all(&sh_bad) != 0)) {
     if (tid == 0 && rank == 0) {
       moves[0] = -1;
       report_status(c.status, PI05_DEV_BAD_INDEX);
@@ -562,8 +563,8 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
       if (lane == 0) sh_counts[0] = sum;
     }
     sync_all();
-    for (int r = 0; r < rank; ++r) ties += peer(&sh_counts[0], r);
-    ties += sum_before(warp_a, w, lane);
+    const int others = of_all(&sh_counts[0]);
+    ties = __reduce_add_sync(~0u, lane < rank ? others : 0) + sum_before(warp_a, w, lane);
     sync_all();  // before the counts are written anew
   }
   auto classify = [&](int g, int& seen, bool& hole, bool& tail) {
@@ -598,17 +599,10 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
     if (lane == 0) sh_counts[0] = x, sh_counts[1] = y;
   }
   sync_all();
-  int all = 0, at_hole = 0, at_tail = 0;
-  for (int r = 0; r < ctas; ++r) {
-    const int x = peer(&sh_counts[0], r);
-    all += x;
-    if (r < rank) {
-      at_hole += x;
-      at_tail += peer(&sh_counts[1], r);
-    }
-  }
-  at_hole += sum_before(warp_a, w, lane);
-  at_tail += sum_before(warp_b, w, lane);
+  const int their_holes = of_all(&sh_counts[0]), their_tails = of_all(&sh_counts[1]);
+  const int all = __reduce_add_sync(~0u, their_holes);
+  int at_hole = __reduce_add_sync(~0u, lane < rank ? their_holes : 0) + sum_before(warp_a, w, lane);
+  int at_tail = __reduce_add_sync(~0u, lane < rank ? their_tails : 0) + sum_before(warp_b, w, lane);
   seen = ties;
   for (int g = g0; g < g0 + per; ++g) {
     bool hole, tail;
