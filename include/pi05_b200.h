@@ -460,8 +460,8 @@ int pi05_rope(const Pi05RopeArgs* args, const Pi05Rotary* rotary, void* stream);
 /* A key-value cache in pages, shared by `batch` sequences.  Row r of sequence b is
  * line r % page_size of page page_table[b, r / page_size].  Host struct of device
  * pointers, owned by the caller.  Ops on one cache must be ordered on one stream.
- * A page that an op writes (append, evict, attention with `track`) belongs to one
- * sequence; pages that are only read may be shared.  A page number outside
+ * A page that an op writes (append, evict, attention with `track`) stands once in the
+ * table, with one sequence; pages that are only read may be shared.  A page number outside
  * [0, num_pages) or a row beyond the table sets PI05_DEV_BAD_INDEX in the workspace
  * status word; the row is then skipped (append), or counts as masked (attention, and
  * eviction leaves the sequence as it is). */

@@ -121,6 +121,16 @@ def _run(name: str, index: int, *args) -> None:
         raise _lib.Pi05Error(name, rc, _lib.last_error())
 
 
+def _strides(t: torch.Tensor):
+    """``t``'s strides, with those of dimensions of one element, which mean nothing, as if it were dense there."""
+    strides, dense = list(t.stride()), 1
+    for i in reversed(range(t.dim())):
+        if t.shape[i] == 1:
+            strides[i] = dense
+        dense = max(dense, strides[i] * t.shape[i])
+    return strides
+
+
 def _cuda(device) -> torch.device:
     device = torch.device(device)
     if device.type != "cuda":
@@ -295,8 +305,9 @@ class PagedKVCache:
     is done by writing to them.
 
     The table is read on the device.  A page number outside the cache, or a row beyond the table,
-    is skipped or masked and sets ``PI05_DEV_BAD_INDEX`` (0x20) in :meth:`read_status`.  A page
-    that a call writes belongs to one sequence.
+    is skipped or masked and sets ``PI05_DEV_BAD_INDEX`` (0x20) in :meth:`read_status`.  A page that a
+    call writes (:meth:`append`, :meth:`evict`, :meth:`attend` with ``track``) stands once in the
+    table, with one sequence; pages that are only read may be shared.
     """
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, counts: torch.Tensor, *,
@@ -304,11 +315,12 @@ class PagedKVCache:
         if k_pages.dim() != 4 or k_pages.dtype not in (torch.bfloat16, torch.float16) or not k_pages.is_cuda:
             raise ValueError("k_pages must be a [pages, kv_heads, page_size, dim] CUDA tensor, bf16 or fp16")
         device = k_pages.device
+        strides = _strides(k_pages)
         if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != device or \
-                v_pages.stride() != k_pages.stride() or k_pages.stride(3) != 1:
+                _strides(v_pages) != strides or strides[3] != 1:
             raise ValueError("v_pages must match k_pages (shape, type, device, strides; rows contiguous)")
         if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device or \
-                page_table.stride(1) != 1:
+                _strides(page_table)[1] != 1:
             raise ValueError("page_table must be int32 [batch, pages_per_seq] on the cache's device, rows contiguous")
         if counts.shape != (2, page_table.shape[0]) or counts.dtype != torch.int32 or counts.device != device or \
                 not counts.is_contiguous():
@@ -326,9 +338,9 @@ class PagedKVCache:
             return None if t is None else t.data_ptr()
 
         self._c = Pi05PagedCache(
-            p(k_pages), p(v_pages), *k_pages.stride()[:3], p(weight), p(pos), p(page_table), p(counts),
+            p(k_pages), p(v_pages), *strides[:3], p(weight), p(pos), p(page_table), p(counts),
             _DTYPES[self.dtype], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, self.batch,
-            self.pages_per_seq, page_table.stride(0), None, 0)
+            self.pages_per_seq, _strides(page_table)[0], None, 0)
         self._at, self._index = ctypes.addressof(self._c), device.index
         nbytes = _fn("pi05_paged_workspace_bytes")(self._at)
         # status word, ticket and the eviction's lists; zeroed once
@@ -427,7 +439,8 @@ class PagedKVCache:
         ``scale`` is ``head_dim ** -0.5`` if not given.  ``key_valid`` (bool or uint8 ``[batch, n]``):
         rows that are False are left out, whatever they hold; rows from ``n`` on count (a prompt's
         padding mask need not grow with the sequence).  ``track`` adds the probabilities
-        to the cache's ``weight``.  A sequence with no row gives zeros (lse ``-inf``).  Returns
+        to the cache's ``weight`` (its scratch holds a score for every row there can be and query head, so
+        a table much longer than its sequences costs memory).  A sequence with no row gives zeros (lse ``-inf``).  Returns
         ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32 natural-log sums
         ``[batch, heads]``.
         """
@@ -447,7 +460,8 @@ class PagedKVCache:
         valid_at = pitch = valid_rows = 0
         if key_valid is not None:
             if key_valid.dim() != 2 or key_valid.dtype not in (torch.bool, torch.uint8) or \
-                    key_valid.shape[0] != batch or key_valid.get_device() != self._index or key_valid.stride(1) != 1:
+                    key_valid.shape[0] != batch or key_valid.get_device() != self._index or \
+                    (key_valid.stride(1) != 1 and key_valid.shape[1] > 1):
                 raise ValueError("key_valid must be bool or uint8 [batch, rows] on the cache's device, rows contiguous")
             valid_at, pitch, valid_rows = key_valid.data_ptr(), key_valid.stride(0), key_valid.shape[1]
         # from torch's allocator, call by call: calls on different streams, and graphs, never share it

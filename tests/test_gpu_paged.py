@@ -433,6 +433,10 @@ def test_attend_shared_pages_two_streams():
     (1, 2, 128, 24, [5000], 4999, 2000, 10, "heads"),
     (1, 1, 64, 16, [40], 30, 26, 4, "heads"),        # nothing but protected rows stays
     (40, 4, 64, 16, [(37 * i) % 300 for i in range(40)], 100, 10, 2, "heads"),
+    (1, 1, 8, 16, [33000], 20000, 100, 4, "heads"),      # a cluster of CTAs for the one pair
+    (1, 2, 8, 16, [20000], 19998, 1000, 4, "lines"),     # two rows to go, in a cluster
+    (2, 1, 8, 64, [8200, 30], 8196, 4, 0, "heads"),      # four, in two CTAs
+    (1, 1, 8, 16, [8300], 100, 0, 0, "heads"),
 ])
 def test_evict(dtype, batch, heads, dim, page, lens, budget, recent, sinks, pages):
     c, t = make(batch, heads, dim, page, max(lens) + 3, dtype=dtype, layout=pages)
@@ -463,6 +467,35 @@ def test_evict(dtype, batch, heads, dim, page, lens, budget, recent, sinks, page
     same_rows(c, t)
     c.evict(budget, recent=recent, sinks=sinks)  # nothing is over the budget now
     same_rows(c, t)
+    assert c.read_status() == 0
+
+
+def test_evict_more_rows_than_a_cta_holds():
+    """80 sequences, so one CTA each, of up to 50000 rows: keys beyond the shared memory are worked out again."""
+    c, t = make(80, 1, 8, 64, 50000, spare=0)
+    r = np.random.default_rng(5)
+    t.weight[:] = np.float64(np.float32(np.round(r.standard_normal(t.weight.shape), 2)))
+    t.pos[:] = r.integers(0, 60000, t.pos.shape)
+    t.counts[0, :] = 7
+    t.counts[0, [3, 79]] = 50000, 49500
+    t.counts[1, :] = 60000
+    for x, y in ((c.weight, t.weight), (c.pos, t.pos), (c.counts, t.counts)):
+        x.copy_(torch.tensor(y))
+    c.evict(20000, recent=500, sinks=4)
+    t.evict(20000, 500, 4)
+    same_rows(c, t)
+
+
+def test_strides_of_single_elements():
+    """One page, head, line or sequence: whatever stride torch gives that dimension."""
+    base = rnd(2, 5, 1, 72)
+    k, v = (base[i, :, :, 8:].unsqueeze(1).as_strided((5, 1, 1, 64), (72, 3, 7, 1)) for i in range(2))
+    table = torch.tensor([[3]], dtype=torch.int32, device="cuda").as_strided((1, 1), (5, 9))
+    c = PagedKVCache(k, v.as_strided((5, 1, 1, 64), (72, 11, 1, 1)), table,
+                     torch.tensor([[1], [1]], dtype=torch.int32, device="cuda"))
+    t = twin(c)
+    valid = torch.ones(1, 1, dtype=torch.bool, device="cuda").as_strided((1, 1), (1, 4))
+    check_attend(c, t, rnd(1, 2, 64), valid=valid)
     assert c.read_status() == 0
 
 
