@@ -50,6 +50,7 @@ struct AttnParams {
   int q_heads, group, parts;  // query heads per key-value head, cut into `parts` of at most 8 NT heads
   float scale_log2;
   int track, box_rows;
+  int ctas;  // of a pair (SHORT)
   // scratch
   float* part_o;    // [2 n_ctas][8 NT][dim]
   float2* part_ml;  // [2 n_ctas][8 NT]
@@ -101,12 +102,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
 // A tile of 16 rows: boxes of 64 columns, 16 rows of 128 bytes each, whose 16-byte chunk
 // c of row r lies at chunk c ^ (r & 7) (the 128-byte swizzle): ldmatrix without conflicts.
 // KS: steps of 16 columns that the products take; what lies beyond a head is zeros.
-template <int KS, int NT>
+// SHORT (see the kernel) leaves shared memory to the scores.
+template <int KS, int NT, bool SHORT>
 struct Tile {
   static constexpr int kBoxes = (KS + 3) / 4;
   static constexpr int kBox = kWarpRows * 128;
   static constexpr int kBytes = kBoxes * kBox;
-  static constexpr int kStages = kBoxes == 4 && NT == 1 ? 3 : 2;
+  static constexpr int kStages = kBoxes == 4 && NT == 1 && !SHORT ? 3 : 2;
   static constexpr int kRing = kWarps * kStages * 2 * kBytes;
   static constexpr int kSlot = (KS * NT * 4 + NT * 4) * 32 * 4;  // a warp's o, m and l, at a segment's end
   static constexpr int kSmem = 1024 + kRing + 2 * kSlot;
@@ -175,11 +177,11 @@ __device__ __forceinline__ Ref look_up(const AttnParams& p, const Segment& s, in
 // Starts the copies of a tile's K and V by TMA, `p.box_rows` rows of 64 columns at a time
 // (the largest power of two that divides the page size, so that a box lies in one page);
 // a lane for each group of rows.  Returns a bit for each row that counts.
-template <int KS, int NT>
+template <int KS, int NT, bool SHORT>
 __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
                                           const Ref& ref, uint64_t* bar, uint32_t dst, int lane,
                                           uint64_t policy) {
-  using L = Tile<KS, NT>;
+  using L = Tile<KS, NT, SHORT>;
   const bool real = p.c.real(ref.page);
   if (ref.counts && !real) report_status(p.c.status, PI05_DEV_BAD_INDEX);
   const uint32_t mask = __ballot_sync(~0u, ref.counts && real) & 0xffff;
@@ -205,11 +207,20 @@ __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap
   return mask;
 }
 
-template <class T, int KS, int NT>
-__global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
+__device__ __forceinline__ float ld_peer(const float* x, int rank, int ctas) {
+  if (ctas == 1) return *x;
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(x), rank)) : "memory");
+  return v;
+}
+
+// SHORT: a cluster of p.ctas CTAs for each pair instead of equal shares, which joins its
+// parts through distributed shared memory and keeps its scores there: no other kernel.
+template <class T, int KS, int NT, bool SHORT>
+__global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v) {
-  using L = Tile<KS, NT>;
+  using L = Tile<KS, NT, SHORT>;
   constexpr int H = 8 * NT, S = L::kStages;
   extern __shared__ char smem_raw[];
   __shared__ long long sh_sum[kWarps];
@@ -226,67 +237,97 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
   pdl_wait();
   pdl_launch_dependents();
 
-  // All blocks there are, then the sequence that this CTA's share begins in: one scan for
-  // up to kThreads sequences, else a sum and a scan of one part after the other.
-  const int per_block = p.c.heads * p.parts;
-  const bool few = p.c.batch <= kThreads;
-  auto scan = [&](long long own) {  // of the CTA's threads; inclusive
-    for (int sft = 1; sft < 32; sft <<= 1) {
-      const long long u = __shfl_up_sync(~0u, own, sft);
-      if (lane >= sft) own += u;
+  const int d = p.c.dim;
+  long long total = 0, n = 0, lo = 0;  // all blocks, the CTAs that share them, this one's first
+  const long long cta = blockIdx.x;
+  int rank = 0;
+  Segment fs;             // of the copies, which run ahead of the products
+  Walk ahead{0, 0, 0, 0};
+  bool more;
+  if constexpr (SHORT) {
+    const int pair = blockIdx.x / p.ctas;  // the grid is a line of clusters
+    rank = blockIdx.x - pair * p.ctas;
+    const int b = pair / p.c.heads, len = p.c.rows(b), blocks = (len + kBlockRows - 1) / kBlockRows;
+    if (rank == 0 && tid == 0 && len != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
+    fs = Segment{b, pair, pair - b * p.c.heads, 0, len, rank * blocks / p.ctas, 0, false};
+    fs.n = (rank + 1) * blocks / p.ctas - fs.tile0;
+    if (len == 0) {  // the whole cluster alike: nothing to attend to
+      const int head = fs.kvh * p.group;
+      if (rank == 0)
+        for (int i = tid; i < p.group * d; i += kThreads)
+          static_cast<T*>(p.out)[((size_t)b * p.q_heads + head) * d + i] = from_f32<T>(0.f);
+      if (rank == 0 && p.lse != nullptr)
+        for (int i = tid; i < p.group; i += kThreads) p.lse[(size_t)b * p.q_heads + head + i] = -INFINITY;
+      return;
+    }
+    more = fs.n > 0;
+    __syncthreads();  // the barriers are there
+  } else {
+    // All blocks there are, then the sequence that this CTA's share begins in: one scan for
+    // up to kThreads sequences, else a sum and a scan of one part after the other.
+    const int per_block = p.c.heads * p.parts;
+    const bool few = p.c.batch <= kThreads;
+    auto scan = [&](long long own) {  // of the CTA's threads; inclusive
+      for (int sft = 1; sft < 32; sft <<= 1) {
+        const long long u = __shfl_up_sync(~0u, own, sft);
+        if (lane >= sft) own += u;
+      }
+      __syncthreads();
+      if (lane == 31) sh_sum[w] = own;
+      __syncthreads();
+      for (int i = 0; i < w; ++i) own += sh_sum[i];
+      return own;
+    };
+    auto blocks_of = [&](int b) {
+      const int len = p.c.rows(b);
+      if (blockIdx.x == 0 && len != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
+      return (long long)((len + kBlockRows - 1) / kBlockRows) * per_block;
+    };
+    long long own = 0;
+    for (int b = tid; b < p.c.batch; b += kThreads) own += blocks_of(b);
+    long long incl = scan(own);
+    for (int i = 0; i < kWarps; ++i) total += sh_sum[i];
+    n = min((long long)gridDim.x, total);
+    if (cta >= n) return;
+    lo = divide(cta * total, n);
+    const long long hi = divide((cta + 1) * total, n);
+    long long before = 0;
+    for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
+      const int b = b0 + tid;
+      if (!few) {
+        own = b < p.c.batch ? blocks_of(b) : 0;
+        incl = before + scan(own);
+        for (int i = 0; i < kWarps; ++i) before += sh_sum[i];
+      }
+      if (incl - own <= lo && lo < incl) {
+        sh_b = b;
+        sh_base = incl - own;
+      }
+      if (before > lo) break;
     }
     __syncthreads();
-    if (lane == 31) sh_sum[w] = own;
-    __syncthreads();
-    for (int i = 0; i < w; ++i) own += sh_sum[i];
-    return own;
-  };
-  auto blocks_of = [&](int b) {
-    const int len = p.c.rows(b);
-    if (blockIdx.x == 0 && len != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
-    return (long long)((len + kBlockRows - 1) / kBlockRows) * per_block;
-  };
-  long long own = 0;
-  for (int b = tid; b < p.c.batch; b += kThreads) own += blocks_of(b);
-  long long incl = scan(own), total = 0;
-  for (int i = 0; i < kWarps; ++i) total += sh_sum[i];
-  const long long n = min((long long)gridDim.x, total), cta = blockIdx.x;
-  if (cta >= n) return;
-  const long long lo = divide(cta * total, n), hi = divide((cta + 1) * total, n);
-  long long before = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
-    const int b = b0 + tid;
-    if (!few) {
-      own = b < p.c.batch ? blocks_of(b) : 0;
-      incl = before + scan(own);
-      for (int i = 0; i < kWarps; ++i) before += sh_sum[i];
-    }
-    if (incl - own <= lo && lo < incl) {
-      sh_b = b;
-      sh_base = incl - own;
-    }
-    if (before > lo) break;
+
+    ahead = Walk{sh_b, sh_base, lo, hi};
+    more = ahead.next(p, fs);
   }
-  __syncthreads();
 
   const uint32_t base_addr = (smem_u32(smem_raw) + 1023) & ~1023u;  // swizzled boxes start at multiples of 1024
   const uint32_t ring = base_addr + w * S * 2 * L::kBytes;
   float* slots = reinterpret_cast<float*>(smem_raw + (base_addr - smem_u32(smem_raw)) + L::kRing);
   uint64_t* bars = all_bars + w * S;
-  const int d = p.c.dim;
+  float* my_scores = slots + 2 * (L::kSlot / 4);  // SHORT: [rows of this CTA][score_pitch]
 
   // K and V pass through L2 once, unless other parts of the query heads read them too; what
   // is written for the kernels behind this one (scores: 34 of 1110 MB) should stay there.
   const uint64_t policy = p.parts == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
 
   // The warp's copies run ahead of its products, across the segments' borders.
-  Walk ahead{sh_b, sh_base, lo, hi}, walk = ahead;
-  Segment fs;
-  bool more = ahead.next(p, fs);
+  Segment next = fs;
+  Walk walk = ahead;
   int fj = 0;
   auto next_ref = [&]() {
     if (more && fj == fs.n) {
-      more = ahead.next(p, fs);
+      more = !SHORT && ahead.next(p, fs);
       fj = 0;
     }
     if (!more) return Ref{0, 0, 0, false, false};
@@ -298,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
   for (int j = 0; j < S - 1; ++j) {
     const Ref now = ref;
     ref = next_ref();
-    live[j] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane, policy) : 0u;
+    live[j] = now.tile ? fetch<KS, NT, SHORT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane, policy) : 0u;
   }
   int stage = 0;
   uint32_t phase = 0;
@@ -326,13 +367,12 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
         }
       }
   };
-  Segment next;
-  bool have = walk.next(p, next);
-  if (have) load_q(next);
+  load_q(next);
+  bool have = true;
   for (int slot = 2 * (int)cta; have; slot |= 1) {
     const Segment s = next;
     const int heads = min(H, p.group - s.part * H), head0 = s.kvh * p.group + s.part * H;
-    if (s.tile0 == 0 && tid == 0) {
+    if (!SHORT && s.tile0 == 0 && tid == 0) {
       // the row's last block, and the CTA that has it
       const long long end = walk.at - s.n + (s.len + kBlockRows - 1) / kBlockRows;
       p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)divide(end * n - 1, total));
@@ -358,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
         const Ref now = ref;
         ref = next_ref();
         const int to = stage == 0 ? S - 1 : stage - 1;
-        live[S - 1] = now.tile ? fetch<KS, NT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane, policy) : 0u;
+        live[S - 1] = now.tile ? fetch<KS, NT, SHORT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane, policy) : 0u;
       }
       const uint32_t tile = ring + stage * 2 * L::kBytes, rows = live[0];
       if (++stage == S) {
@@ -416,7 +456,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
         for (int i = 0; i < 4; ++i) xs[i] = (i < 2 ? live0 : live1) ? (xs[i] + x2[nt][i]) * p.scale_log2 : -INFINITY;
         if (p.track) {
           const int h = nt * 8 + 2 * (lane & 3), r0 = ((s.tile0 + j) * kWarps + w) * kWarpRows + (lane >> 2);
-          float* dst = p.scores + ((size_t)s.row * p.c.capacity + r0) * p.score_pitch + h;
+          float* dst = SHORT ? my_scores + (r0 - s.tile0 * kBlockRows) * p.score_pitch + h
+                             : p.scores + ((size_t)s.row * p.c.capacity + r0) * p.score_pitch + h;
           if (r0 < s.len && h < heads) *reinterpret_cast<float2*>(dst) = make_float2(xs[0], xs[1]);
           if (r0 + 8 < s.len && h < heads)
             *reinterpret_cast<float2*>(dst + 8 * (size_t)p.score_pitch) = make_float2(xs[2], xs[3]);
@@ -460,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
       }
     }
 
-    have = walk.next(p, next);
+    have = !SHORT && walk.next(p, next);
     if (have) load_q(next);  // on its way while this segment is joined
 
     // The four warps' results, joined two by two in a fixed order: warps 2 and 3 hand theirs
@@ -509,6 +550,13 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
     if (w < 2) take(w);
     if (w == 1) give(1);
     __syncthreads();
+    if (SHORT) {
+      if (w == 0) {
+        take(1);
+        give(0);
+      }
+      break;
+    }
     if (w == 0) {
       take(1);
 #pragma unroll
@@ -542,6 +590,73 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT>::kPerSM)
           }
         }
     }
+  }
+
+  if constexpr (SHORT) {
+    __shared__ float sh_lse[H];
+    const int ctas = p.ctas, heads = p.group, head0 = fs.kvh * p.group;
+    auto sync_all = [&]() {
+      if (ctas > 1) cluster_sync_all();
+      else __syncthreads();
+    };
+    sync_all();
+    // Value e of a slot: fragment e / 32 of lane e % 32, as give() lays them out.  The
+    // cluster's CTAs take every ctas-th run of values and add the parts up in rank order.
+    auto total_of = [&](int nt, int i, int of_lane, float* scale) {  // scale[r]: what rank r's part counts
+      const float* ml = slots + (nt * 4 + i) * 32 + of_lane;
+      float m[8], l[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        m[r] = r < ctas ? ld_peer(ml, r, ctas) : -INFINITY;
+        l[r] = r < ctas ? ld_peer(ml + 64, r, ctas) : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) top = fmaxf(top, m[r]);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        scale[r] = ex2_approx(m[r] - base);
+        sum += l[r] * scale[r];
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a sum of 0 has no row that counts; NaN stays NaN
+#pragma unroll
+      for (int r = 0; r < 8; ++r) scale[r] *= inv;
+      return sum == 0.f ? -INFINITY : top + log2f(sum);
+    };
+    float scale[8];
+    for (int e = rank * kThreads + tid; e < KS * NT * 4 * 32; e += ctas * kThreads) {
+      const int at = e >> 5, l = e & 31, i = at & 3, nt = (at >> 2) % NT, ks = (at >> 2) / NT;
+      const int h = nt * 8 + 2 * (l & 3) + (i & 1), x = ks * 16 + (i >> 1) * 8 + (l >> 2);
+      if (h >= heads || x >= d) continue;
+      const float lse2 = total_of(nt, i & 1, l, scale);
+      const float* o = slots + NT * 4 * 32 + e;
+      float part[8], v = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) part[r] = r < ctas ? ld_peer(o, r, ctas) : 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ctas) v += part[r] * scale[r];
+      const size_t head = (size_t)fs.b * p.q_heads + head0 + h;
+      static_cast<T*>(p.out)[head * d + x] = from_f32<T>(v);
+      if (x == 0 && p.lse != nullptr) p.lse[head] = lse2 * kLn2;
+    }
+    if (p.track) {
+      if (tid < heads) {
+        const float lse2 = total_of(tid >> 3, tid & 1, (tid & 7) >> 1, scale);
+        sh_lse[tid] = lse2 == -INFINITY ? 0.f : lse2;  // no row: every score is -inf, and stays so
+      }
+      __syncthreads();
+      const int r_first = fs.tile0 * kBlockRows, r_end = min(fs.len, r_first + fs.n * kBlockRows);
+      for (int r = r_first + tid; r < r_end; r += kThreads) {
+        int line;
+        const int page = p.c.page_of(fs.b, r, &line);
+        const float* sc = my_scores + (r - r_first) * p.score_pitch;
+        float add = 0.f;
+        for (int h = 0; h < heads; ++h) add += ex2_approx(sc[h] - sh_lse[h]);
+        if (p.c.real(page)) p.c.weight[p.c.slot_at(page, fs.kvh, line)] += add;
+      }
+    }
+    if (ctas > 1) cluster_sync_all();  // nobody leaves while others look at its shared memory
   }
 }
 
@@ -684,6 +799,8 @@ __global__ void __launch_bounds__(kFinishThreads) paged_track_kernel(const __gri
 // ---- host ----------------------------------------------------------------------
 struct Plan {
   int nt, parts, ks, ctas, rows, score_pitch;
+  int short_ctas;       // CTAs of a pair in the form without further kernels, or 0
+  size_t short_scores;  // its shared memory for scores
   size_t part_o, part_ml, row_info, row_lse, scores, bytes;
 };
 
@@ -707,20 +824,47 @@ auto with_steps(int ks, F f) {
   }
 }
 
+constexpr size_t kMaxSmem = 227 * 1024 - 2048;  // dynamic; the kernels have some static
+
+size_t short_smem(int ks, int nt) {
+  return with_steps(ks, [&](auto k) { return nt == 1 ? Tile<k(), 1, true>::kSmem : Tile<k(), 2, true>::kSmem; });
+}
+
 int per_sm(int ks, int nt) {
-  return with_steps(ks, [&](auto k) { return nt == 1 ? Tile<k(), 1>::kPerSM : Tile<k(), 2>::kPerSM; });
+  return with_steps(ks, [&](auto k) { return nt == 1 ? Tile<k(), 1, false>::kPerSM : Tile<k(), 2, false>::kPerSM; });
 }
 
 Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
-  Plan s;
+  Plan s{};
   const int group = q_heads / c->n_kv_heads;
   s.nt = group <= 8 ? 1 : 2;
   s.parts = (group + 8 * s.nt - 1) / (8 * s.nt);
   s.ks = steps_for(c->head_dim);
   s.rows = c->batch * c->n_kv_heads * s.parts;
   const long long capacity = (long long)c->pages_per_seq * c->page_size;
-  const long long blocks = (capacity + kBlockRows - 1) / kBlockRows * s.rows;
+  auto blocks_of = [](long long rows) { return (rows + kBlockRows - 1) / kBlockRows; };
+  const long long blocks = blocks_of(capacity) * s.rows;
   s.ctas = (int)std::min<long long>(blocks, (long long)kSMs * per_sm(s.ks, s.nt));
+  s.score_pitch = 2;
+  while (s.score_pitch < std::min(8 * s.nt, group)) s.score_pitch *= 2;
+  // The form without further kernels: up to 8 CTAs for each pair while two of them (one,
+  // for heads over 128) have an SM to themselves, with 1024 rows each at most; and one CTA
+  // for each of many pairs of small heads.  us a call there / with equal shares (32 / 8
+  // heads of 128, uniform lengths): 32 pairs of 1000 rows 7.7 / 15.5, of 8000 26 / 32; 128
+  // of 512 13 / 18, of 2000 28 / 34; 1600 of 512 and 64 columns 46 / 62.  Beyond: 320 pairs
+  // of 512 rows with tracking 36 / 28; 384 of 1 to 1500 rows 49 / 42; 150 of 512 and 256
+  // columns 40 / 29: the longest sequence, or the scores' share of an SM, is what counts.
+  const long long pairs = (long long)c->batch * c->n_kv_heads, at_once = s.ks <= 8 ? 2 * kSMs : kSMs;
+  int ctas = 8;
+  while (ctas > 1 && (pairs * ctas > at_once || ctas > blocks_of(capacity))) ctas /= 2;
+  const size_t scores = (size_t)((blocks_of(capacity) + ctas - 1) / ctas) * kBlockRows * s.score_pitch * 4;
+  if (s.parts == 1 && capacity <= 1024 * ctas && (pairs * ctas <= at_once || s.ks <= 4) &&
+      short_smem(s.ks, s.nt) + scores <= kMaxSmem) {  // with or without tracking, so that it changes no result
+    s.short_ctas = ctas;
+    s.short_scores = track ? scores : 0;
+    s.bytes = 256;
+    return s;
+  }
   const size_t h = 8 * s.nt;
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -732,8 +876,6 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   s.part_ml = take(2 * (size_t)s.ctas * h * 8);
   s.row_info = take((size_t)s.rows * 8);
   s.row_lse = take((size_t)s.rows * h * 4);
-  s.score_pitch = 2;
-  while (s.score_pitch < std::min((int)h, group)) s.score_pitch *= 2;
   s.scores = take(track ? (size_t)s.rows * capacity * s.score_pitch * 4 : 0);
   s.bytes = at;
   return s;
@@ -741,13 +883,22 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
 
 template <class T, int KS, int NT>
 int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream_t st) {
-  constexpr int kSmem = Tile<KS, NT>::kSmem;
-  static_assert(kSmem <= 227 * 1024, "shared memory");
-  auto kernel = paged_attention_kernel<T, KS, NT>;
+  using L = Tile<KS, NT, false>;
+  using LS = Tile<KS, NT, true>;
+  static_assert(L::kSmem <= 227 * 1024 && LS::kSmem <= kMaxSmem, "shared memory");
+  if (s.short_ctas > 0) {
+    static std::atomic<uint64_t> allowed{0};
+    auto kernel = paged_attention_kernel<T, KS, NT, true>;
+    int rc = allow_smem(kernel, kMaxSmem, &allowed, "paged_attention");
+    if (rc) return rc;
+    return launch_pdl_cluster(kernel, dim3(p.c.batch * p.c.heads * s.short_ctas), dim3(kThreads),
+                              LS::kSmem + s.short_scores, st, pdl_enabled(), dim3(s.short_ctas), p, tm[0], tm[1]);
+  }
   static std::atomic<uint64_t> allowed{0};
-  int rc = allow_smem(kernel, kSmem, &allowed, "paged_attention");
+  auto kernel = paged_attention_kernel<T, KS, NT, false>;
+  int rc = allow_smem(kernel, L::kSmem, &allowed, "paged_attention");
   if (rc) return rc;
-  rc = launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), kSmem, st, pdl_enabled(), p, tm[0], tm[1]);
+  rc = launch_pdl(kernel, dim3(s.ctas), dim3(kThreads), L::kSmem, st, pdl_enabled(), p, tm[0], tm[1]);
   if (rc) return rc;
   rc = launch_pdl(paged_join_kernel<T, 8 * NT>, dim3(p.c.batch * p.q_heads), dim3(kFinishThreads), 0, st,
                   pdl_enabled(), p);
@@ -836,6 +987,7 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
   p.row_lse = reinterpret_cast<float*>(sc + s.row_lse);
   p.scores = reinterpret_cast<float*>(sc + s.scores);
   p.score_pitch = s.score_pitch;
+  p.ctas = s.short_ctas;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   p.box_rows = std::min(kWarpRows, cache->page_size & -cache->page_size);
   const uint64_t dims[4] = {(uint64_t)cache->head_dim, (uint64_t)cache->page_size, (uint64_t)cache->n_kv_heads,

@@ -319,6 +319,11 @@ ATTEND = [
     (1, 4, 1, 128, 64, [9000], "heads"),             # one sequence over every CTA
     (300, 2, 2, 64, 16, [(7 * i) % 50 for i in range(300)], "heads"),
     (2, 2, 1, 96, 100, [20000, 1], "heads"),
+    (40, 8, 2, 128, 16, [(53 * i) % 701 for i in range(40)], "heads"),   # 80 pairs: clusters of 2
+    (16, 16, 4, 112, 32, [(97 * i) % 900 for i in range(16)], "lines"),  # 64: of 4
+    (70, 4, 2, 256, 8, [(31 * i) % 333 for i in range(70)], "heads"),    # 140 of 256 columns: one CTA each
+    (160, 2, 1, 256, 8, [(31 * i) % 333 for i in range(160)], "heads"),  # 160: equal shares
+    (330, 9, 3, 64, 16, [(7 * i) % 1000 for i in range(330)], "heads"),  # many of 64 columns: one CTA each
 ]
 
 
