@@ -222,6 +222,21 @@ def _rope(x, positions, freqs, out, transpose):
     return out
 
 
+def _leaf_node(x: torch.Tensor):
+    """The node that accumulates leaf ``x``'s gradient, marked with the stream it was first seen on.
+
+    Torch makes it with the first graph that uses the leaf and keeps it as long as any lives; a backward
+    pass waits for its stream, which a capture on another stream cannot (torch then breaks the capture off
+    and leaves its random generator in it).  So a captured call is refused while such a graph is alive.
+    """
+    node = torch.autograd.graph.get_gradient_edge(x).node
+    stream = _raw_stream(x.get_device())
+    if node.metadata.setdefault("pi05_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+        raise ValueError("x is a leaf that an earlier graph, made on another stream, still uses: drop that graph "
+                         "before capturing this call")
+    return node
+
+
 class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, freqs, transpose):
@@ -233,23 +248,11 @@ class _Rope(torch.autograd.Function):
     def backward(ctx, g):
         (positions,) = ctx.saved_tensors
         g = g if g.stride(-1) == 1 else g.contiguous()
-        return _Rope.apply(g, positions, ctx.freqs, not ctx.transpose), None, None, None
-
-
-def _leaf_node(x: torch.Tensor):
-    """The node that accumulates leaf ``x``'s gradient, marked with the stream it was first seen on.
-
-    Torch makes it with the first graph that uses the leaf and keeps it as long as any lives; a backward
-    pass waits for its stream, which a capture on another stream cannot (torch then breaks the capture off
-    and leaves its random generator in it).  So a captured call is refused while such a graph is alive.
-    """
-    node = torch.autograd.graph.get_gradient_edge(x).node
-    stream = torch.cuda.current_stream(x.device).cuda_stream
-    first = node.metadata.setdefault("pi05_stream", stream)
-    if first != stream and torch.cuda.is_current_stream_capturing():
-        raise ValueError("x is a leaf that an earlier graph, made on another stream, still uses: drop that graph "
-                         "before capturing this call")
-    return node
+        if torch.is_grad_enabled():  # a gradient of the gradient is wanted
+            gx = _Rope.apply(g, positions, ctx.freqs, not ctx.transpose)
+        else:
+            gx = _rope(g, positions, ctx.freqs, torch.empty_like(g), not ctx.transpose)
+        return gx, None, None, None
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, transpose: bool = False,

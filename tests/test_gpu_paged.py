@@ -148,6 +148,18 @@ def test_rope_gradient(layout, scaling):
     assert abs(lhs - rhs) <= 20 * F * size
 
 
+def test_rope_second_gradient():
+    """The gradient is linear in what comes in: its own gradient is the forward rotation."""
+    f = RopeFrequencies(64)
+    pos = torch.arange(9, device="cuda")
+    x = rnd(9, 2, 64, dtype=FP, g=gen(6)).requires_grad_(True)
+    w = rnd(9, 2, 64, dtype=FP, g=gen(7)).requires_grad_(True)
+    (gx,) = torch.autograd.grad(rope(x, pos, f), x, w, create_graph=True)
+    v = rnd(9, 2, 64, dtype=FP, g=gen(8))
+    (gw,) = torch.autograd.grad(gx, w, v)
+    check_rope(gw, v, pos, 64, "half")
+
+
 def test_rope_gradient_in_a_graph():
     """A captured forward and backward pass; refused, with nothing broken, while an eager graph of the same leaf
     is alive (torch itself would break the capture off)."""
@@ -161,6 +173,10 @@ def test_rope_gradient_in_a_graph():
         with torch.cuda.graph(graph):
             rope(x, pos, f)
     torch.randn(3, device="cuda")
+    rope(x, pos, f)  # a later graph, gone at once, hides the first from nobody
+    with pytest.raises(ValueError, match="earlier graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            rope(x, pos, f)
     (ge,) = torch.autograd.grad(eager, x, w)
     check_rope(ge, w, pos, 64, "half", back=True)
     del eager
