@@ -862,8 +862,7 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
       short_smem(s.ks, s.nt) + scores <= kMaxSmem) {  // with or without tracking, so that it changes no result
     s.short_ctas = ctas;
     s.short_scores = track ? scores : 0;
-    s.bytes = 256;
-    return s;
+    return s;  // no scratch
   }
   const size_t h = 8 * s.nt;
   size_t at = 0;
@@ -959,7 +958,7 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
     return PI05_ERR_ALIGN;
   }
   const Plan s = make_plan(cache, a->n_q_heads, a->track);
-  if (a->scratch == nullptr || a->scratch_bytes < s.bytes) {
+  if (s.bytes > 0 && (a->scratch == nullptr || a->scratch_bytes < s.bytes)) {
     set_last_error("paged_attention: scratch missing or too small (%zu bytes needed)", s.bytes);
     return PI05_ERR_WORKSPACE;
   }

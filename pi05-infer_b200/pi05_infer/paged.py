@@ -468,11 +468,11 @@ class PagedKVCache:
                 raise ValueError("key_valid must be bool or uint8 [batch, rows] on the cache's device, rows contiguous")
             valid_at, pitch, valid_rows = key_valid.data_ptr(), key_valid.stride(0), key_valid.shape[1]
         # from torch's allocator, call by call: calls on different streams, and graphs, never share it
-        scratch = torch.empty_like(like, memory_format=torch.contiguous_format)
+        scratch = torch.empty_like(like, memory_format=torch.contiguous_format) if need else None
         q_token, q_head, _ = q.stride()
         _run("pi05_paged_attention", self._index, self._at, _ATTEND_ARGS.pack(
             q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), valid_at, q_token, q_head, pitch,
-            valid_rows, heads, dim**-0.5 if scale is None else scale, track, scratch.data_ptr(), need))
+            valid_rows, heads, dim**-0.5 if scale is None else scale, track, scratch.data_ptr() if need else 0, need))
         return (out, lse) if return_lse else out
 
     def _need(self, heads: int, track: bool):

@@ -86,7 +86,8 @@ def test_bad_arguments_are_refused():
     assert attend(n_q_heads=3) == 2 and attend(n_q_heads=0) == 2
     assert attend(cache(weight=None), track=1) == 1
     assert attend(q=HERE + 2) == 3 and attend(q_head_stride=65) == 3
-    assert attend(scratch=None) == 4 and attend(scratch_bytes=64) == 4 and attend(scratch=HERE + 4) == 3
+    big = cache(pages_per_seq=4096, table_pitch=4096)
+    assert attend(big, scratch=None) == 4 and attend(big, scratch_bytes=64) == 4 and attend(big, scratch=HERE + 4) == 3
     assert call("pi05_paged_attention", cache(), None, None)[0] == 1
 
     for args in ((0, 0, 0), (4, -1, 0), (4, 0, -1), (4, 3, 2), (4, 2**31 - 1, 2)):
@@ -111,10 +112,10 @@ def test_sizes():
     ws, sc = paged._fn("pi05_paged_workspace_bytes"), paged._fn("pi05_paged_attention_scratch_bytes")
     assert ws(cache()) >= 16640 + 3 * 2 * (64 + 2) * 4 and ws(cache(batch=0)) == 0 and ws(None) == 0
     # a few short sequences need none; else fp32 partials, and scores of every row that there can be
-    assert 0 < sc(cache(), 8, 0) <= 256 and 0 < sc(cache(), 8, 1) <= 256
+    assert sc(cache(), 8, 0) == 0 and sc(cache(), 8, 1) == 0
     big = dict(pages_per_seq=4096, table_pitch=4096)
     plain, track = sc(cache(**big), 8, 0), sc(cache(**big), 8, 1)
-    assert plain > 256 and track - plain >= 3 * 2 * 4096 * 16 * 4 * 4
+    assert plain > 0 and track - plain >= 3 * 2 * 4096 * 16 * 4 * 4
     assert sc(cache(), 3, 0) == 0 and sc(None, 2, 0) == 0
 
 
