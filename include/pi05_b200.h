@@ -444,8 +444,8 @@ typedef struct Pi05Rotary {
 
 /* out[t, h, :] = x[t, h, :] rotated by positions[t]; `transpose` turns backwards
  * with the same magnitude, which is the gradient of the forward call.  Strides in
- * elements, values of a head contiguous; out may be x itself (same strides), and
- * must not overlap it otherwise.  positions: int32, or int64 with positions_i64;
+ * elements, 0 to 2^31 - 1, values of a head contiguous; out may be x itself (same
+ * strides), and must not overlap it otherwise.  positions: int32, or int64 with positions_i64;
  * any sign.  tokens == 0 is a no-op.  Rotary embedding of modeling_gemma.py:151-216
  * for any position, layout, rotated part and scaling. */
 typedef struct Pi05RopeArgs {

@@ -18,6 +18,14 @@ launches of interest on a small device footprint:
                  (tcgen05 kernel, two key splits merged in-kernel)
   siglip_attention  SigLIP attention: 3 views x 16 heads, 256 x 256, head_dim 72,
                  one launch per layer over 27 layers of q|k|v (143 MB > L2)
+  rope           rotary positions, 32768 tokens x 32 heads of 128, 64 of them rotated,
+                 interleaved (268 MB in, 268 MB out)
+  paged_append   16384 tokens of 8 prompts, 8 query heads and one key-value head of 256,
+                 into fresh pages of 64 rows
+  paged_attention  one token of 64 sequences of 17 to 8192 rows, 32 / 8 heads of 128,
+                 pages of 16 rows (1.08 GB), weights tracked
+  paged_short    one token of 4 sequences of 1000 rows, 32 / 8 heads of 128 (16 MB: L2)
+  paged_evict    one sequence of 65536 rows, 8 key-value heads of 128, cut to 8192
 
 ``python kernel_cases.py duel`` runs the same-box comparison with the reference's
 own Triton kernels (``_geglu_mm_kernel`` and ``_qkv_rope_kernel`` of
@@ -36,10 +44,11 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, os.path.join(HERE, "pi05-infer_b200"))
 
-from pi05_infer import abi, ops  # noqa: E402
+from pi05_infer import abi, ops, paged  # noqa: E402
 
 CASES = ("denoise_geglu", "denoise_down", "prefix_geglu", "prefix_down", "prefix_qkv", "siglip_fc1", "siglip_out",
-         "mqa_attention", "prefix_attention", "siglip_attention")
+         "mqa_attention", "prefix_attention", "siglip_attention", "rope", "paged_append", "paged_attention",
+         "paged_short", "paged_evict")
 
 
 def _bf(t):
@@ -156,6 +165,49 @@ def build(case: str, dev="cuda"):
                 raise RuntimeError(f"pi05_siglip_attention: {rc}")
 
         return f, views * seq * 4 * width * 2, 4 * views * heads * seq * seq * hd
+    if case == "rope":
+        x = rnd(32768, 32, 128)
+        out, pos = torch.empty_like(x), torch.arange(32768, device=dev, dtype=torch.int32)
+        freqs = paged.RopeFrequencies(64, layout="interleaved", device=dev)
+        return (lambda: paged.rope(x, pos, freqs, out=out)), 4 * x.numel(), 3 * 32768 * 32 * 64
+    if case.startswith("paged_"):
+        batch, heads, kv, d, page, lens = {
+            "paged_append": (8, 8, 1, 256, 64, [0] * 8),
+            "paged_attention": (64, 32, 8, 128, 16, [17 + (8192 - 17) * i // 63 for i in range(64)]),
+            "paged_short": (4, 32, 8, 128, 64, [1000] * 4),
+            "paged_evict": (1, 8, 8, 128, 64, [65536]),
+        }[case]
+        tokens = 16384 if case == "paged_append" else batch
+        rows = tokens // batch if case == "paged_append" else max(lens)
+        each = -(-rows // page)
+        c = paged.PagedKVCache.allocate(batch * each, page, kv, d, batch, each, device=dev)
+        for t in (c.k_pages, c.v_pages):
+            t.copy_(rnd(*t.shape))
+        c.weight.copy_(torch.randn(c.weight.shape, device=dev, generator=g).exp())
+        c.pos.copy_(torch.arange(each * page, device=dev).reshape(1, each, 1, page).expand(batch, -1, kv, -1)
+                    .reshape(c.pos.shape))
+        c.page_table.copy_(torch.randperm(batch * each, device=dev, generator=g).reshape(batch, each))
+        start = torch.tensor([lens, lens], dtype=torch.int32, device=dev)
+        c.counts.copy_(start)
+        q, k, v = rnd(tokens, heads, d), rnd(tokens, kv, d), rnd(tokens, kv, d)
+        held = sum(lens) * kv
+        if case == "paged_append":
+            freqs = paged.RopeFrequencies(d, device=dev)
+            cu = torch.arange(0, tokens + 1, rows, device=dev, dtype=torch.int32)
+
+            def f():
+                c.counts.copy_(start)
+                c.append(k, v, q=q, freqs=freqs, cu_tokens=cu)
+
+            return f, 4 * (q.numel() + 2 * k.numel()), 3 * (q.numel() + k.numel())
+        if case == "paged_evict":
+            def f():
+                c.counts.copy_(start)
+                c.evict(8192, recent=512, sinks=4)
+
+            return f, 8 * held + 8192 * 7 // 8 * kv * (8 * d + 16), None
+        track = case == "paged_attention"
+        return (lambda: c.attend(q, track=track)), held * (4 * d + 8 * track) + 4 * q.numel(), 4 * sum(lens) * heads * d
     raise ValueError(case)
 
 

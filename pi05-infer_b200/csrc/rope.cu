@@ -5,8 +5,10 @@
 // Memory bound: x read once, out written once.  A CTA takes a few tokens: it asks for its
 // first values, works out the tokens' cos and sin into shared memory while they are on
 // their way (once for all heads), then streams.  A thread keeps its place within a head
-// and goes from head to head: with the place worked out for every word, integer
-// arithmetic filled 76% of the issue slots at 5.6 TB/s.
+// and goes from head to head; values that pass through go by themselves, so that no warp
+// does both.  32768 tokens of 32 heads of 128, half of each rotated (537 MB): 87 us;
+// with a word's place worked out for every word 99 (integer arithmetic in 76% of the issue
+// slots), with turned and passed words in the same warps 90.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -17,11 +19,13 @@ namespace {
 constexpr int kThreads = 128;
 
 struct RopeParams {
-  long long xt, xh, ot, oh;  // strides, elements
+  int xt, xh, ot, oh;  // strides, elements
   const void* positions;
   const uint64_t* turns;
   FastDiv by_heads, by_pairs;
-  int pos64, tokens, heads, dim, rotary, interleaved, back, per_cta, units, turned, lanes;
+  int pos64, tokens, heads, dim, rotary, interleaved, back, per_cta;
+  int turned, turned_lanes;  // units of a head that turn; threads to a head
+  int passed, passed_lanes;  // units that pass through
   float magnitude;
 };
 
@@ -35,53 +39,66 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const T* x, T* out, cons
   const int n = (int)min((long long)p.per_cta, p.tokens - t0), rows = n * p.heads;
   x += t0 * p.xt;
   out += t0 * p.ot;
-  // `lanes` threads to a head's units, kThreads / lanes heads at a time.
-  const int row0 = tid / p.lanes, u0 = tid - row0 * p.lanes, step = kThreads / p.lanes;
-  bool ready = false;
-  for (int u = u0; u < p.units || u == u0; u += p.lanes) {
-    const bool mine = u < p.units && row0 < step;
-    for (int r = row0; r < rows || !ready; r += J * step) {
-      Unit<T, V> unit[J];
-      int token[J], head[J];
+  // `lanes` threads to a head's units, kThreads / lanes heads at a time, J of them at once.
+  // `first`: what is done between the first loads and the first stores.
+  auto stream = [&](int units, int lanes, auto load, auto store, auto first) {
+    const int row0 = tid / lanes, u0 = tid - row0 * lanes, step = kThreads / lanes;
+    bool begun = false;
+    for (int u = u0; u < units || !begun; u += lanes) {
+      const bool mine = u < units && row0 < step;
+      for (int r = row0; r < rows || !begun; r += J * step) {
+        Unit<T, V> unit[J];
+        int token[J], head[J];
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int row = r + j * step;
-        token[j] = p.by_heads.div(row);
-        head[j] = row - token[j] * p.heads;
-        if (mine && row < rows)
-          unit[j].load(x + token[j] * p.xt + head[j] * p.xh, u, p.turned, p.rotary, p.interleaved);
+        for (int j = 0; j < J; ++j) {
+          const int row = r + j * step;
+          token[j] = p.by_heads.div(row);
+          head[j] = row - token[j] * p.heads;
+          if (mine && row < rows)
+            load(unit[j], x + (long long)token[j] * p.xt + (long long)head[j] * p.xh, u);
+        }
+        if (!begun) first();
+        begun = true;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (mine && r + j * step < rows)
+            store(unit[j], out + (long long)token[j] * p.ot + (long long)head[j] * p.oh, u, token[j]);
       }
-      if (!ready) {
+    }
+  };
+  stream(
+      p.turned, p.turned_lanes,
+      [&](Unit<T, V>& unit, const T* src, int u) { unit.load(src, u, p.turned, p.rotary, p.interleaved); },
+      [&](Unit<T, V>& unit, T* dst, int u, int t) {
+        unit.store(dst, u, p.turned, p.rotary, p.interleaved, cs + t * pairs);
+      },
+      [&]() {
         for (int i = tid; i < n * pairs; i += kThreads) {
-          const int t = p.by_pairs.div(i);
+          const int t = p.by_pairs.div(i), f = i - t * pairs;
           const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + t]
                                         : static_cast<const int32_t*>(p.positions)[t0 + t];
-          const int f = i - t * pairs;
           cs[t * pairs + Unit<T, V>::place(f, p.turned, p.interleaved)] =
               rotation(pos, p.turns[f], p.magnitude, p.back);
         }
         __syncthreads();
-        ready = true;
-      }
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (mine && r + j * step < rows)
-          unit[j].store(out + token[j] * p.ot + head[j] * p.oh, u, p.turned, p.rotary, p.interleaved,
-                        cs + token[j] * pairs);
-    }
-  }
+      });
+  if (p.passed > 0)
+    stream(
+        p.passed, p.passed_lanes, [&](Unit<T, V>& unit, const T* src, int u) { unit.load_row(src + p.rotary, u); },
+        [&](Unit<T, V>& unit, T* dst, int u, int) { unit.store_row(dst + p.rotary, u); }, [] {});
 }
 
 template <class T, int V>
 int rope_run(const void* x, void* out, RopeParams p, cudaStream_t stream) {
   constexpr int J = 4;
   p.turned = rotary_units<V>(p.rotary, p.interleaved);
-  p.units = p.turned + (x == out ? 0 : (p.dim - p.rotary) / V);  // in place, the rest is there already
-  p.lanes = std::min(p.units, kThreads);
+  p.passed = x == out ? 0 : (p.dim - p.rotary) / V;  // in place, the rest is there already
+  p.turned_lanes = std::min(p.turned, kThreads);
+  p.passed_lanes = std::min(p.passed, kThreads);
   p.by_heads = FastDiv(p.heads);
   p.by_pairs = FastDiv(p.rotary / 2);
   // A few batches of loads for a CTA, but for tokens enough to fill the SMs.
-  const int fill = std::max(1, 4 * J * (kThreads / p.lanes) / p.heads);
+  const int fill = std::max(1, 4 * J * (kThreads / p.turned_lanes) / p.heads);
   p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 48 * 1024 / (p.rotary / 2 * (int)sizeof(float2))}));
   return launch_pdl(rope_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kThreads),
                     (size_t)p.per_cta * (p.rotary / 2) * sizeof(float2), stream, pdl_enabled(),
@@ -122,12 +139,17 @@ extern "C" int pi05_rope(const Pi05RopeArgs* a, const Pi05Rotary* rotary, void* 
     set_last_error("rope: in place needs the same strides");
     return PI05_ERR_INVALID_ARG;
   }
+  for (long long stride : {a->x_token_stride, a->x_head_stride, a->out_token_stride, a->out_head_stride})
+    if (stride < 0 || stride >= 1ll << 31) {
+      set_last_error("rope: stride of %lld elements", stride);
+      return PI05_ERR_SHAPE;
+    }
   if (a->tokens == 0) return PI05_OK;
   RopeParams p;
-  p.xt = a->x_token_stride;
-  p.xh = a->x_head_stride;
-  p.ot = a->out_token_stride;
-  p.oh = a->out_head_stride;
+  p.xt = (int)a->x_token_stride;
+  p.xh = (int)a->x_head_stride;
+  p.ot = (int)a->out_token_stride;
+  p.oh = (int)a->out_head_stride;
   p.positions = a->positions;
   p.turns = rotary->turns;
   p.pos64 = a->positions_i64;
