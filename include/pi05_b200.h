@@ -487,7 +487,7 @@ typedef struct Pi05PagedCache {
 size_t pi05_paged_workspace_bytes(const Pi05PagedCache* cache);
 
 /* Appends `tokens` new rows and moves the counts on.  k, v [tokens, n_kv_heads,
- * head_dim] with token and head strides in elements; token t is number
+ * head_dim] with token and head strides in elements (0 to 2^31 - 1); token t is number
  * t - cu_tokens[b] of sequence b's new tokens, for cu_tokens[b] <= t <
  * cu_tokens[b + 1] (int32 device prefix sums [batch + 1] from 0); tokens from
  * cu_tokens[batch] on are padding and leave everything as it was.  cu_tokens NULL:

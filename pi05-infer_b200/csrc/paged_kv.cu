@@ -74,7 +74,7 @@ constexpr int kAppendThreads = 128;
 struct AppendParams {
   const void *k, *v, *q;
   void* q_out;
-  long long kt, kh, vt, vh, qt, qh;  // strides, elements
+  int kt, kh, vt, vh, qt, qh;  // strides, elements
   const int32_t* cu;
   const float* new_weight;
   const uint64_t* turns;
@@ -108,6 +108,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const int t0 = blockIdx.x * p.per_cta;
   const int used = p.cu != nullptr ? min(max(p.cu[c.batch], 0), p.tokens) : p.tokens;
   const int n = max(0, min(p.per_cta, used - t0));  // 0: padding alone
+
+  const T* q = static_cast<const T*>(p.q) + (long long)t0 * p.qt;
+  const T* k = static_cast<const T*>(p.k) + (long long)t0 * p.kt;
+  const T* v = static_cast<const T*>(p.v) + (long long)t0 * p.vt;
+  T* q_out = static_cast<T*>(p.q_out) + (long long)t0 * p.q_heads * c.dim;
 
   // Where the CTA's tokens go, and their cos and sin.
   const bool few = p.cu != nullptr && c.batch <= kAppendThreads;
@@ -173,12 +178,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   constexpr int C = ROT ? 2 : 4;
   const int copy_rows = n * c.heads, copy0 = tid / p.row_lanes, copy_step = kAppendThreads / p.row_lanes;
   const int copy_u = tid - copy0 * p.row_lanes;
-  auto copy_load = [&](Unit<T, V>* unit, const void* src, long long tt, long long hh, int r, int u) {
+  auto copy_load = [&](Unit<T, V>* unit, const T* src, int tt, int hh, int r, int u) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int row = r + j * copy_step, t = p.by_heads.div(row), h = row - t * c.heads;
       if (copy0 < copy_step && row < copy_rows && u < p.row_units)
-        unit[j].load_row(static_cast<const T*>(src) + (t0 + t) * tt + h * hh, u);
+        unit[j].load_row(src + (long long)t * tt + (long long)h * hh, u);
     }
   };
   auto copy_store = [&](const Unit<T, V>* unit, char* pages, int r, int u) {
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         unit[j].store_row(reinterpret_cast<T*>(pages + row_of[t].at + h * c.head_stride), u);
     }
   };
-  auto copy_rest = [&](const void* src, long long tt, long long hh, char* pages, bool all) {
+  auto copy_rest = [&](const T* src, int tt, int hh, char* pages, bool all) {
     for (int u = copy_u; u < p.row_units; u += p.row_lanes)
       for (int r = copy0 + (u == copy_u && !all ? C * copy_step : 0); r < copy_rows; r += C * copy_step) {
         Unit<T, V> unit[C];
@@ -200,12 +205,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
   if constexpr (!ROT) {
     Unit<T, V> k_first[C], v_first[C];
-    copy_load(k_first, p.k, p.kt, p.kh, copy0, copy_u);
-    copy_load(v_first, p.v, p.vt, p.vh, copy0, copy_u);
+    copy_load(k_first, k, p.kt, p.kh, copy0, copy_u);
+    copy_load(v_first, v, p.vt, p.vh, copy0, copy_u);
     find_rows();
     copy_store(k_first, c.k, copy0, copy_u);
     copy_store(v_first, c.v, copy0, copy_u);
-    copy_rest(p.k, p.kt, p.kh, c.k, false);
+    copy_rest(k, p.kt, p.kh, c.k, false);
   } else {  // q and k: `lanes` threads to a head's units, kAppendThreads / lanes heads at a time
     constexpr int J = 2;
     bool ready = false;
@@ -222,9 +227,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
           token[j] = p.by_qk.div(row);
           head[j] = row - token[j] * heads;
           if (mine && row < rows)
-            unit[j].load(head[j] < p.q_heads
-                             ? static_cast<const T*>(p.q) + (t0 + token[j]) * p.qt + head[j] * p.qh
-                             : static_cast<const T*>(p.k) + (t0 + token[j]) * p.kt + (head[j] - p.q_heads) * p.kh,
+            unit[j].load(head[j] < p.q_heads ? q + (long long)token[j] * p.qt + (long long)head[j] * p.qh
+                                             : k + (long long)token[j] * p.kt + (long long)(head[j] - p.q_heads) * p.kh,
                          u, p.turned, p.rotary, p.interleaved);
         }
         if (!ready) find_rows();
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
           if (!mine || r + j * step >= rows) continue;
           T* dst;
           if (head[j] < p.q_heads) {
-            dst = static_cast<T*>(p.q_out) + ((size_t)(t0 + token[j]) * p.q_heads + head[j]) * c.dim;
+            dst = q_out + (long long)(token[j] * p.q_heads + head[j]) * c.dim;
           } else {
             const long long at = row_of[token[j]].at;
             if (at < 0) continue;
@@ -245,7 +249,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       }
     }
   }
-  copy_rest(p.v, p.vt, p.vh, c.v, ROT);
+  copy_rest(v, p.vt, p.vh, c.v, ROT);
   if (p.cu == nullptr) return;
   // Ragged: the CTA that finishes last moves the counts on, when all have read them.
   __syncthreads();
@@ -707,18 +711,24 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, voi
     set_last_error("paged_append: the cache keeps no weights");
     return PI05_ERR_INVALID_ARG;
   }
+  for (long long stride : {a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->q_token_stride,
+                           a->q_head_stride})
+    if (stride < 0 || stride >= 1ll << 31) {
+      set_last_error("paged_append: stride of %lld elements", stride);
+      return PI05_ERR_SHAPE;
+    }
   if (a->tokens == 0) return PI05_OK;
   AppendParams p;
   p.k = a->k;
   p.v = a->v;
   p.q = a->q;
   p.q_out = a->q_out;
-  p.kt = a->k_token_stride;
-  p.kh = a->k_head_stride;
-  p.vt = a->v_token_stride;
-  p.vh = a->v_head_stride;
-  p.qt = a->q_token_stride;
-  p.qh = a->q_head_stride;
+  p.kt = (int)a->k_token_stride;
+  p.kh = (int)a->k_head_stride;
+  p.vt = (int)a->v_token_stride;
+  p.vh = (int)a->v_head_stride;
+  p.qt = (int)a->q_token_stride;
+  p.qh = (int)a->q_head_stride;
   p.cu = a->cu_tokens;
   p.new_weight = a->new_weight;
   p.turns = rot ? rot->turns : nullptr;
