@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // the weights from L2 in every pass took 100 us for 512 pairs of 2049 rows and 409 us for
 // 8 pairs of 65536.  With 8 bits a pass, 26 and 57 us: a weight's top 8 bits are its
 // sign and exponent but one bit, so that most rows of a pass add to the same few counters,
-// one after the other.  This form: EVICT_TOKEN and EVICT_LONG.
+// one after the other.  This form: 10 us (one row to go) and 31 us.
 constexpr int kFew = 4;  // rows to go that are looked for one by one
 constexpr int kBuckets = 2048;
 constexpr int kMaxKeys = 48 * 1024;  // that a CTA holds; later ones are worked out again
