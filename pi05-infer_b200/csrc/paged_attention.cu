@@ -128,32 +128,44 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
   return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// Walks through a CTA's share of the blocks, segment by segment.
+// Starting and joining a pair costs a CTA about as much as kBorder blocks, so each pair
+// counts for so many more than it has: shares of equal numbers of blocks left the CTAs with
+// the shortest sequences, a border at every block, behind: 38 us where the others took 24 (24
+// sequences of 1 to 1500 rows, 16 heads of 80).
+constexpr int kBorder = 2;
+
+// Walks through a CTA's share, segment by segment, in units of a block; the first kBorder
+// units of a pair stand for its border.
 struct Walk {
   int b;
-  long long base, at, end;  // first block of sequence b; the next block; the share's end
+  long long base, at, end;  // first unit of sequence b; the next unit; the share's end
+  long long pair_end;       // of the pair of the last segment
 
   __device__ __forceinline__ bool next(const AttnParams& p, Segment& s) {
-    if (at >= end) return false;
     const int per = p.c.heads * p.parts;
-    int blocks;
-    while (true) {
+    while (at < end) {
       s.len = p.c.rows(b);
-      blocks = (s.len + kBlockRows - 1) / kBlockRows;
-      if (at < base + (long long)blocks * per) break;
-      base += (long long)blocks * per;
-      ++b;
+      const int blocks = (s.len + kBlockRows - 1) / kBlockRows, units = blocks > 0 ? blocks + kBorder : 0;
+      if (at >= base + (long long)units * per) {
+        base += (long long)units * per;
+        ++b;
+        continue;
+      }
+      const int pair = (int)divide(at - base, units);
+      const long long first_block = base + (long long)pair * units + kBorder;
+      pair_end = first_block + blocks;
+      s.tile0 = (int)max(at - first_block, 0ll);
+      at = min(end, pair_end);
+      s.n = (int)(at - first_block) - s.tile0;
+      if (s.n <= 0) continue;  // nothing but the border
+      s.b = b;
+      s.row = b * per + pair;
+      s.kvh = pair / p.parts;
+      s.part = pair - s.kvh * p.parts;
+      s.whole = s.n == blocks;
+      return true;
     }
-    const int pair = (int)divide(at - base, blocks);
-    s.b = b;
-    s.row = b * per + pair;
-    s.kvh = pair / p.parts;
-    s.part = pair - s.kvh * p.parts;
-    s.tile0 = (int)((at - base) - (long long)pair * blocks);
-    s.n = (int)min((long long)(blocks - s.tile0), end - at);
-    s.whole = s.n == blocks;
-    at += s.n;
-    return true;
+    return false;
   }
 };
 
@@ -238,11 +250,11 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
   pdl_launch_dependents();
 
   const int d = p.c.dim;
-  long long total = 0, n = 0, lo = 0;  // all blocks, the CTAs that share them, this one's first
+  long long total = 0, n = 0;  // all units, and the CTAs that share them
   const long long cta = blockIdx.x;
   int rank = 0;
   Segment fs;             // of the copies, which run ahead of the products
-  Walk ahead{0, 0, 0, 0};
+  Walk ahead{0, 0, 0, 0, 0};
   bool more;
   if constexpr (SHORT) {
     const int pair = blockIdx.x / p.ctas;  // the grid is a line of clusters
@@ -263,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     more = fs.n > 0;
     __syncthreads();  // the barriers are there
   } else {
-    // All blocks there are, then the sequence that this CTA's share begins in: one scan for
+    // All units there are, then the sequence that this CTA's share begins in: one scan for
     // up to kThreads sequences, else a sum and a scan of one part after the other.
     const int per_block = p.c.heads * p.parts;
     const bool few = p.c.batch <= kThreads;
@@ -278,24 +290,23 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
       for (int i = 0; i < w; ++i) own += sh_sum[i];
       return own;
     };
-    auto blocks_of = [&](int b) {
+    auto units_of = [&](int b) {
       const int len = p.c.rows(b);
       if (blockIdx.x == 0 && len != p.c.counts[b]) report_status(p.c.status, PI05_DEV_BAD_INDEX);
-      return (long long)((len + kBlockRows - 1) / kBlockRows) * per_block;
+      return len > 0 ? (long long)((len + kBlockRows - 1) / kBlockRows + kBorder) * per_block : 0ll;
     };
     long long own = 0;
-    for (int b = tid; b < p.c.batch; b += kThreads) own += blocks_of(b);
+    for (int b = tid; b < p.c.batch; b += kThreads) own += units_of(b);
     long long incl = scan(own);
     for (int i = 0; i < kWarps; ++i) total += sh_sum[i];
     n = min((long long)gridDim.x, total);
     if (cta >= n) return;
-    lo = divide(cta * total, n);
-    const long long hi = divide((cta + 1) * total, n);
+    const long long lo = divide(cta * total, n), hi = divide((cta + 1) * total, n);
     long long before = 0;
     for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
       const int b = b0 + tid;
       if (!few) {
-        own = b < p.c.batch ? blocks_of(b) : 0;
+        own = b < p.c.batch ? units_of(b) : 0;
         incl = before + scan(own);
         for (int i = 0; i < kWarps; ++i) before += sh_sum[i];
       }
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     }
     __syncthreads();
 
-    ahead = Walk{sh_b, sh_base, lo, hi};
+    ahead = Walk{sh_b, sh_base, lo, hi, 0};
     more = ahead.next(p, fs);
   }
 
@@ -324,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
   // The warp's copies run ahead of its products, across the segments' borders.
   Segment next = fs;
   Walk walk = ahead;
+  bool have = SHORT || more;  // a segment to work on, `next`: now, since `more` runs ahead
   int fj = 0;
   auto next_ref = [&]() {
     if (more && fj == fs.n) {
@@ -367,15 +379,13 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         }
       }
   };
-  load_q(next);
-  bool have = true;
+  if (have) load_q(next);
   for (int slot = 2 * (int)cta; have; slot |= 1) {
     const Segment s = next;
     const int heads = min(H, p.group - s.part * H), head0 = s.kvh * p.group + s.part * H;
     if (!SHORT && s.tile0 == 0 && tid == 0) {
-      // the row's last block, and the CTA that has it
-      const long long end = walk.at - s.n + (s.len + kBlockRows - 1) / kBlockRows;
-      p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)divide(end * n - 1, total));
+      // the CTA that has the pair's last block
+      p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)divide(walk.pair_end * n - 1, total));
     }
     float o[KS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
