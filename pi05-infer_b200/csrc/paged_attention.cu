@@ -345,13 +345,15 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     if (!more) return Ref{0, 0, 0, false, false};
     return look_up(p, fs, ((fs.tile0 + fj++) * kWarps + w) * kWarpRows, lane);
   };
-  uint32_t live[S];  // rows that count of the tiles in flight, the oldest first
+  int flying = 0;    // tiles asked for and not read yet
+  uint32_t live[S];  // rows that count of these, the oldest first
   Ref ref = next_ref();
 #pragma unroll
   for (int j = 0; j < S - 1; ++j) {
     const Ref now = ref;
     ref = next_ref();
     live[j] = now.tile ? fetch<KS, NT, SHORT>(p, &tm_k, &tm_v, now, bars + j, ring + j * 2 * L::kBytes, lane, policy) : 0u;
+    flying += now.tile;
   }
   int stage = 0;
   uint32_t phase = 0;
@@ -409,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         ref = next_ref();
         const int to = stage == 0 ? S - 1 : stage - 1;
         live[S - 1] = now.tile ? fetch<KS, NT, SHORT>(p, &tm_k, &tm_v, now, bars + to, ring + to * 2 * L::kBytes, lane, policy) : 0u;
+        flying += now.tile ? 0 : -1;
       }
       const uint32_t tile = ring + stage * 2 * L::kBytes, rows = live[0];
       if (++stage == S) {
@@ -602,6 +605,15 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     }
   }
 
+  if (broken) {  // no copy may land in the shared memory of a CTA that has ended
+    for (; flying > 0; --flying) {
+      mbar_wait(bars + stage, phase);
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  }
   if constexpr (SHORT) {
     __shared__ float sh_lse[H];
     const int ctas = p.ctas, heads = p.group, head0 = fs.kvh * p.group;
