@@ -241,6 +241,12 @@ struct Pages {
   }
 };
 
+// Whether every pointer (or none) starts on a multiple of n bytes.
+template <class... P>
+bool aligned_to(size_t n, P... p) {
+  return (((reinterpret_cast<uintptr_t>(p) % n) == 0) && ...);
+}
+
 // Lets a kernel have `bytes` of dynamic shared memory, once for each device (the call
 // costs a microsecond).  `done`: a static of the kernel's own.
 template <class K>

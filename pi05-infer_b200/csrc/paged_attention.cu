@@ -978,8 +978,11 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
     set_last_error("paged_attention: the cache keeps no weights");
     return PI05_ERR_INVALID_ARG;
   }
-  if ((reinterpret_cast<uintptr_t>(a->q) & 3) || a->q_token_stride % 2 || a->q_head_stride % 2) {
-    set_last_error("paged_attention: q rows must start on 4-byte boundaries");
+  // The stride of a dimension of one element means nothing.
+  const long long q_token = cache->batch > 1 ? a->q_token_stride : 0;
+  const long long q_head = a->n_q_heads > 1 ? a->q_head_stride : 0;
+  if (!aligned_to(4, a->q, a->lse) || !aligned_to(2, a->out) || q_token % 2 || q_head % 2) {
+    set_last_error("paged_attention: q rows and lse must start on 4-byte boundaries, out on 2-byte ones");
     return PI05_ERR_ALIGN;
   }
   const Plan s = make_plan(cache, a->n_q_heads, a->track);
@@ -996,8 +999,8 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
   p.out = a->out;
   p.lse = a->lse;
   p.valid = a->key_valid;
-  p.qt = a->q_token_stride;
-  p.qh = a->q_head_stride;
+  p.qt = q_token;
+  p.qh = q_head;
   p.valid_pitch = a->valid_pitch;
   p.valid_rows = a->key_valid != nullptr ? a->valid_rows : 0;
   p.q_heads = a->n_q_heads;

@@ -29,6 +29,10 @@ int paged_check(const Pi05PagedCache* c, const char* op, Pages* out) {
     set_last_error("%s: cache rows must start on 16-byte boundaries", op);
     return PI05_ERR_ALIGN;
   }
+  if (!aligned_to(4, c->weight, c->pos, c->page_table, c->counts)) {
+    set_last_error("%s: weight, pos, page_table and counts must be 4-byte aligned", op);
+    return PI05_ERR_ALIGN;
+  }
   if (c->workspace == nullptr || c->workspace_bytes < kWsAccumOffset + paged_moves_bytes(c)) {
     set_last_error("%s: workspace missing or too small", op);
     return PI05_ERR_WORKSPACE;
@@ -337,7 +341,7 @@ __device__ __forceinline__ Victim warp_least(Victim v) {
 
 // Moves of row list `moves`: [0] their number (-1: the sequence stays as it is), [1] the
 // rows left, then the holes, ascending, and from [2 + left] on the rows that fill them.
-// `move_here`: few enough to do them on the spot.  FIT: a CTA holds all its keys.
+// `move_here`: few enough, however long the sequence, to do them on the spot.  FIT: a CTA holds all its keys.
 template <int NT, bool FIT>
 __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant__ Pages c, int budget, int recent,
                                                           int sinks, int ctas, int held, int move_here) {
@@ -425,7 +429,8 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
 
   // A few rows to go (one, in a program that evicts after every token): one by one, the
   // least that comes after the last.
-  if (move_here && len - budget <= kFew) {
+  if (len - budget <= kFew) {
+    if (tid == 0 && rank == 0) moves[0] = -1;  // done here
     Victim gone[kFew];
     const int few = len - budget;
 #pragma unroll
@@ -710,6 +715,11 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, voi
   if (a->new_weight != nullptr && c.weight == nullptr) {
     set_last_error("paged_append: the cache keeps no weights");
     return PI05_ERR_INVALID_ARG;
+  }
+  if (!aligned_to(2, a->k, a->v, a->q, a->q_out) || !aligned_to(4, a->cu_tokens, a->new_weight) ||
+      (rot != nullptr && !aligned_to(8, rot->turns))) {
+    set_last_error("paged_append: pointer not aligned to its elements");
+    return PI05_ERR_ALIGN;
   }
   for (long long stride : {a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->q_token_stride,
                            a->q_head_stride})

@@ -144,6 +144,11 @@ extern "C" int pi05_rope(const Pi05RopeArgs* a, const Pi05Rotary* rotary, void* 
       set_last_error("rope: stride of %lld elements", stride);
       return PI05_ERR_SHAPE;
     }
+  if (!aligned_to(a->dtype == PI05_FP32 ? 4 : 2, a->x, a->out) || !aligned_to(a->positions_i64 ? 8 : 4, a->positions) ||
+      !aligned_to(8, rotary->turns)) {
+    set_last_error("rope: pointer not aligned to its elements");
+    return PI05_ERR_ALIGN;
+  }
   if (a->tokens == 0) return PI05_OK;
   RopeParams p;
   p.xt = (int)a->x_token_stride;

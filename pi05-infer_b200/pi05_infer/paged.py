@@ -286,8 +286,9 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
         out = torch.empty_like(x)
     elif grad:
         raise ValueError("out= is not differentiable")
-    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index or out.stride(2) != 1:
-        raise ValueError("out must have x's shape, type and device, contiguous in dim")
+    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index or out.stride(2) != 1 or \
+            (out.requires_grad and torch.is_grad_enabled()):
+        raise ValueError("out must have x's shape, type and device, contiguous in dim, and need no gradient")
     return _rope(x, positions, freqs, out, bool(transpose))
 
 
@@ -377,6 +378,8 @@ class PagedKVCache:
                 t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
                freqs: Optional[RopeFrequencies] = None, cu_tokens: Optional[torch.Tensor] = None,
@@ -441,11 +444,11 @@ class PagedKVCache:
 
         ``scale`` is ``head_dim ** -0.5`` if not given.  ``key_valid`` (bool or uint8 ``[batch, n]``):
         rows that are False are left out, whatever they hold; rows from ``n`` on count (a prompt's
-        padding mask need not grow with the sequence).  ``track`` adds the probabilities
-        to the cache's ``weight`` (its scratch holds a score for every row there can be and query head, so
-        a table much longer than its sequences costs memory).  A sequence with no row gives zeros (lse ``-inf``).  Returns
-        ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32 natural-log sums
-        ``[batch, heads]``.
+        padding mask need not grow with the sequence).  ``track`` adds the probabilities to the
+        cache's ``weight`` (its scratch holds a score for every row there can be and query head, so a
+        table much longer than its sequences costs memory).  A sequence with no row gives zeros (lse
+        ``-inf``).  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
+        natural-log sums ``[batch, heads]``.
         """
         self._rows(q, "q", None)
         batch, heads, dim = q.shape

@@ -406,6 +406,22 @@ def test_attend_large_scores():
     check_attend(c, t, q, scale=-0.3)
 
 
+def test_gradients_are_refused():
+    """Nothing that would need one is dropped in silence."""
+    c, _ = make(2, 1, 64, 16, 32)
+    f, x = RopeFrequencies(64), rnd(2, 1, 64)
+    g = x.clone().requires_grad_(True)
+    for call in (lambda: c.append(g, x), lambda: c.append(x, g), lambda: c.append(x, x, q=g, freqs=f),
+                 lambda: c.attend(g), lambda: rope(g, torch.zeros(2, device="cuda", dtype=torch.int32), f, out=x),
+                 lambda: rope(x, torch.zeros(2, device="cuda", dtype=torch.int32), f, out=g)):
+        with pytest.raises(ValueError, match="gradient|differentiable"):
+            call()
+    with torch.no_grad():
+        c.append(g, g, q=g, freqs=f)
+        c.attend(g)
+    assert c.lens.tolist() == [1, 1] and c.read_status() == 0
+
+
 def test_attend_bad_pages_and_counts():
     c, t = make(3, 1, 64, 16, 64)
     c.page_table[0, 1], c.page_table[0, 2], c.page_table[1, 0] = -7, c.num_pages, 2**31 - 1
@@ -458,6 +474,7 @@ def test_attend_shared_pages_two_streams():
     (1, 2, 8, 16, [20000], 19998, 1000, 4, "lines"),     # two rows to go, in a cluster
     (2, 1, 8, 64, [8200, 30], 8196, 4, 0, "heads"),      # four, in two CTAs
     (1, 1, 8, 16, [8300], 100, 0, 0, "heads"),
+    (3, 2, 64, 16, [203, 900, 201], 200, 20, 2, "heads"),  # three to go, one to go, and 700, in pages for many more
 ])
 def test_evict(dtype, batch, heads, dim, page, lens, budget, recent, sinks, pages):
     c, t = make(batch, heads, dim, page, max(lens) + 3, dtype=dtype, layout=pages)

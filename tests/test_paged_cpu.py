@@ -39,7 +39,8 @@ BAD_CACHES = [
     (dict(page_size=0), 2), (dict(num_pages=0), 2), (dict(batch=0), 2), (dict(n_kv_heads=0), 2),
     (dict(pages_per_seq=5), 2), (dict(pages_per_seq=1 << 28, table_pitch=1 << 28), 2), (dict(k_pages=HERE + 8), 3),
     (dict(page_stride=2 * 16 * 64 + 4), 3), (dict(row_stride=68), 3), (dict(workspace=None), 4),
-    (dict(workspace_bytes=1000), 4), (dict(workspace=HERE + 16), 3),
+    (dict(workspace_bytes=1000), 4), (dict(workspace=HERE + 16), 3), (dict(counts=HERE + 2), 3),
+    (dict(weight=HERE + 1), 3), (dict(pos=HERE + 2), 3), (dict(page_table=HERE + 3), 3),
 ]
 
 
@@ -74,6 +75,9 @@ def test_bad_arguments_are_refused():
     assert append(tokens=4) == 2 and append(tokens=-1, cu_tokens=HERE) == 2
     assert append(new_weight=HERE) == 1
     assert append(tokens=0, cu_tokens=HERE) == 0         # nothing to do
+    assert append(k=HERE + 1) == 3 and append(v=HERE + 1) == 3 and append(cu_tokens=HERE + 2) == 3
+    assert append(paged.Pi05Rotary(HERE + 4, 64, 0, 1.0)) == 3
+    assert append(k_token_stride=1 << 31) == 2 and append(v_head_stride=-64) == 2
     assert call("pi05_paged_append", cache(), None, None)[0] == 1
 
     def attend(c=None, **kw):
@@ -85,7 +89,8 @@ def test_bad_arguments_are_refused():
     assert attend(q=None) == 1 and attend(out=None) == 1
     assert attend(n_q_heads=3) == 2 and attend(n_q_heads=0) == 2
     assert attend(cache(weight=None), track=1) == 1
-    assert attend(q=HERE + 2) == 3 and attend(q_head_stride=65) == 3
+    assert attend(q=HERE + 2) == 3 and attend(q_head_stride=65) == 3 and attend(q_token_stride=65) == 3
+    assert attend(out=HERE + 1) == 3 and attend(lse=HERE + 2) == 3
     big = cache(pages_per_seq=4096, table_pitch=4096)
     assert attend(big, scratch=None) == 4 and attend(big, scratch_bytes=64) == 4 and attend(big, scratch=HERE + 4) == 3
     assert call("pi05_paged_attention", cache(), None, None)[0] == 1
@@ -105,6 +110,9 @@ def test_bad_arguments_are_refused():
     assert turn(tokens=-1) == 2 and turn(heads=0) == 2 and turn(dim=62) == 2
     assert turn(r=paged.Pi05Rotary(HERE, 3, 0, 1.0)) == 2 and turn(r=paged.Pi05Rotary(HERE, 0, 0, 1.0)) == 2
     assert turn(ot=256) == 1  # in place, but with other strides
+    assert turn(x=HERE + 1) == 3 and turn(out=HERE + 2, dtype=2) == 3 and turn(pos=HERE + 2) == 3
+    assert turn(r=paged.Pi05Rotary(HERE + 4, 64, 0, 1.0)) == 3
+    assert turn(out=HERE + 4096, xt=1 << 31) == 2 and turn(out=HERE + 4096, oh=-64) == 2
     assert turn(tokens=0) == 0
 
 
