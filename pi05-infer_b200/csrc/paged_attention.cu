@@ -928,7 +928,8 @@ int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream
                   pdl_enabled(), p);
   if (rc || !p.track) return rc;
   const int per_cta = (p.score_pitch == 16 ? 2 : 4) * kFinishThreads;
-  const dim3 grid(p.c.batch * p.c.heads, std::min((p.c.capacity + per_cta - 1) / per_cta, 65535));
+  const int pairs = p.c.batch * p.c.heads;  // CTAs for the longest there can be, but not many more than can run
+  const dim3 grid(pairs, std::min((p.c.capacity + per_cta - 1) / per_cta, std::max(8, 16384 / pairs)));
   if constexpr (NT == 2)
     return launch_pdl(paged_track_kernel<16, 16>, grid, dim3(kFinishThreads), 0, st, pdl_enabled(), p);
   else
