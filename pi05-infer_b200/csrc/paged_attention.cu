@@ -929,7 +929,7 @@ int launch(const AttnParams& p, const Plan& s, const CUtensorMap* tm, cudaStream
   if (rc || !p.track) return rc;
   const int per_cta = (p.score_pitch == 16 ? 2 : 4) * kFinishThreads;
   const int pairs = p.c.batch * p.c.heads;  // CTAs for the longest there can be, but not many more than can run
-  const dim3 grid(pairs, std::min((p.c.capacity + per_cta - 1) / per_cta, std::max(8, 16384 / pairs)));
+  const dim3 grid(pairs, std::min((p.c.capacity + per_cta - 1) / per_cta, std::max(16, 4096 / pairs)));
   if constexpr (NT == 2)
     return launch_pdl(paged_track_kernel<16, 16>, grid, dim3(kFinishThreads), 0, st, pdl_enabled(), p);
   else
