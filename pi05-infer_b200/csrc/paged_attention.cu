@@ -870,17 +870,19 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   s.score_pitch = 2;
   while (s.score_pitch < std::min(8 * s.nt, group)) s.score_pitch *= 2;
   // The form without further kernels: up to 8 CTAs for each pair while two of them (one,
-  // for heads over 128) have an SM to themselves, with 1024 rows each at most; and one CTA
-  // for each of many pairs of small heads.  us a call there / with equal shares (32 / 8
-  // heads of 128, uniform lengths): 32 pairs of 1000 rows 7.7 / 15.5, of 8000 26 / 32; 128
-  // of 512 13 / 18, of 2000 28 / 34; 1600 of 512 and 64 columns 46 / 62.  Beyond: 320 pairs
-  // of 512 rows with tracking 36 / 28; 384 of 1 to 1500 rows 49 / 42; 150 of 512 and 256
-  // columns 40 / 29: the longest sequence, or the scores' share of an SM, is what counts.
-  const long long pairs = (long long)c->batch * c->n_kv_heads, at_once = s.ks <= 8 ? 2 * kSMs : kSMs;
+  // for heads over 128) have an SM to themselves, with 1024 rows each at most (512).  us a
+  // call there / with equal shares (32 / 8 heads of 128, uniform lengths): 32 pairs of 1000
+  // rows 7.8 / 13.3, of 8000 26 / 30; 128 of 512 13 / 16, of 2000 28 / 29, of 1 to 2000 24 /
+  // 21; 120 of 512 rows of 256 columns 22 / 27.  Beyond, the longest sequence or the scores'
+  // share of an SM decides: 320 pairs of 512 rows, tracked, 36 / 28; 384 of 1 to 1500 rows
+  // of 80 columns 30 / 25; 150 of 512 rows of 256 columns 41 / 29; 1600 of 512 rows of 64
+  // columns 44 / 42.
+  const bool narrow = s.ks <= 8;
+  const long long pairs = (long long)c->batch * c->n_kv_heads, at_once = narrow ? 2 * kSMs : kSMs;
   int ctas = 8;
   while (ctas > 1 && (pairs * ctas > at_once || ctas > blocks_of(capacity))) ctas /= 2;
   const size_t scores = (size_t)((blocks_of(capacity) + ctas - 1) / ctas) * kBlockRows * s.score_pitch * 4;
-  if (s.parts == 1 && capacity <= 1024 * ctas && (pairs * ctas <= at_once || s.ks <= 4) &&
+  if (s.parts == 1 && capacity <= (narrow ? 1024 : 512) * ctas && pairs * ctas <= at_once &&
       short_smem(s.ks, s.nt) + scores <= kMaxSmem) {  // with or without tracking, so that it changes no result
     s.short_ctas = ctas;
     s.short_scores = track ? scores : 0;

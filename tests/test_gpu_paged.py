@@ -339,7 +339,8 @@ ATTEND = [
     (16, 16, 4, 112, 32, [(97 * i) % 900 for i in range(16)], "lines"),  # 64: of 4
     (70, 4, 2, 256, 8, [(31 * i) % 333 for i in range(70)], "heads"),    # 140 of 256 columns: one CTA each
     (160, 2, 1, 256, 8, [(31 * i) % 333 for i in range(160)], "heads"),  # 160: equal shares
-    (330, 9, 3, 64, 16, [(7 * i) % 1000 for i in range(330)], "heads"),  # many of 64 columns: one CTA each
+    (250, 3, 1, 64, 8, [(31 * i) % 222 for i in range(250)], "heads"),   # 250 of 64: one CTA each
+    (330, 9, 3, 64, 16, [(7 * i) % 1000 for i in range(330)], "heads"),  # many of 64 columns: equal shares
 ]
 
 
