@@ -10,7 +10,8 @@
 // pairs, laid end to end, are dealt out in equal contiguous shares to a fixed grid, so
 // lengths may differ at will and the host need not know them.  A share that covers a
 // whole pair writes its result; pairs cut between CTAs leave fp32 partials (o, m, l)
-// that the join kernel adds up in order.
+// that the join kernel adds up in order.  Few short sequences take a cluster of CTAs for
+// each pair instead, and no other kernel (SHORT, and make_plan).
 //
 // A warp takes 16 rows at a time, brought by TMA into a ring of its own (no block barrier
 // in the loop), and its copies run ahead of its products across the borders of pairs.  The
@@ -18,7 +19,7 @@
 // then O^T += V^T P^T, where the probabilities pass from one fragment layout to the other
 // by a matrix transpose in registers; with the heads as N = 8, half as many products and
 // accumulators as with 16 padded query rows.  The probabilities enter the second product
-// in the cache's 16-bit type (2^-9 relative for bf16, the size of the output's own
+// in the cache's 16-bit type (2^-8 relative at most for bf16, as the output's own
 // rounding); m, l and o stay fp32, l sums the unrounded ones.
 //
 // Measured: 2 x 131072 rows, 32 / 8 heads of 128: 157 us = 6.8 TB/s + 5 us for the join.
