@@ -407,6 +407,28 @@ def test_attend_large_scores():
     check_attend(c, t, q, scale=-0.3)
 
 
+def test_attend_two_graphs_at_once():
+    """Two captured calls on one cache (read only), replayed on two streams: each has scratch of its own."""
+    c, t = make(2, 2, 128, 16, 9000)
+    c.counts[0] = torch.tensor([9000, 5000])
+    t.counts[0] = [9000, 5000]
+    qs = [rnd(2, 8, 128, g=gen(i)) for i in range(2)]
+    want = [check_attend(c, t, q) for q in qs]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in qs], [], []
+    for q, s in zip(qs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(c.attend(q))
+        graphs.append(g)
+    for _ in range(20):
+        for g, s, o in zip(graphs, streams, outs):
+            with torch.cuda.stream(s):
+                o.zero_()
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want)) and c.read_status() == 0
+
+
 def test_gradients_are_refused():
     """Nothing that would need one is dropped in silence."""
     c, _ = make(2, 1, 64, 16, 32)
