@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <initializer_list>
 
 #include "../../include/pi05_b200.h"
 #include "host_util.h"
@@ -16,6 +17,12 @@ namespace pi05 {
 
 constexpr int kMaxRotary = 512;
 constexpr int kSMs = 148;
+
+// Whether every pointer (or none) starts on a multiple of n bytes.
+template <class... P>
+bool aligned_to(size_t n, P... p) {
+  return (((reinterpret_cast<uintptr_t>(p) % n) == 0) && ...);
+}
 
 // ---- element types ---------------------------------------------------------
 template <class T>
@@ -77,17 +84,19 @@ __device__ __forceinline__ float2 rotation(long long position, uint64_t turns, f
 
 // What one thread does at a time: V pairs of the half layout (two words of V elements),
 // or V / 2 pairs of the interleaved one, or a word of the values that pass through.  V = 1
-// takes single elements, a pair at a time.
+// takes single elements, a pair at a time (half layout with an odd number of pairs, or
+// rows at odd elements).
 template <int V>
 __host__ __device__ __forceinline__ int rotary_units(int rotary, bool interleaved) {
   return rotary / (interleaved && V > 1 ? V : 2 * V);
 }
 
-// (a, b) -> (a c - b s, b c + a s)
+// (a, b) -> (a c - b s, b c + a s); which product is fused stands here, so that every word
+// width gives the same bits.
 __device__ __forceinline__ void turn(float& a, float& b, float2 r) {
   const float x = a;
-  a = x * r.x - b * r.y;
-  b = b * r.x + x * r.y;
+  a = fmaf(-b, r.y, x * r.x);
+  b = fmaf(x, r.y, b * r.x);
 }
 
 // A unit in registers between its load and its store, so that a thread has several
@@ -127,36 +136,55 @@ struct Unit<T, 1> {
 __device__ __forceinline__ uint4 ld16(const void* p) { return *static_cast<const uint4*>(p); }
 __device__ __forceinline__ void st16(void* p, const uint4& v) { *static_cast<uint4*>(p) = v; }
 
-// 16-byte words: V = 8 of the 16-bit types, 4 of fp32.
+// 4 * NW bytes that are loaded and stored at once, and the 32-bit words in them.
+template <int NW>
+struct WordOf;
+template <>
+struct WordOf<4> {
+  using type = uint4;
+  static __device__ __forceinline__ void split(uint32_t (&x)[4], uint4 v) {
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  }
+  static __device__ __forceinline__ uint4 join(const uint32_t (&x)[4]) { return make_uint4(x[0], x[1], x[2], x[3]); }
+};
+template <>
+struct WordOf<2> {
+  using type = uint2;
+  static __device__ __forceinline__ void split(uint32_t (&x)[2], uint2 v) { x[0] = v.x, x[1] = v.y; }
+  static __device__ __forceinline__ uint2 join(const uint32_t (&x)[2]) { return make_uint2(x[0], x[1]); }
+};
+template <>
+struct WordOf<1> {
+  using type = uint32_t;
+  static __device__ __forceinline__ void split(uint32_t (&x)[1], uint32_t v) { x[0] = v; }
+  static __device__ __forceinline__ uint32_t join(const uint32_t (&x)[1]) { return x[0]; }
+};
+
+// Words of 4, 8 or 16 bytes: V = 2, 4 or 8 of the 16-bit types, 2 or 4 of fp32.
 template <class T, int V>
 struct Unit {
-  static_assert(V * sizeof(T) == 16, "a word");
-  uint4 a, b;
+  static constexpr int NW = V * sizeof(T) / 4;
+  using Words = WordOf<NW>;
+  using Word = typename Words::type;
+  Word a, b;
   static __device__ __forceinline__ int place(int i, int turned, bool interleaved) {
     const int per = interleaved ? V / 2 : V;
+    if (V == 2 && interleaved) return i;  // a pair to a unit
     return (i % per / 2 * turned + i / per) * 2 + (i & 1);
   }
-  __device__ __forceinline__ void load_row(const T* src, int u) { a = ld16(src + u * V); }
-  __device__ __forceinline__ void store_row(T* dst, int u) const { st16(dst + u * V, a); }
+  static __device__ __forceinline__ Word get(const T* p) { return *reinterpret_cast<const Word*>(p); }
+  static __device__ __forceinline__ void put(T* p, const Word& v) { *reinterpret_cast<Word*>(p) = v; }
+  __device__ __forceinline__ void load_row(const T* src, int u) { a = get(src + u * V); }
+  __device__ __forceinline__ void store_row(T* dst, int u) const { put(dst + u * V, a); }
   __device__ __forceinline__ void load(const T* src, int u, int turned, int rotary, bool interleaved) {
-    a = ld16(src + (u < turned ? u * V : rotary + (u - turned) * V));
-    if (u < turned && !interleaved) b = ld16(src + rotary / 2 + u * V);
+    a = get(src + (u < turned ? u * V : rotary + (u - turned) * V));
+    if (u < turned && !interleaved) b = get(src + rotary / 2 + u * V);
   }
-  // r: cos and sin of two pairs.  Interleaved: each word a pair (16 bit), or each two (fp32).
-  static __device__ __forceinline__ void turn_pairs(uint32_t& x, uint32_t& y, float4 r) {
-    float2 v = unpack2<T>(x), w = unpack2<T>(y);
-    turn(v.x, v.y, make_float2(r.x, r.y));
-    turn(w.x, w.y, make_float2(r.z, r.w));
+  // One pair in a word of two 16-bit values, or in two words of fp32.
+  static __device__ __forceinline__ void turn_word(uint32_t& x, float c, float s) {
+    float2 v = unpack2<T>(x);
+    turn(v.x, v.y, make_float2(c, s));
     x = pack2<T>(v.x, v.y);
-    y = pack2<T>(w.x, w.y);
-  }
-  // Half layout: two values of one half and their partners.
-  static __device__ __forceinline__ void turn_halves(uint32_t& x, uint32_t& y, float4 r) {
-    float2 v = unpack2<T>(x), w = unpack2<T>(y);
-    turn(v.x, w.x, make_float2(r.x, r.y));
-    turn(v.y, w.y, make_float2(r.z, r.w));
-    x = pack2<T>(v.x, v.y);
-    y = pack2<T>(w.x, w.y);
   }
   static __device__ __forceinline__ void turn_f32(uint32_t& x, uint32_t& y, float c, float s) {
     float v = __uint_as_float(x), w = __uint_as_float(y);
@@ -164,38 +192,72 @@ struct Unit {
     x = __float_as_uint(v);
     y = __float_as_uint(w);
   }
+  // Half layout: two 16-bit values of one half and their partners.
+  static __device__ __forceinline__ void turn_halves(uint32_t& x, uint32_t& y, float4 r) {
+    float2 v = unpack2<T>(x), w = unpack2<T>(y);
+    turn(v.x, w.x, make_float2(r.x, r.y));
+    turn(v.y, w.y, make_float2(r.z, r.w));
+    x = pack2<T>(v.x, v.y);
+    y = pack2<T>(w.x, w.y);
+  }
   __device__ __forceinline__ void store(T* dst, int u, int turned, int rotary, bool interleaved, const float2* cs) {
     if (u >= turned) {
-      st16(dst + rotary + (u - turned) * V, a);
+      put(dst + rotary + (u - turned) * V, a);
       return;
     }
-    const float4* r = reinterpret_cast<const float4*>(cs) + u;
+    const float4* r = reinterpret_cast<const float4*>(cs) + u;  // two pairs
+    uint32_t x[NW], y[NW];
+    Words::split(x, a);
     if (interleaved) {
-      if constexpr (V == 8) {
-        turn_pairs(a.x, a.y, r[0]);
-        turn_pairs(a.z, a.w, r[turned]);
+      if constexpr (V == 2) {
+        if constexpr (sizeof(T) == 2) turn_word(x[0], cs[u].x, cs[u].y);
+        else turn_f32(x[0], x[1], cs[u].x, cs[u].y);
       } else {
-        turn_f32(a.x, a.y, r[0].x, r[0].y);
-        turn_f32(a.z, a.w, r[0].z, r[0].w);
+#pragma unroll
+        for (int g = 0; g < V / 4; ++g) {
+          const float4 v = r[g * turned];
+          if constexpr (sizeof(T) == 2) {
+            turn_word(x[2 * g], v.x, v.y);
+            turn_word(x[2 * g + 1], v.z, v.w);
+          } else {
+            turn_f32(x[4 * g], x[4 * g + 1], v.x, v.y);
+            turn_f32(x[4 * g + 2], x[4 * g + 3], v.z, v.w);
+          }
+        }
       }
-      st16(dst + u * V, a);
     } else {
-      if constexpr (V == 8) {
-        turn_halves(a.x, b.x, r[0]);
-        turn_halves(a.y, b.y, r[turned]);
-        turn_halves(a.z, b.z, r[2 * turned]);
-        turn_halves(a.w, b.w, r[3 * turned]);
-      } else {
-        turn_f32(a.x, b.x, r[0].x, r[0].y);
-        turn_f32(a.y, b.y, r[0].z, r[0].w);
-        turn_f32(a.z, b.z, r[turned].x, r[turned].y);
-        turn_f32(a.w, b.w, r[turned].z, r[turned].w);
+      Words::split(y, b);
+#pragma unroll
+      for (int g = 0; g < V / 2; ++g) {
+        const float4 v = r[g * turned];
+        if constexpr (sizeof(T) == 2) {
+          turn_halves(x[g], y[g], v);
+        } else {
+          turn_f32(x[2 * g], y[2 * g], v.x, v.y);
+          turn_f32(x[2 * g + 1], y[2 * g + 1], v.z, v.w);
+        }
       }
-      st16(dst + u * V, a);
-      st16(dst + rotary / 2 + u * V, b);
+      put(dst + rotary / 2 + u * V, Words::join(y));
     }
+    put(dst + u * V, Words::join(x));
   }
 };
+
+// Values to a unit: as many as a word of 16, 8 or 4 bytes holds (or one) that divide the pairs' halves,
+// the head, every stride and every pointer.  `bytes`: of a value.  Single values cost an
+// instruction each: 32768 tokens of 32 heads of 72 (36 pairs, no multiple of the 8
+// values of 16 bytes) turn in 50 us with 8-byte words and took 160 with single values; the append of 16384
+// tokens of 8 + 8 heads of 72 takes 30 instead of 93.
+template <class... P>
+int unit_values(int bytes, int rotary, bool interleaved, int dim, std::initializer_list<long long> strides,
+                P... pointers) {
+  for (int v = 16 / bytes; v > 1; v /= 2) {
+    bool fits = (interleaved ? rotary : rotary / 2) % v == 0 && dim % v == 0 && aligned_to(v * bytes, pointers...);
+    for (long long s : strides) fits = fits && s % v == 0;
+    if (fits) return v;
+  }
+  return 1;
+}
 
 // ---- division by a number known at launch (n < 2^31) ------------------------
 struct FastDiv {
@@ -240,12 +302,6 @@ struct Pages {
     return ((size_t)page * heads + head) * page_size + line;
   }
 };
-
-// Whether every pointer (or none) starts on a multiple of n bytes.
-template <class... P>
-bool aligned_to(size_t n, P... p) {
-  return (((reinterpret_cast<uintptr_t>(p) % n) == 0) && ...);
-}
 
 // Lets a kernel have `bytes` of dynamic shared memory, once for each device (the call
 // costs a microsecond).  `done`: a static of the kernel's own.

@@ -99,7 +99,7 @@ struct __align__(16) TokenRow {
 // occupancy: with v's first batch held over the row search as well, the append of 16384
 // rotated tokens took 44 us instead of 37; without, that of 65536 plain ones 105 instead
 // of 93.
-template <class T, int V, bool ROT>
+template <class T, int V, int VC, bool ROT>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ Pages c,
                                                                 const __grid_constant__ AppendParams p) {
   extern __shared__ __align__(16) char smem[];
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   constexpr int C = ROT ? 2 : 4;
   const int copy_rows = n * c.heads, copy0 = tid / p.row_lanes, copy_step = kAppendThreads / p.row_lanes;
   const int copy_u = tid - copy0 * p.row_lanes;
-  auto copy_load = [&](Unit<T, V>* unit, const T* src, int tt, int hh, int r, int u) {
+  auto copy_load = [&](Unit<T, VC>* unit, const T* src, int tt, int hh, int r, int u) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int row = r + j * copy_step, t = p.by_heads.div(row), h = row - t * c.heads;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         unit[j].load_row(src + (long long)t * tt + (long long)h * hh, u);
     }
   };
-  auto copy_store = [&](const Unit<T, V>* unit, char* pages, int r, int u) {
+  auto copy_store = [&](const Unit<T, VC>* unit, char* pages, int r, int u) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int row = r + j * copy_step, t = p.by_heads.div(row), h = row - t * c.heads;
@@ -201,14 +201,14 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   auto copy_rest = [&](const T* src, int tt, int hh, char* pages, bool all) {
     for (int u = copy_u; u < p.row_units; u += p.row_lanes)
       for (int r = copy0 + (u == copy_u && !all ? C * copy_step : 0); r < copy_rows; r += C * copy_step) {
-        Unit<T, V> unit[C];
+        Unit<T, VC> unit[C];
         copy_load(unit, src, tt, hh, r, u);
         copy_store(unit, pages, r, u);
       }
   };
 
   if constexpr (!ROT) {
-    Unit<T, V> k_first[C], v_first[C];
+    Unit<T, VC> k_first[C], v_first[C];
     copy_load(k_first, k, p.kt, p.kh, copy0, copy_u);
     copy_load(v_first, v, p.vt, p.vh, copy0, copy_u);
     find_rows();
@@ -647,12 +647,12 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) c.counts[b] = left;
 }
 
-template <class T, int V>
+template <class T, int V, int VC, bool ROT>
 int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
-  p.turned = p.rotary > 0 ? rotary_units<V>(p.rotary, p.interleaved) : 0;
+  p.turned = ROT ? rotary_units<V>(p.rotary, p.interleaved) : 0;
   p.units = p.turned + (c.dim - p.rotary) / V;
   p.lanes = std::min(p.units, kAppendThreads);
-  p.row_units = c.dim / V;
+  p.row_units = c.dim / VC;
   p.row_lanes = std::min(p.row_units, kAppendThreads);
   p.by_qk = FastDiv(p.q_heads + c.heads);
   p.by_heads = FastDiv(c.heads);
@@ -660,18 +660,31 @@ int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
   // A few batches of loads for a CTA, but for tokens enough to fill the SMs.
   const int fill = 16 * (kAppendThreads / p.lanes) / (p.q_heads + c.heads);
   p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 40}));  // 40 x (1 KB + 32) of shared memory at most
-  return launch_pdl(p.turned > 0 ? append_kernel<T, V, true> : append_kernel<T, V, false>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kAppendThreads),
+  return launch_pdl(append_kernel<T, V, VC, ROT>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kAppendThreads),
                     p.per_cta * (sizeof(TokenRow) + (size_t)(p.rotary / 2) * sizeof(float2)), stream, pdl_enabled(), c,
                     p);
 }
 
+// The turned rows and the copied ones each take the widest word of their own.
+template <class T, int V>
+int append_rotated(const Pages& c, const AppendParams& p, bool rows, cudaStream_t stream) {
+  return rows ? append_run<T, V, 8, true>(c, p, stream) : append_run<T, V, 1, true>(c, p, stream);
+}
+
 template <class T>
 int append_type(const Pages& c, const AppendParams& p, cudaStream_t stream) {
-  const bool vec = aligned16(p.k) && aligned16(p.v) && p.kt % 8 == 0 && p.kh % 8 == 0 && p.vt % 8 == 0 &&
-                   p.vh % 8 == 0 &&
-                   (p.q == nullptr || (aligned16(p.q) && aligned16(p.q_out) && p.qt % 8 == 0 && p.qh % 8 == 0)) &&
-                   p.rotary % (p.interleaved ? 8 : 16) == 0;
-  return vec ? append_run<T, 8>(c, p, stream) : append_run<T, 1>(c, p, stream);
+  if (p.rotary == 0) {
+    const bool rows = unit_values(2, 0, false, c.dim, {p.vt, p.vh, p.kt, p.kh}, p.v, p.k) == 8;
+    return rows ? append_run<T, 8, 8, false>(c, p, stream) : append_run<T, 1, 1, false>(c, p, stream);
+  }
+  const bool rows = unit_values(2, 0, false, c.dim, {p.vt, p.vh}, p.v) == 8;
+  const long long qt = p.q != nullptr ? p.qt : 0, qh = p.q != nullptr ? p.qh : 0;
+  switch (unit_values(2, p.rotary, p.interleaved, c.dim, {p.kt, p.kh, qt, qh}, p.k, p.q, p.q_out)) {
+    case 8: return append_rotated<T, 8>(c, p, rows, stream);
+    case 4: return append_rotated<T, 4>(c, p, rows, stream);
+    case 2: return append_rotated<T, 2>(c, p, rows, stream);
+    default: return append_rotated<T, 1>(c, p, rows, stream);
+  }
 }
 
 }  // namespace

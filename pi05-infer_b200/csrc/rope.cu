@@ -6,7 +6,7 @@
 // first values, works out the tokens' cos and sin into shared memory while they are on
 // their way (once for all heads), then streams.  A thread keeps its place within a head
 // and goes from head to head; values that pass through go by themselves, so that no warp
-// does both.  32768 tokens of 32 heads of 128, half of each rotated (537 MB): 87 us;
+// does both.  32768 tokens of 32 heads of 128, half of each rotated (537 MB): 86 us;
 // with a word's place worked out for every word 99 (integer arithmetic in 76% of the issue
 // slots), with turned and passed words in the same warps 90.
 #include <algorithm>
@@ -97,8 +97,11 @@ int rope_run(const void* x, void* out, RopeParams p, cudaStream_t stream) {
   p.passed_lanes = std::min(p.passed, kThreads);
   p.by_heads = FastDiv(p.heads);
   p.by_pairs = FastDiv(p.rotary / 2);
-  // A few batches of loads for a CTA, but for tokens enough to fill the SMs.
-  const int fill = std::max(1, 4 * J * (kThreads / p.turned_lanes) / p.heads);
+  // A few batches of loads for a CTA, but for tokens enough to fill the SMs.  The longer of
+  // the two passes counts: with many tokens to a CTA, L2 has lost the sectors and lines that
+  // both touch before the second comes (32768 tokens of 32 heads of 80, 40 of them turned: 80
+  // us; by the turned part alone 137).
+  const int fill = std::max(1, 4 * J * (kThreads / std::max(p.turned_lanes, p.passed_lanes)) / p.heads);
   p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 48 * 1024 / (p.rotary / 2 * (int)sizeof(float2))}));
   return launch_pdl(rope_kernel<T, V, J>, dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kThreads),
                     (size_t)p.per_cta * (p.rotary / 2) * sizeof(float2), stream, pdl_enabled(),
@@ -107,11 +110,13 @@ int rope_run(const void* x, void* out, RopeParams p, cudaStream_t stream) {
 
 template <class T>
 int rope_type(const void* x, void* out, const RopeParams& p, cudaStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  // 16-byte chunks need every row, and the partner half of a row, on a 16-byte boundary.
-  const bool vec = aligned16(x) && aligned16(out) && p.xt % V == 0 && p.xh % V == 0 && p.ot % V == 0 && p.oh % V == 0 &&
-                   p.dim % V == 0 && p.rotary % (p.interleaved ? V : 2 * V) == 0;
-  return vec ? rope_run<T, V>(x, out, p, stream) : rope_run<T, 1>(x, out, p, stream);
+  switch (unit_values(sizeof(T), p.rotary, p.interleaved, p.dim, {p.xt, p.xh, p.ot, p.oh}, x, out)) {
+    case 8:
+      if constexpr (sizeof(T) == 2) return rope_run<T, 8>(x, out, p, stream);
+    case 4: return rope_run<T, 4>(x, out, p, stream);
+    case 2: return rope_run<T, 2>(x, out, p, stream);
+    default: return rope_run<T, 1>(x, out, p, stream);
+  }
 }
 
 }  // namespace

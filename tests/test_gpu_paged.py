@@ -76,6 +76,24 @@ def test_rope(dtype, layout, tokens, heads, dim, rotary):
     assert rope(z, pos, f, out=z) is z and torch.equal(z, y)  # in place
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("rotary", [4, 8, 12, 20, 36, 40])
+@pytest.mark.parametrize("skip,dim,room", [(0, 40, 0), (4, 40, 4), (2, 42, 2), (1, 41, 0), (0, 40, 1)])
+def test_rope_words(dtype, layout, rotary, skip, dim, room):
+    """Every word that pairs, strides and the first row's address allow gives the same values."""
+    n, h = 19, 3
+    buf = rnd(n, h * dim + skip + room, dtype=dtype, g=gen(rotary))
+    x = buf[:, skip : skip + h * dim].unflatten(1, (h, dim))
+    pos = torch.arange(n, device="cuda", dtype=torch.int32) * 31 - 100
+    f = RopeFrequencies(rotary, layout=layout)
+    out = torch.full_like(buf, 7.0)
+    y = rope(x, pos, f, out=out[:, skip : skip + h * dim].unflatten(1, (h, dim)))
+    check_rope(y, x, pos, rotary, layout)
+    assert (out[:, :skip] == 7).all() and (out[:, skip + h * dim :] == 7).all()
+    assert torch.equal(rope(x.contiguous(), pos, f), y)
+
+
 @pytest.mark.parametrize("kw", [
     dict(scaling="linear", factor=4.0), dict(scaling="ntk", factor=8.0, base=500000.0),
     dict(scaling="yarn", factor=16.0, original_len=8192),
@@ -257,6 +275,30 @@ def test_append(dtype, batch, heads, kv_heads, dim, page, rotary, layout, pages)
         same_rows(c, t, k_tol=small + u(dtype) * (np.abs(t.k) + small) + 2.0**-25)
         t.k = np64(c.k_pages).copy()
     assert c.read_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("rotary", [0, 2, 4, 8, 12, 20, 40])
+@pytest.mark.parametrize("k_skip,v_skip", [(0, 0), (4, 0), (2, 1), (1, 0), (0, 1)])
+def test_append_words(layout, rotary, k_skip, v_skip):
+    """Every word that pairs, strides and the first row's address allow, for the turned and the copied rows."""
+    g, h, d, n = gen(rotary), 3, 40, 13
+    c, t = make(1, h, d, 5, 4)
+    wide = [rnd(n, h * d + 8, g=g) for _ in range(2)]
+    k, v = (w[:, s : s + h * d].unflatten(1, (h, d)) for w, s in zip(wide, (k_skip, v_skip)))
+    if rotary == 0:
+        c.append(k, v, cu_tokens=torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+        t.append(np64(k), np64(v), np.array([0, n]))
+        same_rows(c, t)
+        return
+    q = rnd(n, 2 * d * h + 8, g=g)[:, k_skip : k_skip + 2 * d * h].unflatten(1, (2 * h, d))
+    f = RopeFrequencies(rotary, layout=layout)
+    out = c.append(k, v, q=q, freqs=f, cu_tokens=torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    check_rope(out, q, torch.arange(n), rotary, layout)
+    k_ref, size = rotate(np64(k), np.arange(n), rotary, layout)
+    t.append(k_ref, np64(v), np.array([0, n]))
+    small = 8 * F * size.max()
+    same_rows(c, t, k_tol=small + u(BF) * (np.abs(t.k) + small) + 2.0**-25)
 
 
 def test_append_without_rotation_or_weights():
