@@ -18,9 +18,8 @@
 // products run on the tensor cores with the rows as M:  S^T = K q^T (16 rows x 8 heads),
 // then O^T += V^T P^T, where the probabilities pass from one fragment layout to the other
 // by a matrix transpose in registers; with the heads as N = 8, half as many products and
-// accumulators as with 16 padded query rows.  The probabilities enter the second product
-// in the cache's 16-bit type (2^-8 relative at most for bf16, as the output's own
-// rounding); m, l and o stay fp32, l sums the unrounded ones.
+// accumulators as with 16 padded query rows.  The probabilities enter the second product as
+// a sum of two numbers of the cache's 16-bit type (see halves()); m, l and o stay fp32.
 //
 // Measured: 2 x 131072 rows, 32 / 8 heads of 128: 157 us = 6.8 TB/s + 5 us for the join.
 // The same with 16-byte cp.async copies through registers' addresses: 190 us (430
@@ -74,6 +73,30 @@ __device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, co
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// A probability x <= 1 as hi + lo for the matrix unit, which takes 16-bit numbers: one alone
+// would be off by as much as the output's own rounding (2^-9 of it in bf16), and in fp16 lose
+// what lies below 2^-25.  hi has x's leading bits (8 in bf16, 11 in fp16) and lo rounds the rest,
+// to 2^-16 of x in bf16 and 2^-21 in fp16, where both hold 2^15 x, so that nothing above 2^-39
+// of the largest is lost either.  hi lies below x, so that lo is not 0: hi * inf + 0 * inf would be
+// NaN where x * inf is infinite.
+template <class T>
+struct Prob;
+template <>
+struct Prob<__nv_bfloat16> {
+  static constexpr float kOne = 1.f;
+  static constexpr uint32_t kLeading = 0xffff0000u;
+};
+template <>
+struct Prob<__half> {
+  static constexpr float kOne = 0x1p15f;
+  static constexpr uint32_t kLeading = 0xffffe000u;
+};
+template <class T>
+__device__ __forceinline__ float2 halves(float x) {
+  const float v = x * Prob<T>::kOne, hi = __uint_as_float((max(__float_as_uint(v), 1u) - 1) & Prob<T>::kLeading);
+  return make_float2(hi, v - hi);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
@@ -462,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
 #pragma unroll
       for (int ks = 0; ks < B; ++ks)
         load_v(va[ks], ks);
-      uint32_t pf[NT][2];
+      uint32_t pf[NT][2], pl[NT][2];  // the probabilities' hi and lo
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float* xs = x[nt];
@@ -496,8 +519,12 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
             }
           }
         }
-        pf[nt][0] = transpose8x8(pack2<T>(xs[0], xs[1]));
-        pf[nt][1] = transpose8x8(pack2<T>(xs[2], xs[3]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 a = halves<T>(xs[2 * i]), b = halves<T>(xs[2 * i + 1]);
+          pf[nt][i] = transpose8x8(pack2<T>(a.x, b.x));
+          pl[nt][i] = transpose8x8(pack2<T>(a.y, b.y));
+        }
       }
 #pragma unroll
       for (int k0 = 0; k0 < KS; k0 += B) {
@@ -510,7 +537,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         for (int ks = 0; ks < B; ++ks)
           if (k0 + ks < KS) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[k0 + ks][nt], va[ks], pf[nt]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<T>(o[k0 + ks][nt], va[ks], pl[nt]);
+              mma16816<T>(o[k0 + ks][nt], va[ks], pf[nt]);
+            }
           }
       }
     }
@@ -581,7 +611,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
           if (h >= heads) continue;
           const float sum = l[nt][i];
           // A sum of 0 has no row that counts; NaN stays NaN.
-          const float lse2 = sum == 0.f ? -INFINITY : m[nt][i] + log2f(sum), scale = sum == 0.f ? 0.f : 1.f / sum;
+          const float lse2 = sum == 0.f ? -INFINITY : m[nt][i] + log2f(sum);
+          const float scale = sum == 0.f ? 0.f : 1.f / (sum * Prob<T>::kOne);
           T* out = static_cast<T*>(p.out) + ((size_t)s.b * p.q_heads + head0 + h) * d;
           float* part = p.part_o + ((size_t)slot * H + h) * d;
 #pragma unroll
@@ -592,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
               if (x >= d) continue;
               const float v = o[ks][nt][i + 2 * k];
               if (s.whole) out[x] = from_f32<T>(sum == 0.f ? 0.f : v * scale);
-              else part[x] = v;
+              else part[x] = v * (1.f / Prob<T>::kOne);
             }
           if (lane < 4) {
             if (!s.whole) {
@@ -641,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         scale[r] = ex2_approx(m[r] - base);
         sum += l[r] * scale[r];
       }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a sum of 0 has no row that counts; NaN stays NaN
+      const float inv = sum == 0.f ? 0.f : 1.f / (sum * Prob<T>::kOne);  // a sum of 0 has no row that counts; NaN stays NaN
 #pragma unroll
       for (int r = 0; r < 8; ++r) scale[r] *= inv;
       return sum == 0.f ? -INFINITY : top + log2f(sum);

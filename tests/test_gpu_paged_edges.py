@@ -1,0 +1,86 @@
+"""GPU tests of the text-decoding operators at their edges: precision, values that are not finite, overlapping
+views, forward-mode derivatives, tables far longer than their sequences.  Model, tolerances and helpers as in
+``test_gpu_paged.py``."""
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_paged import BF, F, HF, check_attend, gen, make, np64, rnd, twin, u
+
+from pi05_infer import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# attention: the probabilities' bits
+# ---------------------------------------------------------------------------
+
+# batch, heads, kv_heads, dim, rows: a cluster for each pair, then equal shares; up to 8 query heads, then more
+BITS = [(2, 8, 1, 256, 900), (3, 8, 2, 80, 500), (2, 12, 1, 128, 700), (2, 8, 2, 128, 20000), (2, 16, 1, 256, 9000),
+        (4, 3, 1, 64, 9000)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,rows", BITS)
+def test_attend_adds_no_rounding_of_16_bits(dtype, batch, heads, kv_heads, dim, rows):
+    """The output is the sum of exact products within fp32's errors and a probability's two 16-bit parts (2^-16 of
+    it in bf16, 2^-21 in fp16 and 2^-39 of the largest), rounded once: the last term alone is of the type's size."""
+    c, t = make(batch, kv_heads, dim, 64, rows, dtype=dtype)
+    t.counts[0] = rows
+    c.counts[0] = rows
+    q = rnd(batch, heads, dim, dtype=dtype, g=gen(3), scale=2.0)
+    out = np64(c.attend(q))
+    ref, _, size, reach = t.attend(np64(q), dim**-0.5)
+    p = 2 * ((2 * dim + 4) * F * reach) + 16 * F
+    parts = 2.0**-16 if dtype == BF else 2.0**-21
+    # sums of `rows` products in fp32, in the matrix unit's order: 2 rows 2^-24 at most, and it is far from it
+    near = (parts + p)[..., None] * size + 2 * rows * F * size
+    if dtype == HF:
+        near = near + rows * 2.0**-39 * np.abs(t.v).max() + 2.0**-25
+    assert (np.abs(out - ref) <= u(dtype) * (np.abs(ref) + near) + near).all()
+    # and so most outputs are the correctly rounded ones
+    assert (torch.tensor(ref).to(dtype).double().numpy() == out).mean() > 0.95
+
+
+@pytest.mark.parametrize("rows,batch", [(1000, 200), (4000, 120)])  # one CTA a pair; equal shares
+def test_attend_long_flat_tail(rows, batch):
+    """fp16: rows of 2^-25.5 of the largest probability each, which hold all of the values, count."""
+    c, t = make(batch, 1, 64, 16, rows, dtype=HF)
+    c.k_pages.zero_()
+    c.v_pages.fill_(1000.0)
+    c.k_pages[..., 0] = -25.5 * np.log(2)
+    for b in range(batch):  # the largest in every warp's first tile
+        for r in (0, 16, 32, 48):
+            p, line = t.at(b, r)
+            c.k_pages[p, 0, line, 0] = 0.0
+            c.v_pages[p, 0, line] = 0.0
+    c.counts[0] = rows
+    t = twin(c)
+    q = torch.zeros(batch, 2, 64, dtype=HF, device="cuda")
+    q[..., 0] = 1.0
+    ref, _, size, reach = t.attend(np64(q), 1.0)
+    assert ref.min() > 5e-3
+    near = (2.0**-21 + 2 * (132 * F * reach) + 16 * F + 2 * rows * F)[..., None] * size + rows * 2.0**-39 * 1000
+    assert (np.abs(np64(c.attend(q, scale=1.0)) - ref) <= u(HF) * (ref + near) + near + 2.0**-25).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows", [200, 20000])
+def test_attend_infinite_values(dtype, rows):
+    """An infinite value of any probability gives that infinity, as a product of whole probabilities does."""
+    c, t = make(1, 1, 64, 16, rows, dtype=dtype)
+    c.k_pages.zero_()
+    weights = [0.0, -1.0, -3.3, -12.0]  # scores of the rows with infinities; 0 for all others
+    for i, s in enumerate(weights):
+        p, line = t.at(0, 17 * i + 5)
+        c.k_pages[p, 0, line, 0] = s
+        c.v_pages[p, 0, line, i] = float("inf")
+        c.v_pages[p, 0, line, i + 8] = -float("inf")
+    c.counts[0] = rows
+    q = torch.zeros(1, 3, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    out = c.attend(q, scale=1.0)
+    assert (out[..., :4] == float("inf")).all() and (out[..., 8:12] == -float("inf")).all()
+    assert torch.isfinite(out[..., 12:]).all() and torch.isfinite(out[..., 4:8]).all()
