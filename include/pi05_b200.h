@@ -514,7 +514,7 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* args, 
  * of key-value head h / (n_q_heads / n_kv_heads), in the cache's type; statistics and
  * sums in fp32.  key_valid [batch, valid_rows] bytes with a row pitch (0 = masked row), or
  * NULL; rows from valid_rows on count.  What a masked row holds is not read.  A sequence with no row left gives
- * out = 0, lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.  `track`
+ * out = 0, lse = -inf; rows that count but all score -inf give out = NaN (0 / 0), lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.  `track`
  * adds each row's probability, summed over the query heads of its key-value head, to
  * the cache's `weight`.  q with strides, out dense [batch, n_q_heads, head_dim].
  * `scratch`: pi05_paged_attention_scratch_bytes() bytes (0 for a few short sequences),

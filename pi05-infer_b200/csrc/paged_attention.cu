@@ -38,6 +38,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kWarpRows = 16;
 constexpr int kBlockRows = kWarps * kWarpRows;
 constexpr float kLn2 = 0.69314718055994530942f;
+// The running maximum is -inf while no row has counted and at least this from then on, so that
+// rows whose scores are all -inf (0 / 0, NaN) are told from no rows (0) at the end.  A row that
+// counts leaves this score for -inf, and a masked one -inf, to the tracking.
+constexpr float kLowest = -3.402823466e38f;
 
 struct AttnParams {
   Pages c;
@@ -241,6 +245,13 @@ __device__ __forceinline__ uint32_t fetch(const AttnParams& p, const CUtensorMap
     }
   }
   return mask;
+}
+
+// What a row adds to its weight, by its score and the logarithm of its head's sum (log2 units);
+// a sum of 0 gives NaN to the rows that count.
+__device__ __forceinline__ float track_lse(float lse2) { return lse2 == -INFINITY ? NAN : lse2; }
+__device__ __forceinline__ float probability(float score, float lse2) {
+  return score == -INFINITY ? 0.f : ex2_approx(score - lse2);
 }
 
 __device__ __forceinline__ float ld_peer(const float* x, int rank, int ctas) {
@@ -495,16 +506,19 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
           const int h = nt * 8 + 2 * (lane & 3), r0 = ((s.tile0 + j) * kWarps + w) * kWarpRows + (lane >> 2);
           float* dst = SHORT ? my_scores + (r0 - s.tile0 * kBlockRows) * p.score_pitch + h
                              : p.scores + ((size_t)s.row * p.c.capacity + r0) * p.score_pitch + h;
-          if (r0 < s.len && h < heads) *reinterpret_cast<float2*>(dst) = make_float2(xs[0], xs[1]);
+          auto score = [](bool counts, float x) { return counts && x == -INFINITY ? kLowest : x; };
+          if (r0 < s.len && h < heads)
+            *reinterpret_cast<float2*>(dst) = make_float2(score(live0, xs[0]), score(live0, xs[1]));
           if (r0 + 8 < s.len && h < heads)
-            *reinterpret_cast<float2*>(dst + 8 * (size_t)p.score_pitch) = make_float2(xs[2], xs[3]);
+            *reinterpret_cast<float2*>(dst + 8 * (size_t)p.score_pitch) =
+                make_float2(score(live1, xs[2]), score(live1, xs[3]));
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float top = fmaxf(xs[i], xs[i + 2]);
 #pragma unroll
           for (int sft = 4; sft < 32; sft <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, sft));
-          top = fmaxf(top, m[nt][i]);
+          top = fmaxf(top, fmaxf(m[nt][i], rows != 0 ? kLowest : -INFINITY));
           const float base = top == -INFINITY ? 0.f : top;
           const float keep = ex2_approx(m[nt][i] - base);
           m[nt][i] = top;
@@ -610,9 +624,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
           const int h = nt * 8 + 2 * (lane & 3) + i;
           if (h >= heads) continue;
           const float sum = l[nt][i];
-          // A sum of 0 has no row that counts; NaN stays NaN.
-          const float lse2 = sum == 0.f ? -INFINITY : m[nt][i] + log2f(sum);
-          const float scale = sum == 0.f ? 0.f : 1.f / (sum * Prob<T>::kOne);
+          const bool none = m[nt][i] == -INFINITY;
+          const float lse2 = m[nt][i] + log2f(sum), scale = 1.f / (sum * Prob<T>::kOne);
           T* out = static_cast<T*>(p.out) + ((size_t)s.b * p.q_heads + head0 + h) * d;
           float* part = p.part_o + ((size_t)slot * H + h) * d;
 #pragma unroll
@@ -622,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
               const int x = ks * 16 + k * 8 + (lane >> 2);
               if (x >= d) continue;
               const float v = o[ks][nt][i + 2 * k];
-              if (s.whole) out[x] = from_f32<T>(sum == 0.f ? 0.f : v * scale);
+              if (s.whole) out[x] = from_f32<T>(none ? 0.f : v * scale);
               else part[x] = v * (1.f / Prob<T>::kOne);
             }
           if (lane < 4) {
@@ -630,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
               p.part_ml[(size_t)slot * H + h] = make_float2(m[nt][i], sum);
             } else {
               if (p.lse != nullptr) p.lse[(size_t)s.b * p.q_heads + head0 + h] = lse2 * kLn2;
-              if (p.track) p.row_lse[(size_t)s.row * H + h] = lse2;
+              if (p.track) p.row_lse[(size_t)s.row * H + h] = track_lse(lse2);
             }
           }
         }
@@ -672,10 +685,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         scale[r] = ex2_approx(m[r] - base);
         sum += l[r] * scale[r];
       }
-      const float inv = sum == 0.f ? 0.f : 1.f / (sum * Prob<T>::kOne);  // a sum of 0 has no row that counts; NaN stays NaN
+      const float inv = top == -INFINITY ? 0.f : 1.f / (sum * Prob<T>::kOne);
 #pragma unroll
       for (int r = 0; r < 8; ++r) scale[r] *= inv;
-      return sum == 0.f ? -INFINITY : top + log2f(sum);
+      return top + log2f(sum);
     };
     float scale[8];
     for (int e = rank * kThreads + tid; e < KS * NT * 4 * 32; e += ctas * kThreads) {
@@ -696,8 +709,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     }
     if (p.track) {
       if (tid < heads) {
-        const float lse2 = total_of(tid >> 3, tid & 1, (tid & 7) >> 1, scale);
-        sh_lse[tid] = lse2 == -INFINITY ? 0.f : lse2;  // no row: every score is -inf, and stays so
+        sh_lse[tid] = track_lse(total_of(tid >> 3, tid & 1, (tid & 7) >> 1, scale));
       }
       __syncthreads();
       const int r_first = fs.tile0 * kBlockRows, r_end = min(fs.len, r_first + fs.n * kBlockRows);
@@ -706,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         const int page = p.c.page_of(fs.b, r, &line);
         const float* sc = my_scores + (r - r_first) * p.score_pitch;
         float add = 0.f;
-        for (int h = 0; h < heads; ++h) add += ex2_approx(sc[h] - sh_lse[h]);
+        for (int h = 0; h < heads; ++h) add += probability(sc[h], sh_lse[h]);
         if (p.c.real(page)) p.c.weight[p.c.slot_at(page, fs.kvh, line)] += add;
       }
     }
@@ -723,7 +735,7 @@ constexpr int kFinishThreads = 128;
 
 struct Total {
   float top, sum;  // log2 units
-  __device__ __forceinline__ float lse2() const { return sum == 0.f ? -INFINITY : top + log2f(sum); }
+  __device__ __forceinline__ float lse2() const { return top + log2f(sum); }
 };
 
 // A row's partials are the first's slot and the even ones after it, up to the last CTA's.
@@ -784,11 +796,11 @@ __global__ void __launch_bounds__(kFinishThreads) paged_join_kernel(const __grid
     const float* v = reinterpret_cast<const float*>(acc_of) + i;
     float x = 0.f;
     for (int j = 0; j < groups; ++j) x += v[j * d];
-    out[i] = from_f32<T>(t.sum == 0.f ? 0.f : x / t.sum);
+    out[i] = from_f32<T>(t.top == -INFINITY ? 0.f : x / t.sum);
   }
   if (threadIdx.x == 0) {
     if (p.lse != nullptr) p.lse[(size_t)b * p.q_heads + head] = t.lse2() * kLn2;
-    if (p.track) p.row_lse[(size_t)row * H + h] = t.lse2();
+    if (p.track) p.row_lse[(size_t)row * H + h] = track_lse(t.lse2());
   }
 }
 
@@ -837,11 +849,9 @@ __global__ void __launch_bounds__(kFinishThreads) paged_track_kernel(const __gri
         }
 #pragma unroll
       for (int h = 0; h < P; ++h) {
-        // A head with no row at all: every score is -inf, and so is what is left of it.
-        const float from_top = lse[h] == -INFINITY ? 0.f : lse[h];
 #pragma unroll
         for (int i = 0; i < R; ++i)
-          if (h < heads) add[i] += ex2_approx(s[i][h] - from_top);
+          if (h < heads) add[i] += probability(s[i][h], lse[h]);
       }
     }
 #pragma unroll

@@ -447,7 +447,7 @@ class PagedKVCache:
         padding mask need not grow with the sequence).  ``track`` adds the probabilities to the
         cache's ``weight`` (its scratch holds a score for every row there can be and query head, so a
         table much longer than its sequences costs memory).  A sequence with no row gives zeros (lse
-        ``-inf``).  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
+        ``-inf``); rows that count but all score ``-inf`` give NaN, as a softmax of them does.  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
         natural-log sums ``[batch, heads]``.
         """
         self._rows(q, "q", None)

@@ -84,3 +84,48 @@ def test_attend_infinite_values(dtype, rows):
     out = c.attend(q, scale=1.0)
     assert (out[..., :4] == float("inf")).all() and (out[..., 8:12] == -float("inf")).all()
     assert torch.isfinite(out[..., 12:]).all() and torch.isfinite(out[..., 4:8]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows", [150, 20000])  # a cluster for each pair; equal shares, joined
+@pytest.mark.parametrize("kv_heads,heads", [(2, 4), (1, 11)])
+def test_attend_scores_that_are_not_finite(dtype, rows, kv_heads, heads):
+    """Rows that count and score -inf, all of them: softmax is 0 / 0, NaN, for the output and their weights, and
+    log 0 for the sum; some of them: nothing.  Masked rows add nothing to their weight whatever the others hold."""
+    g = gen(5)
+    c, t = make(4, kv_heads, 64, 16, rows, dtype=dtype)
+    c.k_pages.copy_(c.k_pages.abs())
+    q = rnd(4, heads, 64, dtype=dtype, g=g).abs() + 0.1
+    valid = torch.rand(4, rows, device="cuda", generator=g) > 0.3
+    valid[1] = False
+    c.counts[0] = rows
+    good, good_lse = c.attend(q, key_valid=valid, return_lse=True)
+    live = valid.cpu().numpy()
+    spoiled = np.zeros((4, rows), dtype=bool)
+    spoiled[0] = spoiled[1] = True       # all; all, but masked
+    spoiled[2] = ~live[2]                # masked rows alone: the result stays
+    bad = np.flatnonzero(live[3])[:1]    # one NaN
+    at = torch.arange(rows, device="cuda")
+    for b in range(4):
+        r = at[torch.tensor(spoiled[b], device="cuda")]
+        c.k_pages[c.page_table[b, r // 16].long(), :, r % 16, 3] = -float("inf")
+    p, line = t.at(3, int(bad[0]))
+    c.k_pages[p, :, line, 0] = float("nan")
+    before = c.weight.clone()
+    out, lse = c.attend(q, key_valid=valid, return_lse=True, track=True)
+    assert torch.isnan(out[0]).all() and (lse[0] == -float("inf")).all()
+    assert (out[1] == 0).all() and (lse[1] == -float("inf")).all()
+    assert torch.equal(out[2], good[2]) and torch.equal(lse[2], good_lse[2])
+    assert torch.isnan(out[3]).all() and torch.isnan(lse[3]).all()
+    for b in range(4):
+        pg, line = c.page_table[b, at // 16].long(), at % 16
+        was, now = before[pg, :, line], c.weight[pg, :, line]
+        assert torch.equal(was[~valid[b]], now[~valid[b]])
+        counted = now[valid[b]]
+        assert torch.isnan(counted).all() if b in (0, 3) else torch.isfinite(counted).all()
+    c.k_pages[p, :, line[int(bad[0])], 0] = 0  # and one row of -inf among others is left out
+    p2, line2 = t.at(3, int(bad[0]))
+    c.k_pages[p2, :, line2, 0], c.k_pages[p2, :, line2, 1] = 0, -float("inf")
+    without = valid.clone()
+    without[3, int(bad[0])] = False
+    assert torch.equal(c.attend(q, key_valid=valid)[3], c.attend(q, key_valid=without)[3])
