@@ -222,6 +222,20 @@ def _rope(x, positions, freqs, out, transpose):
     return out
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """Place for what ``x`` turns into: ``x``'s strides, or dense rows where torch cannot keep them (views that
+    overlap) and would part a head's values."""
+    y = torch.empty_like(x)
+    return y if y.stride(2) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _rows_apart(x: torch.Tensor) -> bool:
+    """Whether the heads of ``x``, contiguous ones, lie apart: tokens before heads in memory, or after."""
+    (tokens, heads, dim), (t, h, _) = x.shape, x.stride()
+    return (heads <= 1 or h >= dim) and (tokens <= 1 or t >= max(heads - 1, 0) * h + dim) or \
+        (tokens <= 1 or t >= dim) and (heads <= 1 or h >= max(tokens - 1, 0) * t + dim)
+
+
 def _leaf_node(x: torch.Tensor):
     """The node that accumulates leaf ``x``'s gradient, marked with the stream it was first seen on.
 
@@ -242,7 +256,7 @@ class _Rope(torch.autograd.Function):
     def forward(ctx, x, positions, freqs, transpose):
         ctx.save_for_backward(positions)
         ctx.freqs, ctx.transpose = freqs, transpose
-        return _rope(x, positions, freqs, torch.empty_like(x), transpose)
+        return _rope(x, positions, freqs, _like(x), transpose)
 
     @staticmethod
     def backward(ctx, g):
@@ -251,7 +265,7 @@ class _Rope(torch.autograd.Function):
         if torch.is_grad_enabled():  # a gradient of the gradient is wanted
             gx = _Rope.apply(g, positions, ctx.freqs, not ctx.transpose)
         else:
-            gx = _rope(g, positions, ctx.freqs, torch.empty_like(g), not ctx.transpose)
+            gx = _rope(g, positions, ctx.freqs, _like(g), not ctx.transpose)
         return gx, None, None, None
 
 
@@ -261,7 +275,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
     to ``positions`` ``[tokens]`` (int32 or int64, any sign).
 
     bf16, fp16 or fp32, fp32 math, one rounding.  Any token and head strides (a q|k|v row's q and k
-    heads in one call, say); values of a head contiguous.  ``out`` may be ``x`` (in place), but not
+    heads in one call, say, or views that overlap); values of a head contiguous.  ``out`` may be ``x`` (in place), but not
     overlap it otherwise.  ``transpose`` turns backwards.  Differentiable in ``x`` when ``out`` is
     not given; a captured call with a leaf ``x`` is refused while a graph of it from another stream
     is alive.
@@ -283,12 +297,14 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
             y = _Rope.apply(x, positions, freqs, bool(transpose))
             del node
             return y
-        out = torch.empty_like(x)
+        out = _like(x)
     elif grad:
         raise ValueError("out= is not differentiable")
     elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index or out.stride(2) != 1 or \
             (out.requires_grad and torch.is_grad_enabled()):
         raise ValueError("out must have x's shape, type and device, contiguous in dim, and need no gradient")
+    elif not _rows_apart(out):
+        raise ValueError("out's heads overlap")
     return _rope(x, positions, freqs, out, bool(transpose))
 
 

@@ -6,9 +6,9 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged import BF, F, HF, check_attend, gen, make, np64, rnd, twin, u
+from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, twin, u
 
-from pi05_infer import PagedKVCache
+from pi05_infer import RopeFrequencies, rope
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,46 @@ def test_attend_scores_that_are_not_finite(dtype, rows, kv_heads, heads):
     without = valid.clone()
     without[3, int(bad[0])] = False
     assert torch.equal(c.attend(q, key_valid=valid)[3], c.attend(q, key_valid=without)[3])
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+
+def overlapping():
+    g = gen(8)
+    return [
+        rnd(6, 66, g=g).unfold(1, 64, 1),                                  # heads one value apart
+        rnd(73, g=g).unfold(0, 64, 1).unsqueeze(1),                        # tokens one value apart
+        rnd(1, 3, 64, g=g).expand(5, 3, 64), rnd(5, 1, 64, g=g).expand(5, 3, 64),
+        rnd(200, g=g).as_strided((4, 5, 64), (16, 8, 1)),
+    ]
+
+
+@pytest.mark.parametrize("case", range(5))
+def test_rope_of_overlapping_views(case):
+    """The same as of a copy, forward and for such a view as the incoming gradient."""
+    x = overlapping()[case]
+    f, pos = RopeFrequencies(64), torch.arange(x.shape[0], device="cuda") * 7
+    want = rope(x.contiguous(), pos, f)
+    check_rope(want, x, pos, 64, "half")
+    assert torch.equal(rope(x, pos, f), want)
+    leaf = x.contiguous().requires_grad_(True)
+    (gx,) = torch.autograd.grad(rope(leaf, pos, f), leaf, x)
+    assert torch.equal(gx, rope(x.contiguous(), pos, f, transpose=True))
+    leaf = x.detach().requires_grad_(True)  # an overlapping leaf
+    (gx,) = torch.autograd.grad(rope(leaf, pos, f), leaf, torch.ones_like(want))
+    assert torch.equal(gx, rope(torch.ones_like(want), pos, f, transpose=True))
+
+
+def test_rope_into_overlapping_views_is_refused():
+    x = rnd(6, 3, 64)
+    f, pos = RopeFrequencies(64), torch.arange(6, device="cuda")
+    for out in (rnd(6, 66).unfold(1, 64, 1), rnd(1, 3, 64).expand(6, 3, 64), rnd(6, 1, 64).expand(6, 3, 64),
+                rnd(700).as_strided((6, 3, 64), (64, 64, 1)), rnd(700).as_strided((6, 3, 64), (100, 64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            rope(x, pos, f, out=out)
+    want = rope(x, pos, f)
+    for out in (rnd(3, 6, 70)[:, :, 3:67].transpose(0, 1), rnd(6, 4, 64)[:, 1:], rnd(6, 3, 64)):
+        assert torch.equal(rope(x, pos, f, out=out), want)
