@@ -28,6 +28,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -119,6 +120,11 @@ def _run(name: str, index: int, *args) -> None:
             rc = _fn(name)(*args, _raw_stream(index))
     if rc != _lib.PI05_OK:
         raise _lib.Pi05Error(name, rc, _lib.last_error())
+
+
+def _dual(t: torch.Tensor) -> bool:
+    """Whether ``t`` carries a forward-mode tangent (which ``requires_grad`` does not tell)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def _strides(t: torch.Tensor):
@@ -255,6 +261,7 @@ class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, freqs, transpose):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.freqs, ctx.transpose = freqs, transpose
         return _rope(x, positions, freqs, _like(x), transpose)
 
@@ -268,6 +275,12 @@ class _Rope(torch.autograd.Function):
             gx = _rope(g, positions, ctx.freqs, _like(g), not ctx.transpose)
         return gx, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        (positions,) = ctx.saved_tensors
+        tangent = tangent if tangent.stride(-1) == 1 else tangent.contiguous()
+        return _Rope.apply(tangent, positions, ctx.freqs, ctx.transpose)
+
 
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, transpose: bool = False,
          out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -276,8 +289,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
 
     bf16, fp16 or fp32, fp32 math, one rounding.  Any token and head strides (a q|k|v row's q and k
     heads in one call, say, or views that overlap); values of a head contiguous.  ``out`` may be ``x`` (in place), but not
-    overlap it otherwise.  ``transpose`` turns backwards.  Differentiable in ``x`` when ``out`` is
-    not given; a captured call with a leaf ``x`` is refused while a graph of it from another stream
+    overlap it otherwise.  ``transpose`` turns backwards.  Differentiable in ``x``, in reverse and
+    forward mode, when ``out`` is not given; a captured call with a leaf ``x`` is refused while a graph of it from another stream
     is alive.
     """
     if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda or x.stride(2) != 1:
@@ -290,10 +303,11 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
         raise ValueError(f"the frequencies are on {freqs.device}, x is on {x.device}")
     if freqs.rotary_dim > x.shape[2]:
         raise ValueError(f"rotary_dim {freqs.rotary_dim} is more than the head's {x.shape[2]} values")
-    grad = x.requires_grad and torch.is_grad_enabled()
+    needs_grad = x.requires_grad and torch.is_grad_enabled()
+    grad = needs_grad or _dual(x)
     if out is None:
         if grad:
-            node = _leaf_node(x) if x.is_leaf else None  # alive until the new graph holds it
+            node = _leaf_node(x) if needs_grad and x.is_leaf else None  # alive until the new graph holds it
             y = _Rope.apply(x, positions, freqs, bool(transpose))
             del node
             return y
@@ -301,7 +315,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
     elif grad:
         raise ValueError("out= is not differentiable")
     elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index or out.stride(2) != 1 or \
-            (out.requires_grad and torch.is_grad_enabled()):
+            (out.requires_grad and torch.is_grad_enabled()) or _dual(out):
         raise ValueError("out must have x's shape, type and device, contiguous in dim, and need no gradient")
     elif not _rows_apart(out):
         raise ValueError("out's heads overlap")
@@ -394,7 +408,7 @@ class PagedKVCache:
                 t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
-        if t.requires_grad and torch.is_grad_enabled():
+        if (t.requires_grad and torch.is_grad_enabled()) or _dual(t):
             raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,

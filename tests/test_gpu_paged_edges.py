@@ -5,6 +5,7 @@ views, forward-mode derivatives, tables far longer than their sequences.  Model,
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, twin, u
 
@@ -172,3 +173,37 @@ def test_rope_into_overlapping_views_is_refused():
     want = rope(x, pos, f)
     for out in (rnd(3, 6, 70)[:, :, 3:67].transpose(0, 1), rnd(6, 4, 64)[:, 1:], rnd(6, 3, 64)):
         assert torch.equal(rope(x, pos, f, out=out), want)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_rope_forward_mode(layout, reverse):
+    """The tangent turns as the values do (the map is linear), whether or not a gradient is wanted as well."""
+    f, pos = RopeFrequencies(20, layout=layout), torch.arange(7, device="cuda") * 11
+    x, d = rnd(7, 3, 24, g=gen(1)).requires_grad_(reverse), rnd(7, 24, 3, g=gen(2)).transpose(1, 2)
+    want, turned = rope(x.detach(), pos, f), rope(d.contiguous(), pos, f)
+    with forward_ad.dual_level():
+        y = rope(forward_ad.make_dual(x, d), pos, f)
+        value, tangent = forward_ad.unpack_dual(y)
+        assert torch.equal(value, want) and torch.equal(tangent, turned)
+        if reverse:
+            w = torch.ones_like(want)
+            assert torch.equal(torch.autograd.grad(value, x, w)[0], rope(w, pos, f, transpose=True))
+    with torch.no_grad(), forward_ad.dual_level():
+        assert torch.equal(forward_ad.unpack_dual(rope(forward_ad.make_dual(x, d), pos, f, transpose=True)).tangent,
+                           rope(d.contiguous(), pos, f, transpose=True))
+
+
+def test_forward_mode_is_refused_where_it_would_be_lost():
+    c, _ = make(2, 1, 64, 16, 32)
+    f, pos, x, t = RopeFrequencies(64), torch.arange(2, device="cuda"), rnd(2, 1, 64), rnd(2, 1, 64)
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(x.clone(), t)
+        for call in (lambda: c.append(g, x), lambda: c.append(x, g), lambda: c.append(x, x, q=g, freqs=f),
+                     lambda: c.attend(g), lambda: rope(g, pos, f, out=x), lambda: rope(x, pos, f, out=g)):
+            with pytest.raises(ValueError, match="gradient|differentiable"):
+                call()
+        c.append(x, x, q=x, freqs=f)  # within a level, but without tangents
+        c.attend(x)
+        rope(x, pos, f, out=x)
+    assert c.lens.tolist() == [1, 1] and c.read_status() == 0
