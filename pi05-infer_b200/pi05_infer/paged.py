@@ -17,7 +17,8 @@ lengths, long contexts -- keeps its keys and values in pages::
 Rotary embedding: the reference's ``modeling_gemma.py:151-216`` (half layout, no
 scaling); the cache has no counterpart there.  Calls run on the current stream of the
 tensors' device and never synchronise; calls on one cache are to be ordered on one
-stream (or by events).  Everything can be captured in a CUDA graph.
+stream (or by events).  Everything can be captured in a CUDA graph; ``torch.jit.trace`` and
+``make_fx``, which see none of these calls, are refused.
 """
 
 from __future__ import annotations
@@ -29,6 +30,7 @@ from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -111,8 +113,22 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+# Whether torch records operators: what there is to ask in 0.2 us, where get_proxy_mode() and
+# torch.jit.is_tracing() take 0.5.
+_is_tracing = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None) or (lambda: 1)
+_early_modes = (torch._ops.mode_stack_state_for_pre_dispatch().count
+                if hasattr(torch._ops, "mode_stack_state_for_pre_dispatch") else (lambda: 1))
+
+
 def _run(name: str, index: int, *args) -> None:
-    """Calls the library on the current stream of device ``index``, whichever device is current."""
+    """Calls the library on the current stream of device ``index``, whichever device is current.
+
+    Refused where torch records the operators that run (``torch.jit.trace``, ``make_fx``): a call of the
+    library leaves nothing in such a record, whose replay would return memory that nobody wrote.
+    """
+    if _is_tracing() or (_modes() or _early_modes()) and get_proxy_mode() is not None:
+        raise ValueError(f"{name} cannot be recorded by torch.jit.trace or make_fx (a CUDA graph can hold it)")
     if index == _raw_device():
         rc = _fn(name)(*args, _raw_stream(index))
     else:
@@ -122,9 +138,11 @@ def _run(name: str, index: int, *args) -> None:
         raise _lib.Pi05Error(name, rc, _lib.last_error())
 
 
-def _dual(t: torch.Tensor) -> bool:
-    """Whether ``t`` carries a forward-mode tangent (which ``requires_grad`` does not tell)."""
-    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+def _wants_grad(t: torch.Tensor) -> bool:
+    """Whether a derivative of what is made of ``t`` is wanted, in reverse or in forward mode (a tangent, which
+    ``requires_grad`` does not tell)."""
+    return (t.requires_grad and torch.is_grad_enabled()) or \
+        (forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)
 
 
 def _strides(t: torch.Tensor):
@@ -219,20 +237,22 @@ class RopeFrequencies:
 
 
 def _rope(x, positions, freqs, out, transpose):
+    """``out`` None: with ``x``'s strides, or dense where torch cannot keep them (views that overlap) and would part a
+    head's values."""
     tokens, heads, dim = x.shape
     xt, xh, _ = x.stride()
-    ot, oh, _ = out.stride()
+    if out is None:
+        out = torch.empty_like(x)
+        ot, oh, part = out.stride()
+        if part != 1:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            ot, oh, _ = out.stride()
+    else:
+        ot, oh, _ = out.stride()
     _run("pi05_rope", freqs._index, _ROPE_ARGS.pack(
         x.data_ptr(), out.data_ptr(), positions.data_ptr(), xt, xh, ot, oh, _DTYPES[x.dtype], tokens, heads, dim,
         positions.dtype == torch.int64, transpose), freqs._at)
     return out
-
-
-def _like(x: torch.Tensor) -> torch.Tensor:
-    """Place for what ``x`` turns into: ``x``'s strides, or dense rows where torch cannot keep them (views that
-    overlap) and would part a head's values."""
-    y = torch.empty_like(x)
-    return y if y.stride(2) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _rows_apart(x: torch.Tensor) -> bool:
@@ -263,7 +283,7 @@ class _Rope(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.save_for_forward(positions)
         ctx.freqs, ctx.transpose = freqs, transpose
-        return _rope(x, positions, freqs, _like(x), transpose)
+        return _rope(x, positions, freqs, None, transpose)
 
     @staticmethod
     def backward(ctx, g):
@@ -272,7 +292,7 @@ class _Rope(torch.autograd.Function):
         if torch.is_grad_enabled():  # a gradient of the gradient is wanted
             gx = _Rope.apply(g, positions, ctx.freqs, not ctx.transpose)
         else:
-            gx = _rope(g, positions, ctx.freqs, _like(g), not ctx.transpose)
+            gx = _rope(g, positions, ctx.freqs, None, not ctx.transpose)
         return gx, None, None, None
 
     @staticmethod
@@ -295,27 +315,26 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
     """
     if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda or x.stride(2) != 1:
         raise ValueError("x must be a [tokens, heads, dim] CUDA tensor, bf16, fp16 or fp32, contiguous in dim")
-    index = x.get_device()
-    if positions.shape != x.shape[:1] or positions.dtype not in _POSITIONS or positions.get_device() != index or \
+    index, (tokens, _, dim) = x.get_device(), x.shape
+    if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype not in _POSITIONS or positions.get_device() != index or \
             not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32 or int64 [tokens] on x's device")
     if freqs._index != index:
         raise ValueError(f"the frequencies are on {freqs.device}, x is on {x.device}")
-    if freqs.rotary_dim > x.shape[2]:
-        raise ValueError(f"rotary_dim {freqs.rotary_dim} is more than the head's {x.shape[2]} values")
-    needs_grad = x.requires_grad and torch.is_grad_enabled()
-    grad = needs_grad or _dual(x)
+    if freqs.rotary_dim > dim:
+        raise ValueError(f"rotary_dim {freqs.rotary_dim} is more than the head's {dim} values")
+    grad = _wants_grad(x)
     if out is None:
         if grad:
-            node = _leaf_node(x) if needs_grad and x.is_leaf else None  # alive until the new graph holds it
+            # alive until the new graph holds it
+            node = _leaf_node(x) if x.is_leaf and x.requires_grad and torch.is_grad_enabled() else None
             y = _Rope.apply(x, positions, freqs, bool(transpose))
             del node
             return y
-        out = _like(x)
     elif grad:
         raise ValueError("out= is not differentiable")
     elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index or out.stride(2) != 1 or \
-            (out.requires_grad and torch.is_grad_enabled()) or _dual(out):
+            _wants_grad(out):
         raise ValueError("out must have x's shape, type and device, contiguous in dim, and need no gradient")
     elif not _rows_apart(out):
         raise ValueError("out's heads overlap")
@@ -408,7 +427,7 @@ class PagedKVCache:
                 t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
-        if (t.requires_grad and torch.is_grad_enabled()) or _dual(t):
+        if _wants_grad(t):
             raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,

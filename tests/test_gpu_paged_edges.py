@@ -6,6 +6,8 @@ import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
 from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, twin, u
 
@@ -207,3 +209,38 @@ def test_forward_mode_is_refused_where_it_would_be_lost():
         c.attend(x)
         rope(x, pos, f, out=x)
     assert c.lens.tolist() == [1, 1] and c.read_status() == 0
+
+
+def test_recording_is_refused():
+    """torch.jit.trace and make_fx see no call of the library: what they recorded would return unwritten memory.
+    torch.compile leaves the calls to Python, and modes that only look on change nothing."""
+    f, pos = RopeFrequencies(64), torch.arange(3, device="cuda")
+    c, _ = make(3, 2, 64, 16, 32)
+    x, y = rnd(3, 2, 64, g=gen(1)), rnd(3, 2, 64, g=gen(2))
+
+    def step(k):
+        c.append(k, k)
+        return c.attend(k)
+
+    def evict(k):
+        c.evict(8)
+        return k + 1
+
+    for call in (lambda k: rope(k, pos, f), lambda k: rope(k, pos, f, out=k), step, lambda k: c.attend(k), evict):
+        for record in (lambda: torch.jit.trace(call, (x,), check_trace=False), lambda: make_fx(call)(x),
+                       lambda: make_fx(call, pre_dispatch=True)(x)):
+            with pytest.raises(ValueError, match="cannot be recorded"):
+                record()
+    assert c.lens.tolist() == [0, 0, 0] and c.read_status() == 0
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(ValueError, match="cannot be recorded"):
+        make_fx(lambda k: torch.autograd.grad(rope(k, pos, f), k, y)[0])(leaf)
+    compiled, whole = torch.compile(lambda k: rope(k, pos, f) * 2, backend="eager"), torch.compile(step, backend="eager")
+    for k in (x, y, x):
+        assert torch.equal(compiled(k), rope(k, pos, f) * 2)
+        c.counts.zero_()
+        want = step(k)
+        c.counts.zero_()
+        assert torch.equal(whole(k), want) and c.lens.tolist() == [1, 1, 1]
+    with FlopCounterMode(display=False):
+        assert torch.equal(rope(x, pos, f), rope(x, pos, f))
