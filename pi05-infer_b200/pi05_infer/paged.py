@@ -138,6 +138,15 @@ def _run(name: str, index: int, *args) -> None:
         raise _lib.Pi05Error(name, rc, _lib.last_error())
 
 
+_increment_version = torch.autograd.graph.increment_version
+
+
+def _wrote(tensors) -> None:
+    """Tells torch, which cannot see it, that the library wrote into ``tensors``: a graph that saved one of them is
+    then refused its backward pass instead of reading the new values."""
+    _increment_version(tensors)
+
+
 def _wants_grad(t: torch.Tensor) -> bool:
     """Whether a derivative of what is made of ``t`` is wanted, in reverse or in forward mode (a tangent, which
     ``requires_grad`` does not tell)."""
@@ -338,7 +347,10 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
         raise ValueError("out must have x's shape, type and device, contiguous in dim, and need no gradient")
     elif not _rows_apart(out):
         raise ValueError("out's heads overlap")
-    return _rope(x, positions, freqs, out, bool(transpose))
+    y = _rope(x, positions, freqs, out, bool(transpose))
+    if out is not None:
+        _wrote((out,))
+    return y
 
 
 # ---------------------------------------------------------------------------
@@ -395,6 +407,7 @@ class PagedKVCache:
             _DTYPES[self.dtype], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, self.batch,
             self.pages_per_seq, _strides(page_table)[0], None, 0)
         self._at, self._index = ctypes.addressof(self._c), device.index
+        self._state = tuple(t for t in (k_pages, v_pages, counts, weight, pos) if t is not None)
         nbytes = _fn("pi05_paged_workspace_bytes")(self._at)
         # status word, ticket and the eviction's lists; zeroed once
         self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
@@ -422,13 +435,16 @@ class PagedKVCache:
         """Rows held by each sequence (a view of ``counts``)."""
         return self.counts[0]
 
-    def _rows(self, t: torch.Tensor, name: str, heads: Optional[int]) -> None:
-        if t.dim() != 3 or t.dtype != self.dtype or t.get_device() != self._index or t.shape[2] != self.head_dim or \
-                t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
+    def _rows(self, t: torch.Tensor, name: str, heads: Optional[int]):
+        """Checks rows of heads; their shape and strides."""
+        shape, strides = t.shape, t.stride()
+        if len(shape) != 3 or t.dtype != self.dtype or t.get_device() != self._index or shape[2] != self.head_dim or \
+                strides[2] != 1 or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
         if _wants_grad(t):
             raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
+        return shape, strides
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
                freqs: Optional[RopeFrequencies] = None, cu_tokens: Optional[torch.Tensor] = None,
@@ -443,25 +459,26 @@ class PagedKVCache:
         in ``q_out``).  ``weight`` ``[tokens, n_kv_heads]`` fp32 is what the rows start with (0
         otherwise), e.g. what the prompt's own attention gave them.
         """
-        self._rows(k, "k", self.n_kv_heads)
-        self._rows(v, "v", self.n_kv_heads)
-        tokens = k.shape[0]
-        if v.shape[0] != tokens:
-            raise ValueError(f"k has {tokens} tokens, v has {v.shape[0]}")
+        (tokens, _, _), (k_token, k_head, _) = self._rows(k, "k", self.n_kv_heads)
+        (v_tokens, _, _), (v_token, v_head, _) = self._rows(v, "v", self.n_kv_heads)
+        if v_tokens != tokens:
+            raise ValueError(f"k has {tokens} tokens, v has {v_tokens}")
         q_at = q_out_at = q_token = q_head = n_q_heads = rotary = cu_at = weight_at = 0
+        written = self._state
         if q is not None:
-            self._rows(q, "q", None)
+            (q_tokens, n_q_heads, _), (q_token, q_head, _) = self._rows(q, "q", None)
             if freqs is None:
                 raise ValueError("q is only rotated: give freqs, or leave q out")
-            if q.shape[0] != tokens:
-                raise ValueError(f"k has {tokens} tokens, q has {q.shape[0]}")
+            if q_tokens != tokens:
+                raise ValueError(f"k has {tokens} tokens, q has {q_tokens}")
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.get_device() != self._index or \
                     not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous, of q's shape, type and device")
-            q_at, q_out_at, n_q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-            q_token, q_head, _ = q.stride()
+            else:
+                written += (q_out,)
+            q_at, q_out_at = q.data_ptr(), q_out.data_ptr()
         if freqs is not None:
             if freqs._index != self._index or freqs.rotary_dim > self.head_dim:
                 raise ValueError(f"freqs must be on {self.device} with rotary_dim <= {self.head_dim}")
@@ -479,11 +496,10 @@ class PagedKVCache:
                 raise ValueError(f"weight must be contiguous fp32 [{tokens}, {self.n_kv_heads}] on {self.device}, "
                                  "for a cache that keeps weights")
             weight_at = weight.data_ptr()
-        k_token, k_head, _ = k.stride()
-        v_token, v_head, _ = v.stride()
         _run("pi05_paged_append", self._index, self._at, _APPEND_ARGS.pack(
             k.data_ptr(), v.data_ptr(), k_token, k_head, v_token, v_head, q_at, q_out_at, q_token, q_head, tokens,
             n_q_heads, cu_at, weight_at, rotary))
+        _wrote(written)
         return q_out if q is not None else None
 
     def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, key_valid: Optional[torch.Tensor] = None,
@@ -499,17 +515,19 @@ class PagedKVCache:
         ``-inf``); rows that count but all score ``-inf`` give NaN, as a softmax of them does.  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
         natural-log sums ``[batch, heads]``.
         """
-        self._rows(q, "q", None)
-        batch, heads, dim = q.shape
+        (batch, heads, dim), (q_token, q_head, _) = self._rows(q, "q", None)
         if batch != self.batch or heads == 0 or heads % self.n_kv_heads:
             raise ValueError(f"q must be [{self.batch}, a multiple of {self.n_kv_heads}, {dim}], got {list(q.shape)}")
         if track and self.weight is None:
             raise ValueError("this cache keeps no weights: build it with weight=")
+        written = (self.weight,) if track else ()
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != self._index or \
                 not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape, type and device")
+        else:
+            written += (out,)
         need, like, like_lse = self._scratch.get((heads, track)) or self._need(heads, track)
         lse = torch.empty_like(like_lse, memory_format=torch.contiguous_format) if return_lse else None
         valid_at = pitch = valid_rows = 0
@@ -521,10 +539,11 @@ class PagedKVCache:
             valid_at, pitch, valid_rows = key_valid.data_ptr(), key_valid.stride(0), key_valid.shape[1]
         # from torch's allocator, call by call: calls on different streams, and graphs, never share it
         scratch = torch.empty_like(like, memory_format=torch.contiguous_format) if need else None
-        q_token, q_head, _ = q.stride()
         _run("pi05_paged_attention", self._index, self._at, _ATTEND_ARGS.pack(
             q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), valid_at, q_token, q_head, pitch,
             valid_rows, heads, dim**-0.5 if scale is None else scale, track, scratch.data_ptr() if need else 0, need))
+        if written:
+            _wrote(written)
         return (out, lse) if return_lse else out
 
     def _need(self, heads: int, track: bool):
@@ -548,6 +567,7 @@ class PagedKVCache:
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
             raise ValueError(f"need budget >= 1 and 0 <= recent + sinks <= budget, got {budget}, {recent}, {sinks}")
         _run("pi05_paged_evict", self._index, self._at, budget, recent, sinks)
+        _wrote(self._state)
 
     def read_status(self) -> int:
         """Synchronise, read and clear the cache's device status word (0 = nothing went wrong)."""

@@ -244,3 +244,31 @@ def test_recording_is_refused():
         assert torch.equal(whole(k), want) and c.lens.tolist() == [1, 1, 1]
     with FlopCounterMode(display=False):
         assert torch.equal(rope(x, pos, f), rope(x, pos, f))
+
+
+def test_writes_are_seen_by_autograd():
+    """A tensor that a graph saved and a call then wrote to: the backward pass is refused."""
+    c, _ = make(2, 1, 64, 16, 32)
+    f, pos, x = RopeFrequencies(64), torch.arange(2, device="cuda"), rnd(2, 1, 64)
+    c.append(x, x)
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    state = dict(k=c.k_pages, v=c.v_pages, weight=c.weight)
+    for call, names in ((lambda: c.append(x, x, q=x, freqs=f, q_out=y), ("k", "v", "weight", "y")),
+                        (lambda: c.attend(x, track=True), ("weight",)), (lambda: c.attend(x, out=y), ("y",)),
+                        (lambda: c.evict(1), ("k", "v", "weight")), (lambda: rope(x, pos, f, out=y), ("y",))):
+        for name, t in (*state.items(), ("y", y), ("z", z)):
+            w = torch.ones((), device="cuda", dtype=t.dtype, requires_grad=True)
+            loss = (t * w).sum()
+            before = c.counts._version
+            call()
+            assert (c.counts._version > before) == ("k" in names)
+            if name in names:
+                with pytest.raises(RuntimeError, match="inplace operation"):
+                    loss.backward()
+            else:
+                loss.backward()
+    with torch.inference_mode():
+        out = rnd(2, 1, 64)
+        rope(x, pos, f, out=out)
+        c.append(x, x, q=x, freqs=f, q_out=out)
+    rope(x, pos, f, out=out)  # made in inference mode, without a version
