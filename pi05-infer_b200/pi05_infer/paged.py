@@ -442,9 +442,14 @@ class PagedKVCache:
                 strides[2] != 1 or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] "
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
-        if _wants_grad(t):
-            raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
         return shape, strides
+
+    def _no_gradients(self, **tensors) -> None:
+        """The cache has no derivative: refuses one wanted of an input, or through what is written or read."""
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+            for name, t in (*tensors.items(), ("k_pages", self.k_pages), ("v_pages", self.v_pages)):
+                if t is not None and _wants_grad(t):
+                    raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
                freqs: Optional[RopeFrequencies] = None, cu_tokens: Optional[torch.Tensor] = None,
@@ -461,6 +466,7 @@ class PagedKVCache:
         """
         (tokens, _, _), (k_token, k_head, _) = self._rows(k, "k", self.n_kv_heads)
         (v_tokens, _, _), (v_token, v_head, _) = self._rows(v, "v", self.n_kv_heads)
+        self._no_gradients(k=k, v=v, q=q, q_out=q_out, new_weight=weight, weight=self.weight)
         if v_tokens != tokens:
             raise ValueError(f"k has {tokens} tokens, v has {v_tokens}")
         q_at = q_out_at = q_token = q_head = n_q_heads = rotary = cu_at = weight_at = 0
@@ -516,6 +522,7 @@ class PagedKVCache:
         natural-log sums ``[batch, heads]``.
         """
         (batch, heads, dim), (q_token, q_head, _) = self._rows(q, "q", None)
+        self._no_gradients(q=q, out=out, weight=self.weight if track else None)
         if batch != self.batch or heads == 0 or heads % self.n_kv_heads:
             raise ValueError(f"q must be [{self.batch}, a multiple of {self.n_kv_heads}, {dim}], got {list(q.shape)}")
         if track and self.weight is None:
@@ -566,6 +573,7 @@ class PagedKVCache:
             raise ValueError("this cache keeps no weights and positions: build it with weight= and pos=")
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
             raise ValueError(f"need budget >= 1 and 0 <= recent + sinks <= budget, got {budget}, {recent}, {sinks}")
+        self._no_gradients(weight=self.weight)
         _run("pi05_paged_evict", self._index, self._at, budget, recent, sinks)
         _wrote(self._state)
 

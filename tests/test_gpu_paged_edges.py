@@ -11,7 +11,7 @@ from torch.utils.flop_counter import FlopCounterMode
 
 from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, twin, u
 
-from pi05_infer import RopeFrequencies, rope
+from pi05_infer import PagedKVCache, RopeFrequencies, rope
 
 pytestmark = pytest.mark.gpu
 
@@ -272,3 +272,32 @@ def test_writes_are_seen_by_autograd():
         rope(x, pos, f, out=out)
         c.append(x, x, q=x, freqs=f, q_out=out)
     rope(x, pos, f, out=out)  # made in inference mode, without a version
+
+
+@pytest.mark.parametrize("forward", [False, True])
+def test_gradients_of_what_is_written_are_refused(forward):
+    """Outputs given by the caller, new weights and the cache's own tensors: in reverse and in forward mode."""
+    f, x = RopeFrequencies(64), rnd(2, 1, 64)
+
+    def wanting(t):
+        return forward_ad.make_dual(t.clone(), torch.ones_like(t)) if forward else t.clone().requires_grad_(True)
+
+    with forward_ad.dual_level():
+        c, _ = make(2, 1, 64, 16, 32)
+        o, w = wanting(x), wanting(torch.ones(2, 1, device="cuda"))
+        calls = [lambda: c.append(x, x, q=x, freqs=f, q_out=o), lambda: c.append(x, x, weight=w), lambda: c.attend(x, out=o)]
+        for name in ("k", "v", "weight"):
+            t = dict(k=c.k_pages, v=c.v_pages, weight=c.weight)
+            t[name] = wanting(t[name])
+            d = PagedKVCache(t["k"], t["v"], c.page_table, c.counts, weight=t["weight"], pos=c.pos)
+            calls += [lambda d=d: d.append(x, x), lambda d=d: d.attend(x, track=True), lambda d=d: d.evict(1)]
+        for call in calls:
+            with pytest.raises(ValueError, match="not differentiable"):
+                call()
+        assert c.lens.tolist() == [0, 0]
+        d.attend(x)  # has nothing to do with the weights
+        if not forward:
+            with torch.no_grad():
+                for call in calls:
+                    call()
+    assert c.read_status() == 0
