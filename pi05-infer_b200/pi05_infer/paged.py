@@ -574,6 +574,8 @@ class PagedKVCache:
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
             raise ValueError(f"need budget >= 1 and 0 <= recent + sinks <= budget, got {budget}, {recent}, {sinks}")
         self._no_gradients(weight=self.weight)
+        if budget >= self.pages_per_seq * self.page_size:
+            return  # no sequence can hold more; and below, the numbers fit the library's 32 bits
         _run("pi05_paged_evict", self._index, self._at, budget, recent, sinks)
         _wrote(self._state)
 

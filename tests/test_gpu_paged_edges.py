@@ -9,7 +9,7 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
-from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, twin, u
+from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, same_rows, twin, u
 
 from pi05_infer import PagedKVCache, RopeFrequencies, rope
 
@@ -300,4 +300,16 @@ def test_gradients_of_what_is_written_are_refused(forward):
             with torch.no_grad():
                 for call in calls:
                     call()
+    assert c.read_status() == 0
+
+
+@pytest.mark.parametrize("budget,recent,sinks", [(2**32 + 8, 0, 0), (2**33 + 8, 2**32 + 2, 1), (2**63, 2**62, 2**62),
+                                                 (32, 0, 0), (33, 1, 32)])
+def test_evict_numbers_beyond_32_bits(budget, recent, sinks):
+    """A budget that no sequence can reach leaves everything as it is, however large the number."""
+    c, t = make(2, 1, 64, 16, 32)
+    c.counts.fill_(30)
+    t = twin(c)
+    c.evict(budget, recent=recent, sinks=sinks)
+    same_rows(c, t)
     assert c.read_status() == 0
