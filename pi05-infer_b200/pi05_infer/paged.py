@@ -367,13 +367,21 @@ class PagedKVCache:
     eviction ``weight`` (fp32) and ``pos`` (int32) ``[num_pages, n_kv_heads, page_size]``.  Row ``r``
     of sequence ``b`` is line ``r % page_size`` of page ``page_table[b, r // page_size]``.  The
     tensors stay the caller's: who owns which page, and resetting or truncating a sequence (``counts``),
-    is done by writing to them.
+    is done by writing to them, not by putting others in their place, which is refused.
 
     The table is read on the device.  A page number outside the cache, or a row beyond the table,
     is skipped or masked and sets ``PI05_DEV_BAD_INDEX`` (0x20) in :meth:`read_status`.  A page that a
     call writes (:meth:`append`, :meth:`evict`, :meth:`attend` with ``track``) stands once in the
     table, with one sequence; pages that are only read may be shared.
     """
+
+    _FIXED = frozenset(("k_pages", "v_pages", "page_table", "counts", "weight", "pos", "workspace"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and name in self.__dict__:  # the library has the first one's address
+            raise AttributeError(f"{name} stays the tensor that the cache was built with: write into it, or build "
+                                 "another cache")
+        super().__setattr__(name, value)
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, counts: torch.Tensor, *,
                  weight: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None):
