@@ -417,6 +417,11 @@ class PagedKVCache:
         self._at, self._index = ctypes.addressof(self._c), device.index
         self._state = tuple(t for t in (k_pages, v_pages, counts, weight, pos) if t is not None)
         nbytes = _fn("pi05_paged_workspace_bytes")(self._at)
+        # What else the library asks of a cache (head sizes, alignment, 32-bit ranges), before memory is taken: an
+        # append of no tokens checks it and runs nothing; the workspace is not looked at.
+        self._c.workspace, self._c.workspace_bytes = 256, nbytes
+        if _fn("pi05_paged_append")(self._at, _APPEND_ARGS.pack(*[0] * 12, counts.data_ptr(), 0, 0), None) != _lib.PI05_OK:
+            raise ValueError(f"not a cache that the library takes: {_lib.last_error()}")
         # status word, ticket and the eviction's lists; zeroed once
         self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         self._c.workspace, self._c.workspace_bytes = self.workspace.data_ptr(), nbytes

@@ -313,3 +313,26 @@ def test_evict_numbers_beyond_32_bits(budget, recent, sinks):
     c.evict(budget, recent=recent, sinks=sinks)
     same_rows(c, t)
     assert c.read_status() == 0
+
+
+def test_caches_that_the_library_does_not_take():
+    """Refused when they are made, not by the first call; and before the workspace is allocated."""
+    def build(pages=4, heads=1, page=16, dim=64, batch=2, each=2, skip=0, wide=0, counts=None):
+        k = torch.zeros(pages * heads * page * (dim + wide) + skip, dtype=BF, device="cuda")[skip:]
+        k = k.view(pages, heads, page, dim + wide)[..., :dim]
+        table = torch.zeros(batch, each, dtype=torch.int32, device="cuda")
+        counts = torch.zeros(2 * batch, dtype=torch.int32, device="cuda") if counts is None else counts
+        return PagedKVCache(k, k, table, counts.view(2, batch))
+
+    build()
+    build(skip=8, wide=8)
+    for kw in (dict(dim=60), dict(dim=264), dict(skip=4), dict(wide=4), dict(pages=0), dict(heads=0), dict(page=0),
+               dict(batch=0), dict(each=0)):
+        with pytest.raises(ValueError, match="not a cache that the library takes"):
+            build(**kw)
+    k = torch.zeros(1, 1, 1 << 20, 8, dtype=BF, device="cuda")
+    before = torch.cuda.memory_allocated()
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda").expand(1, 2048).contiguous()
+    with pytest.raises(ValueError, match="bad cache shape"):  # 2^31 rows
+        PagedKVCache(k, k, table, torch.zeros(2, 1, dtype=torch.int32, device="cuda"))
+    assert torch.cuda.memory_allocated() - before < 1 << 20
