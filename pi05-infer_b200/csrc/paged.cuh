@@ -24,6 +24,9 @@ bool aligned_to(size_t n, P... p) {
   return (((reinterpret_cast<uintptr_t>(p) % n) == 0) && ...);
 }
 
+// The stride of a dimension of one element means nothing.
+inline long long stride_of(int elements, long long stride) { return elements == 1 ? 0 : stride; }
+
 // ---- element types ---------------------------------------------------------
 template <class T>
 __device__ __forceinline__ float to_f32(T x);

@@ -1023,9 +1023,8 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
     set_last_error("paged_attention: the cache keeps no weights");
     return PI05_ERR_INVALID_ARG;
   }
-  // The stride of a dimension of one element means nothing.
-  const long long q_token = cache->batch > 1 ? a->q_token_stride : 0;
-  const long long q_head = a->n_q_heads > 1 ? a->q_head_stride : 0;
+  const long long q_token = stride_of(cache->batch, a->q_token_stride);
+  const long long q_head = stride_of(a->n_q_heads, a->q_head_stride);
   if (!aligned_to(4, a->q, a->lse) || !aligned_to(2, a->out) || q_token % 2 || q_head % 2) {
     set_last_error("paged_attention: q rows and lse must start on 4-byte boundaries, out on 2-byte ones");
     return PI05_ERR_ALIGN;

@@ -678,8 +678,7 @@ int append_type(const Pages& c, const AppendParams& p, cudaStream_t stream) {
     return rows ? append_run<T, 8, 8, false>(c, p, stream) : append_run<T, 1, 1, false>(c, p, stream);
   }
   const bool rows = unit_values(2, 0, false, c.dim, {p.vt, p.vh}, p.v) == 8;
-  const long long qt = p.q != nullptr ? p.qt : 0, qh = p.q != nullptr ? p.qh : 0;
-  switch (unit_values(2, p.rotary, p.interleaved, c.dim, {p.kt, p.kh, qt, qh}, p.k, p.q, p.q_out)) {
+  switch (unit_values(2, p.rotary, p.interleaved, c.dim, {p.kt, p.kh, p.qt, p.qh}, p.k, p.q, p.q_out)) {
     case 8: return append_rotated<T, 8>(c, p, rows, stream);
     case 4: return append_rotated<T, 4>(c, p, rows, stream);
     case 2: return append_rotated<T, 2>(c, p, rows, stream);
@@ -734,8 +733,11 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, voi
     set_last_error("paged_append: pointer not aligned to its elements");
     return PI05_ERR_ALIGN;
   }
-  for (long long stride : {a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->q_token_stride,
-                           a->q_head_stride})
+  const long long kt = stride_of(a->tokens, a->k_token_stride), kh = stride_of(c.heads, a->k_head_stride);
+  const long long vt = stride_of(a->tokens, a->v_token_stride), vh = stride_of(c.heads, a->v_head_stride);
+  const bool q = a->q != nullptr;
+  const long long qt = q ? stride_of(a->tokens, a->q_token_stride) : 0, qh = q ? stride_of(a->n_q_heads, a->q_head_stride) : 0;
+  for (long long stride : {kt, kh, vt, vh, qt, qh})
     if (stride < 0 || stride >= 1ll << 31) {
       set_last_error("paged_append: stride of %lld elements", stride);
       return PI05_ERR_SHAPE;
@@ -746,17 +748,17 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, voi
   p.v = a->v;
   p.q = a->q;
   p.q_out = a->q_out;
-  p.kt = (int)a->k_token_stride;
-  p.kh = (int)a->k_head_stride;
-  p.vt = (int)a->v_token_stride;
-  p.vh = (int)a->v_head_stride;
-  p.qt = (int)a->q_token_stride;
-  p.qh = (int)a->q_head_stride;
+  p.kt = (int)kt;
+  p.kh = (int)kh;
+  p.vt = (int)vt;
+  p.vh = (int)vh;
+  p.qt = (int)qt;
+  p.qh = (int)qh;
   p.cu = a->cu_tokens;
   p.new_weight = a->new_weight;
   p.turns = rot ? rot->turns : nullptr;
   p.tokens = a->tokens;
-  p.q_heads = a->q != nullptr ? a->n_q_heads : 0;
+  p.q_heads = q ? a->n_q_heads : 0;
   p.rotary = rot ? rot->rotary_dim : 0;
   p.interleaved = rot ? rot->interleaved : 0;
   p.magnitude = rot ? rot->magnitude : 1.f;

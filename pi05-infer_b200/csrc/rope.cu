@@ -140,11 +140,13 @@ extern "C" int pi05_rope(const Pi05RopeArgs* a, const Pi05Rotary* rotary, void* 
     set_last_error("rope: bad shape tokens=%d heads=%d head_dim=%d rotary_dim=%d", a->tokens, a->heads, a->head_dim, r);
     return PI05_ERR_SHAPE;
   }
-  if (a->x == a->out && (a->x_token_stride != a->out_token_stride || a->x_head_stride != a->out_head_stride)) {
+  const long long xt = stride_of(a->tokens, a->x_token_stride), xh = stride_of(a->heads, a->x_head_stride);
+  const long long ot = stride_of(a->tokens, a->out_token_stride), oh = stride_of(a->heads, a->out_head_stride);
+  if (a->x == a->out && (xt != ot || xh != oh)) {
     set_last_error("rope: in place needs the same strides");
     return PI05_ERR_INVALID_ARG;
   }
-  for (long long stride : {a->x_token_stride, a->x_head_stride, a->out_token_stride, a->out_head_stride})
+  for (long long stride : {xt, xh, ot, oh})
     if (stride < 0 || stride >= 1ll << 31) {
       set_last_error("rope: stride of %lld elements", stride);
       return PI05_ERR_SHAPE;
@@ -156,10 +158,10 @@ extern "C" int pi05_rope(const Pi05RopeArgs* a, const Pi05Rotary* rotary, void* 
   }
   if (a->tokens == 0) return PI05_OK;
   RopeParams p;
-  p.xt = (int)a->x_token_stride;
-  p.xh = (int)a->x_head_stride;
-  p.ot = (int)a->out_token_stride;
-  p.oh = (int)a->out_head_stride;
+  p.xt = (int)xt;
+  p.xh = (int)xh;
+  p.ot = (int)ot;
+  p.oh = (int)oh;
   p.positions = a->positions;
   p.turns = rotary->turns;
   p.pos64 = a->positions_i64;

@@ -336,3 +336,28 @@ def test_caches_that_the_library_does_not_take():
     with pytest.raises(ValueError, match="bad cache shape"):  # 2^31 rows
         PagedKVCache(k, k, table, torch.zeros(2, 1, dtype=torch.int32, device="cuda"))
     assert torch.cuda.memory_allocated() - before < 1 << 20
+
+
+def test_rows_with_strides_of_single_elements():
+    """One token or one head: whatever stride torch has for it, beyond 31 bits too, and in place with two kinds."""
+    f, pos = RopeFrequencies(64), torch.tensor([5], device="cuda")
+    far = 2**31 + 5
+    x = rnd(1, 3, 64)
+    odd = x.as_strided((1, 3, 64), (far, 64, 1))
+    want = rope(x, pos, f)
+    assert torch.equal(rope(odd, pos, f), want)
+    assert torch.equal(rope(x, pos, f, out=torch.empty_like(x).as_strided((1, 3, 64), (1, 64, 1))), want)
+    in_place = x.clone()
+    rope(in_place.as_strided((1, 3, 64), (far, 64, 1)), pos, f, out=in_place)
+    assert torch.equal(in_place, want)
+    heads = rnd(4, 1, 64)
+    four = torch.arange(4, device="cuda")
+    assert torch.equal(rope(heads.as_strided((4, 1, 64), (64, far, 1)), four, f), rope(heads, four, f))
+    c, t = make(1, 1, 64, 16, 32)
+    k, v, q = rnd(1, 1, 64), rnd(1, 1, 64), rnd(1, 1, 64)
+    views = [y.as_strided((1, 1, 64), (far, far + 1, 1)) for y in (k, v, q)]
+    c.counts.zero_()
+    a = c.append(views[0], views[1], q=views[2], freqs=f), c.k_pages.clone(), c.v_pages.clone()
+    c.counts.zero_()
+    b = c.append(k, v, q=q, freqs=f), c.k_pages, c.v_pages
+    assert all(torch.equal(y, z) for y, z in zip(a, b)) and c.read_status() == 0
