@@ -258,6 +258,8 @@ def _rope(x, positions, freqs, out, transpose):
             ot, oh, _ = out.stride()
     else:
         ot, oh, _ = out.stride()
+    if heads == 0:
+        return out
     _run("pi05_rope", freqs._index, _ROPE_ARGS.pack(
         x.data_ptr(), out.data_ptr(), positions.data_ptr(), xt, xh, ot, oh, _DTYPES[x.dtype], tokens, heads, dim,
         positions.dtype == torch.int64, transpose), freqs._at)

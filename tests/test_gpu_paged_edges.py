@@ -361,3 +361,11 @@ def test_rows_with_strides_of_single_elements():
     c.counts.zero_()
     b = c.append(k, v, q=q, freqs=f), c.k_pages, c.v_pages
     assert all(torch.equal(y, z) for y, z in zip(a, b)) and c.read_status() == 0
+
+
+def test_rope_of_no_heads():
+    f, pos = RopeFrequencies(64), torch.arange(5, device="cuda")
+    x = torch.empty(5, 0, 64, dtype=BF, device="cuda")
+    assert rope(x, pos, f).shape == (5, 0, 64) and rope(x, pos, f, out=x) is x
+    leaf = x.clone().requires_grad_(True)
+    assert torch.autograd.grad(rope(leaf, pos, f), leaf, x)[0].shape == (5, 0, 64)
