@@ -430,11 +430,12 @@ int pi05_unnormalize_rows(const float* x, int rows, int din, const float* a, con
 #define PI05_FP32 2 /* pi05_rope only */
 
 /* Rotary positions.  Pair i of a head turns by turns[i] / 2^64 of a full turn per
- * position (fixed point, so that the angle of a far position loses nothing: the
- * product with the position wraps modulo one turn in 64-bit integers), then is
- * scaled by `magnitude`.  The pairs are the values (i, i + rotary_dim / 2) of a
- * head, or with `interleaved` (2 i, 2 i + 1); values from rotary_dim on pass
- * through.  fp32 math on each value, one rounding to the element type. */
+ * position (fixed point: the product with the position wraps modulo one turn in
+ * 64-bit integers, so that the angle of a far position is off by the table's
+ * rounding times the position and by nothing else), then is scaled by `magnitude`.
+ * The pairs are the values (i, i + rotary_dim / 2) of a head, or with `interleaved`
+ * (2 i, 2 i + 1); values from rotary_dim on pass through.  fp32 math on each value,
+ * one rounding to the element type. */
 typedef struct Pi05Rotary {
   const uint64_t* turns; /* device [rotary_dim / 2] */
   int rotary_dim;        /* even, <= head_dim, <= 512 */
@@ -513,10 +514,11 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* args, 
  * out[b, h] = sum_r softmax_r(scale * q[b, h] . k[r]) v[r] over the counts[0][b] rows
  * of key-value head h / (n_q_heads / n_kv_heads), in the cache's type; statistics and
  * sums in fp32.  key_valid [batch, valid_rows] bytes with a row pitch (0 = masked row), or
- * NULL; rows from valid_rows on count.  What a masked row holds is not read.  A sequence with no row left gives
- * out = 0, lse = -inf; rows that count but all score -inf give out = NaN (0 / 0), lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.  `track`
- * adds each row's probability, summed over the query heads of its key-value head, to
- * the cache's `weight`.  q with strides, out dense [batch, n_q_heads, head_dim].
+ * NULL; rows from valid_rows on count.  What a masked row holds is not read.  A sequence
+ * with no row left gives out = 0, lse = -inf; rows that count but all score -inf give
+ * out = NaN (0 / 0), lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.
+ * `track` adds each row's probability, summed over the query heads of its key-value head,
+ * to the cache's `weight`.  q with strides, out dense [batch, n_q_heads, head_dim].
  * `scratch`: pi05_paged_attention_scratch_bytes() bytes (0 for a few short sequences),
  * 16-byte aligned, any content.
  * The result does not depend on the run: every sum has a fixed order. */

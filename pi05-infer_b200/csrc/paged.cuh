@@ -73,16 +73,20 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
 }
 
 // ---- rotation --------------------------------------------------------------
-// The angle of a position is position * turns / 2^64 turns.  The product wraps at
-// one turn by itself, for any sign, so its top 32 bits (rounded) are the angle to
-// 2^-33 turn however far the position; a 32-bit float angle would be off by
-// 2^-24 of its size, 0.06 rad at position 10^6.
+// The angle of a position is position * turns / 2^64 turns.  The product wraps at one turn by
+// itself, for any sign, so it is off by the table's 2^-65 turn for each position and no more; a
+// 32-bit float angle would be off by 2^-24 of its size, 0.06 rad at position 10^6.  Of its top 32
+// bits (rounded: 2^-33 turn) what lies beyond the nearest quarter turn, 1/8 turn at most, becomes a
+// float, 2^-28 turn at most; the whole angle as a float would lose 2^-26.
 __device__ __forceinline__ float2 rotation(long long position, uint64_t turns, float magnitude, bool back) {
-  const uint64_t phase = (uint64_t)position * turns + 0x80000000ull;
-  const float half_turns = (float)(int32_t)(phase >> 32) * 0x1p-31f;
+  const uint32_t phase = (uint32_t)(((uint64_t)position * turns + 0x80000000ull) >> 32);
+  const uint32_t quarter = (phase + (1u << 29)) >> 30;
   float s, c;
-  sincospif(half_turns, &s, &c);
-  return make_float2(c * magnitude, (back ? -s : s) * magnitude);
+  sincospif((float)(int32_t)(phase - (quarter << 30)) * 0x1p-31f, &s, &c);
+  const float across = quarter & 1 ? s : c, up = quarter & 1 ? c : s;
+  c = (quarter ^ (quarter >> 1)) & 1 ? -across : across;
+  s = (quarter >> 1 & 1) != back ? -up : up;
+  return make_float2(c * magnitude, s * magnitude);
 }
 
 // What one thread does at a time: V pairs of the half layout (two words of V elements),

@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+from decimal import Decimal, localcontext
 from typing import Optional
 
 import torch
@@ -176,27 +177,46 @@ def _cuda(device) -> torch.device:
 # ---------------------------------------------------------------------------
 
 
-def _pair_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast, beta_slow):
-    """Rad per position of each pair, and the factor on cos and sin."""
-    if scaling == "ntk":
-        base = base * factor ** (rotary_dim / (rotary_dim - 2))
-    inv_freq = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
-    if scaling == "linear":
-        return [f / factor for f in inv_freq], 1.0
-    if scaling != "yarn":
-        return inv_freq, 1.0
+_PI = Decimal("3.1415926535897932384626433832795028841971693993751")
 
-    def pair(turns):  # number (not whole) of the pair that turns so often within original_len
-        return rotary_dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
-    ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(rotary_dim // 2)]
-    return [f / factor * r + f * (1 - r) for f, r in zip(inv_freq, ramp)], 0.1 * math.log(factor) + 1.0
+def _exact_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast, beta_slow):
+    """Rad per position of each pair, to 40 digits (a 64-bit float's 53 bits would show from position 10^8 on), and
+    the factor on cos and sin."""
+    with localcontext() as context:
+        context.prec = 50
+        exact_base, exact_factor = Decimal(base), Decimal(factor)
+        if scaling == "ntk":
+            exact_base *= exact_factor ** (Decimal(rotary_dim) / (rotary_dim - 2))
+        ratio = exact_base ** (Decimal(-2) / rotary_dim)
+        inv_freq = [Decimal(1)]
+        while len(inv_freq) < rotary_dim // 2:
+            inv_freq.append(inv_freq[-1] * ratio)
+        if scaling == "linear":
+            return [f / exact_factor for f in inv_freq], 1.0
+        if scaling != "yarn":
+            return inv_freq, 1.0
+
+        def pair(turns):  # number (not whole) of the pair that turns so often within original_len
+            return rotary_dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
+        width = max(Decimal(high - low), Decimal("0.001"))
+        ramp = [min(max((i - low) / width, Decimal(0)), Decimal(1)) for i in range(rotary_dim // 2)]
+        return [f / exact_factor * r + f * (1 - r) for f, r in zip(inv_freq, ramp)], 0.1 * math.log(factor) + 1.0
+
+
+def _pair_frequencies(*args):
+    """As 64-bit floats."""
+    inv_freq, magnitude = _exact_frequencies(*args)
+    return [float(f) for f in inv_freq], magnitude
 
 
 def _turns(inv_freq):
     """Fractions of a turn per position in units of 2^-64 (below one half: every frequency is at most 1 rad)."""
-    return [int(f / (2 * math.pi) * 2.0**64) for f in inv_freq]
+    with localcontext() as context:
+        context.prec = 50
+        return [round(Decimal(f) / (2 * _PI) * 2**64) for f in inv_freq]
 
 
 class RopeFrequencies:
@@ -213,8 +233,8 @@ class RopeFrequencies:
       divided by ``factor``, those over ``beta_fast`` times are kept, a linear ramp over the pair
       number between; cos and sin times ``0.1 ln(factor) + 1``.
 
-    The device table holds fractions of a turn in 64-bit fixed point, so an angle is as exact at
-    position 10^9 as at 1.
+    The device table holds fractions of a turn in 64-bit fixed point, each rounded once: an angle is
+    off by 2^-65 turn for each position, which is nothing to its fp32 cos and sin up to position 2^36.
     """
 
     def __init__(self, rotary_dim: int, base: float = 10000.0, *, layout: str = "half", scaling: Optional[str] = None,
@@ -235,9 +255,9 @@ class RopeFrequencies:
         if scaling == "yarn" and (original_len is None or original_len <= 0 or not beta_fast > beta_slow > 0):
             raise ValueError("'yarn' scaling needs original_len and beta_fast > beta_slow > 0")
         self.rotary_dim, self.layout = rotary_dim, layout
-        self.inv_freq, self.magnitude = _pair_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast,
-                                                          beta_slow)
-        turns = _turns(self.inv_freq)
+        exact, self.magnitude = _exact_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast, beta_slow)
+        self.inv_freq = [float(f) for f in exact]
+        turns = _turns(exact)
         self.device = _cuda(device)
         self.turns = torch.tensor(turns, dtype=torch.int64).to(self.device)
         self._index = self.device.index

@@ -4,6 +4,7 @@ A cache is held as Python dictionaries {(page, head, line): ...}-like numpy arra
 the package."""
 
 import math
+from decimal import Decimal, localcontext
 
 import numpy as np
 
@@ -35,6 +36,36 @@ def rotate(x, positions, rotary, layout="half", back=False, **kw):
     y[..., lo], y[..., hi] = x[..., lo] * c - x[..., hi] * s, x[..., hi] * c + x[..., lo] * s
     size[..., lo] = size[..., hi] = mag * (np.abs(x[..., lo]) + np.abs(x[..., hi]))
     return y, size
+
+
+def turns_of(rotary, base=10000.0, scaling=None, factor=1.0, original=None, fast=32.0, slow=1.0):
+    """Turns per position of each pair, to some 45 digits: exp(-2 i ln(base) / rotary) / (2 pi)."""
+    with localcontext() as context:
+        context.prec = 50
+        pi, b, f = _pi(), Decimal(base), Decimal(factor)
+        if scaling == "ntk":
+            b *= (f.ln() * rotary / (rotary - 2)).exp()
+        w = [(b.ln() * -2 * i / rotary).exp() / (2 * pi) for i in range(rotary // 2)]
+        if scaling == "linear":
+            w = [x / f for x in w]
+        if scaling == "yarn":
+            lo, hi = (rotary * math.log(original / (n * 2 * math.pi)) / (2 * math.log(base)) for n in (fast, slow))
+            lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), rotary - 1)
+            t = [min(max((i - lo) / max(Decimal(hi - lo), Decimal("0.001")), 0), 1) for i in range(rotary // 2)]
+            w = [x * (y / f + (1 - y)) for x, y in zip(w, t)]
+        return w
+
+
+def _pi():
+    """By Machin's formula, 16 arctan(1/5) - 4 arctan(1/239)."""
+    def arctan(n):
+        x, total, k = Decimal(1) / n, Decimal(0), 0
+        while abs(x) > Decimal(10) ** -55:
+            total += x / (2 * k + 1) * (-1) ** k
+            x, k = x / (n * n), k + 1
+        return total
+
+    return 16 * arctan(5) - 4 * arctan(239)
 
 
 class Cache:

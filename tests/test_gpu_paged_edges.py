@@ -2,6 +2,8 @@
 views, forward-mode derivatives, tables far longer than their sequences.  Model, tolerances and helpers as in
 ``test_gpu_paged.py``."""
 
+from decimal import localcontext
+
 import numpy as np
 import pytest
 import torch
@@ -9,7 +11,8 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
-from test_gpu_paged import BF, F, HF, check_rope, gen, make, np64, rnd, same_rows, twin, u
+from paged_model import turns_of
+from test_gpu_paged import BF, F, FP, HF, check_rope, gen, make, np64, rnd, same_rows, twin, u
 
 from pi05_infer import PagedKVCache, RopeFrequencies, rope
 
@@ -369,3 +372,26 @@ def test_rope_of_no_heads():
     assert rope(x, pos, f).shape == (5, 0, 64) and rope(x, pos, f, out=x) is x
     leaf = x.clone().requires_grad_(True)
     assert torch.autograd.grad(rope(leaf, pos, f), leaf, x)[0].shape == (5, 0, 64)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(), dict(scaling="linear", factor=3.0), dict(scaling="ntk", factor=8.0, base=500000.0),
+    dict(scaling="yarn", factor=16.0, original=8192),
+])
+def test_rope_angles_of_far_positions(kw):
+    """(1, 0) turns to cos and sin: within 4 fp32 roundings of the exact ones, 2 each for the functions, 1.5 for the
+    angle's 2^-28 turn beyond a quarter and half a one for the table's 2^-65 turn a position up to 2^36, more beyond."""
+    f = RopeFrequencies(64, layout="interleaved", **{("original_len" if k == "original" else k): v for k, v in kw.items()})
+    g = np.random.default_rng(3)
+    pos = [0, 1, -1, 2, 12345, 10**6 + 1, 10**9, 2**31 - 1, -(2**31), 2**40 + 3, -(2**45) - 1]
+    pos += g.integers(-(2**36), 2**36, 400).tolist() + g.integers(-(2**31), 2**31, 400).tolist()
+    x = torch.zeros(len(pos), 1, 64, dtype=FP, device="cuda")
+    x[..., 0::2] = 1.0
+    y = np64(rope(x, torch.tensor(pos, device="cuda"), f))[:, 0]
+    with localcontext() as context:
+        context.prec = 50
+        turn = np.array([[float(n * t - round(n * t)) for t in turns_of(64, **kw)] for n in pos])
+    far = np.abs(np.array(pos, dtype=np.float64))[:, None] * 2.0**-65 * 2 * np.pi
+    tol = (4 * F + np.maximum(far - F, 0)) * f.magnitude + F * f.magnitude  # and the product with the magnitude
+    assert (np.abs(y[:, 0::2] - np.cos(2 * np.pi * turn) * f.magnitude) <= tol).all()
+    assert (np.abs(y[:, 1::2] - np.sin(2 * np.pi * turn) * f.magnitude) <= tol).all()
