@@ -139,7 +139,7 @@ def _run(name: str, index: int, *args) -> None:
         raise _lib.Pi05Error(name, rc, _lib.last_error())
 
 
-_increment_version = torch.autograd.graph.increment_version
+_increment_version = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
 
 
 def _wrote(tensors) -> None:
@@ -479,11 +479,13 @@ class PagedKVCache:
                              f"{self.dtype} on {self.device}, contiguous in its last dimension")
         return shape, strides
 
-    def _no_gradients(self, **tensors) -> None:
+    def _no_gradients(self, tensors, names) -> None:
         """The cache has no derivative: refuses one wanted of an input, or through what is written or read."""
-        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
-            for name, t in (*tensors.items(), ("k_pages", self.k_pages), ("v_pages", self.v_pages)):
-                if t is not None and _wants_grad(t):
+        forward = forward_ad._current_level >= 0
+        if forward or torch.is_grad_enabled():
+            for t in tensors:
+                if t is not None and (forward or t.requires_grad) and _wants_grad(t):
+                    name = names[[t is other for other in tensors].index(True)]
                     raise ValueError(f"the cache is not differentiable: {name} needs a gradient (use torch.no_grad())")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
@@ -501,7 +503,8 @@ class PagedKVCache:
         """
         (tokens, _, _), (k_token, k_head, _) = self._rows(k, "k", self.n_kv_heads)
         (v_tokens, _, _), (v_token, v_head, _) = self._rows(v, "v", self.n_kv_heads)
-        self._no_gradients(k=k, v=v, q=q, q_out=q_out, new_weight=weight, weight=self.weight)
+        self._no_gradients((k, v, q, q_out, weight, self.k_pages, self.v_pages, self.weight),
+                           ("k", "v", "q", "q_out", "weight", "k_pages", "v_pages", "the cache's weight"))
         if v_tokens != tokens:
             raise ValueError(f"k has {tokens} tokens, v has {v_tokens}")
         q_at = q_out_at = q_token = q_head = n_q_heads = rotary = cu_at = weight_at = 0
@@ -557,7 +560,8 @@ class PagedKVCache:
         natural-log sums ``[batch, heads]``.
         """
         (batch, heads, dim), (q_token, q_head, _) = self._rows(q, "q", None)
-        self._no_gradients(q=q, out=out, weight=self.weight if track else None)
+        self._no_gradients((q, out, self.k_pages, self.v_pages, self.weight if track else None),
+                           ("q", "out", "k_pages", "v_pages", "the cache's weight"))
         if batch != self.batch or heads == 0 or heads % self.n_kv_heads:
             raise ValueError(f"q must be [{self.batch}, a multiple of {self.n_kv_heads}, {dim}], got {list(q.shape)}")
         if track and self.weight is None:
@@ -608,7 +612,7 @@ class PagedKVCache:
             raise ValueError("this cache keeps no weights and positions: build it with weight= and pos=")
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
             raise ValueError(f"need budget >= 1 and 0 <= recent + sinks <= budget, got {budget}, {recent}, {sinks}")
-        self._no_gradients(weight=self.weight)
+        self._no_gradients((self.k_pages, self.v_pages, self.weight), ("k_pages", "v_pages", "the cache's weight"))
         if budget >= self.pages_per_seq * self.page_size:
             return  # no sequence can hold more; and below, the numbers fit the library's 32 bits
         _run("pi05_paged_evict", self._index, self._at, budget, recent, sinks)
