@@ -484,7 +484,9 @@ typedef struct Pi05PagedCache {
   size_t workspace_bytes;
 } Pi05PagedCache;
 
-/* Workspace bytes of a cache (0 for a struct that the ops refuse). */
+/* Workspace bytes of a cache (0 for a struct that the ops refuse): 17 KB, and with `weight` and
+ * `pos` the eviction's lists, 4 bytes for each row that the table reaches or, beyond 16 MB, for
+ * each row of the pool where that is less. */
 size_t pi05_paged_workspace_bytes(const Pi05PagedCache* cache);
 
 /* Appends `tokens` new rows and moves the counts on.  k, v [tokens, n_kv_heads,

@@ -289,10 +289,14 @@ struct Pages {
   int32_t* counts;
   int* status;
   int* ticket;     // of an append
-  int* tickets;    // of an eviction's sequences
-  int32_t* moves;  // eviction: per (sequence, head) two counts and a list of `capacity`
+  // Eviction: tickets of the sequences; of each (sequence, head) the number of its moves (-1: the
+  // sequence stays as it is) and the rows left; and a list.
+  int* tickets;
+  int2* moves;
+  int32_t* move_list;
   FastDiv page_div;
   int num_pages, page_size, heads, dim, batch, pitch, capacity;
+  bool list_by_slot;
 
   __device__ __forceinline__ int rows(int b) const { return min(max(counts[b], 0), capacity); }
   // Page of row r (r < capacity) as the table has it, and its line.
@@ -331,10 +335,23 @@ int allow_smem(K kernel, int bytes, std::atomic<uint64_t>* done, const char* op)
 int paged_check(const Pi05PagedCache* c, const char* op, Pages* out);
 
 // Workspace of a cache: status word and ticket in the first 16640 bytes (as in the
-// engine's workspace, so that the same status call reads it), then the eviction's tickets
-// and move lists.
+// engine's workspace, so that the same status call reads it); then, for a cache that keeps
+// weights and positions, the eviction's tickets, counts and lists.
+inline size_t paged_pairs(const Pi05PagedCache* c) { return (size_t)c->batch * c->n_kv_heads; }
+
+// A list has an entry for each row that the table can reach, or, where that takes more than 16 MB
+// and more than the pool's rows, stands at the rows' own slots: 4 bytes a slot of the pool, however
+// long the table, for a look into the table with each entry.
+inline bool paged_list_by_slot(const Pi05PagedCache* c) {
+  const size_t reach = paged_pairs(c) * c->pages_per_seq * c->page_size;
+  return reach * sizeof(int32_t) > (16u << 20) && (size_t)c->num_pages * c->n_kv_heads * c->page_size < reach;
+}
+
 inline size_t paged_moves_bytes(const Pi05PagedCache* c) {
-  return (size_t)c->batch * (1 + c->n_kv_heads * ((size_t)c->pages_per_seq * c->page_size + 2)) * sizeof(int32_t);
+  if (c->weight == nullptr || c->pos == nullptr) return 0;
+  const size_t rows = paged_list_by_slot(c) ? (size_t)c->num_pages * c->n_kv_heads * c->page_size
+                                            : paged_pairs(c) * c->pages_per_seq * c->page_size;
+  return ((size_t)c->batch + (c->batch & 1) + 2 * paged_pairs(c) + rows) * sizeof(int32_t);
 }
 
 }  // namespace pi05

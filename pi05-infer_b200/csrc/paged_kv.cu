@@ -54,7 +54,9 @@ int paged_check(const Pi05PagedCache* c, const char* op, Pages* out) {
   out->status = reinterpret_cast<int*>(ws + kWsStatusOffset);
   out->ticket = reinterpret_cast<int*>(ws + kWsCounterOffset);
   out->tickets = reinterpret_cast<int*>(ws + kWsAccumOffset);
-  out->moves = reinterpret_cast<int32_t*>(ws + kWsAccumOffset) + c->batch;
+  out->moves = reinterpret_cast<int2*>(out->tickets + c->batch + (c->batch & 1));
+  out->move_list = reinterpret_cast<int32_t*>(out->moves + paged_pairs(c));
+  out->list_by_slot = paged_list_by_slot(c);
   out->page_div = FastDiv((uint32_t)c->page_size);
   out->num_pages = c->num_pages;
   out->page_size = c->page_size;
@@ -306,10 +308,17 @@ __device__ __forceinline__ int ld_cluster(const void* p, uint32_t rank) {
   return v;
 }
 
-// Copies a row's key and value, weight and position; one warp.
-__device__ __forceinline__ void move_row(const Pages& c, int b, int h, int from_row, int to_row, int lane) {
+// Copies a row's key and value, weight and position; one warp.  Rows of no page can only come
+// from a list at slots that another sequence has, too (which the table may not say); elsewhere the
+// copy does not wait to know.
+__device__ __forceinline__ void move_row(const Pages& c, bool check, int b, int h, int from_row, int to_row,
+                                         int lane) {
   int from_line, to_line;
   const int from = c.page_of(b, from_row, &from_line), to = c.page_of(b, to_row, &to_line);
+  if (check && (!c.real(from) || !c.real(to))) {
+    if (lane == 0) report_status(c.status, PI05_DEV_BAD_INDEX);
+    return;
+  }
   const size_t src = c.row_at(from, h, from_line), dst = c.row_at(to, h, to_line);
   if (lane < c.dim / 8) {
     const uint4 k = ld16(c.k + src + lane * 16), v = ld16(c.v + src + lane * 16);
@@ -339,8 +348,23 @@ __device__ __forceinline__ Victim warp_least(Victim v) {
   return {k, (int)__reduce_min_sync(~0u, v.key == k ? (unsigned)v.row : 0x7fffffffu)};
 }
 
-// Moves of row list `moves`: [0] their number (-1: the sequence stays as it is), [1] the
-// rows left, then the holes, ascending, and from [2 + left] on the rows that fill them.
+// The list of a (sequence, head); entry i is below the rows it holds, all in real pages.
+struct MoveList {
+  const Pages& c;
+  const bool by_slot;
+  int b, h;
+  int32_t* dense;
+  __device__ __forceinline__ MoveList(const Pages& pages, bool slots, int seq, int head)
+      : c(pages), by_slot(slots), b(seq), h(head), dense(pages.move_list + (size_t)(seq * pages.heads + head) * pages.capacity) {}
+  __device__ __forceinline__ int32_t* at(int i) const {
+    if (!by_slot) return dense + i;
+    int line;
+    const int page = c.page_of(b, i, &line);
+    return c.move_list + c.slot_at(page, h, line);
+  }
+};
+
+// The list: the holes, ascending, and from entry `left` on the rows that fill them.
 // `move_here`: few enough, however long the sequence, to do them on the spot.  FIT: a CTA holds all its keys.
 template <int NT, bool FIT>
 __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant__ Pages c, int budget, int recent,
@@ -357,11 +381,10 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   pdl_launch_dependents();
   const int pair = blockIdx.x / ctas, rank = blockIdx.x - pair * ctas;  // the grid is a line of clusters
   const int b = pair / c.heads, h = pair - b * c.heads, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  int32_t* moves = c.moves + (size_t)pair * (c.capacity + 2);
   const int len = c.rows(b);
   const long long recent_from = (long long)c.counts[c.batch + b] - recent;
   if (len <= budget) {  // the whole cluster alike
-    if (tid == 0 && rank == 0) moves[0] = -1;
+    if (tid == 0 && rank == 0) c.moves[pair].x = -1;
     return;
   }
   auto sync_all = [&]() {
@@ -414,7 +437,7 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   auto of_all = [&](const int* x) { return lane < ctas ? peer(x, lane) : 0; };
   if (__any_sync(~0u, of_all(&sh_bad) != 0)) {
     if (tid == 0 && rank == 0) {
-      moves[0] = -1;
+      c.moves[pair].x = -1;
       report_status(c.status, PI05_DEV_BAD_INDEX);
     }
     sync_all();  // nobody leaves while others look at its shared memory
@@ -430,7 +453,7 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   // A few rows to go (one, in a program that evicts after every token): one by one, the
   // least that comes after the last.
   if (len - budget <= kFew) {
-    if (tid == 0 && rank == 0) moves[0] = -1;  // done here
+    if (tid == 0 && rank == 0) c.moves[pair].x = -1;  // done here
     Victim gone[kFew];
     const int few = len - budget;
 #pragma unroll
@@ -472,7 +495,7 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
       const uint32_t tails = __ballot_sync(~0u, stays);
       for (int v = 0; v < __popc(tails); ++v) {
         const int to = __shfl_sync(~0u, mine, __ffs(__ballot_sync(~0u, lane < few && at == v)) - 1);
-        move_row(c, b, h, budget + __fns(tails, 0, v + 1), to, lane);
+        move_row(c, false, b, h, budget + __fns(tails, 0, v + 1), to, lane);
       }
     }
     if (ctas > 1) sync_all();  // nobody leaves while others look at its shared memory
@@ -613,37 +636,38 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   int at_hole = __reduce_add_sync(~0u, lane < rank ? their_holes : 0) + sum_before(warp_a, w, lane);
   int at_tail = __reduce_add_sync(~0u, lane < rank ? their_tails : 0) + sum_before(warp_b, w, lane);
   seen = ties;
+  const MoveList list(c, c.list_by_slot, b, h);
   for (int g = g0; g < g0 + per; ++g) {
     bool hole, tail;
     classify(g, seen, hole, tail);
     const uint32_t m = __ballot_sync(~0u, hole), m2 = __ballot_sync(~0u, tail);
-    if (hole) moves[2 + at_hole + __popc(m & below)] = first + g * 32 + lane;
-    if (tail) moves[2 + budget + at_tail + __popc(m2 & below)] = first + g * 32 + lane;
+    if (hole) *list.at(at_hole + __popc(m & below)) = first + g * 32 + lane;
+    if (tail) *list.at(budget + at_tail + __popc(m2 & below)) = first + g * 32 + lane;
     at_hole += __popc(m);
     at_tail += __popc(m2);
   }
-  if (tid == 0 && rank == 0) {
-    moves[0] = all;
-    moves[1] = budget;
-  }
+  if (tid == 0 && rank == 0) c.moves[pair] = make_int2(all, budget);
   sync_all();  // the lists are written; and nobody leaves while others look at its shared memory
   if (!move_here) return;
-  for (int m = rank * NW + w; m < all; m += ctas * NW) move_row(c, b, h, moves[2 + budget + m], moves[2 + m], lane);
+  for (int m = rank * NW + w; m < all; m += ctas * NW)
+    move_row(c, c.list_by_slot, b, h, *list.at(budget + m), *list.at(m), lane);
   cut_count();
 }
 
+// (At most 32 registers: with 40 the moves of 8 pairs of 65536 rows cut to 8192 take 18 us, not 15.)
 // One warp per move.  Sources lie at or above the budget and targets below it, so no
 // move reads what another writes.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ Pages c) {
+template <bool BY_SLOT>
+__global__ void __launch_bounds__(kMoveThreads, 8) evict_move_kernel(const __grid_constant__ Pages c) {
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads;
-  const int32_t* moves = c.moves + (size_t)blockIdx.x * (c.capacity + 2);
-  const int n = moves[0];
+  const int n = c.moves[blockIdx.x].x;
   if (n < 0) return;
-  const int left = moves[1];
+  const int left = c.moves[blockIdx.x].y;
+  const MoveList list(c, BY_SLOT, b, h);
   for (int m = blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5); m < n; m += gridDim.y * (kMoveThreads / 32))
-    move_row(c, b, h, moves[2 + left + m], moves[2 + m], threadIdx.x & 31);
+    move_row(c, BY_SLOT, b, h, *list.at(left + m), *list.at(m), threadIdx.x & 31);
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) c.counts[b] = left;
 }
 
@@ -805,7 +829,8 @@ int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int si
                           recent, sinks, ctas, held, move_here);
   if (rc || move_here) return rc;
   const int chunks = std::min((most + kMoveThreads / 32 - 1) / (kMoveThreads / 32), std::max(1, kSMs * 16 / pairs));
-  return launch_pdl(evict_move_kernel, dim3(pairs, chunks), dim3(kMoveThreads), 0, st, pdl_enabled(), c);
+  return launch_pdl(c.list_by_slot ? evict_move_kernel<true> : evict_move_kernel<false>, dim3(pairs, chunks),
+                    dim3(kMoveThreads), 0, st, pdl_enabled(), c);
 }
 
 }  // extern "C"

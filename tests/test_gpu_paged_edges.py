@@ -395,3 +395,44 @@ def test_rope_angles_of_far_positions(kw):
     tol = (4 * F + np.maximum(far - F, 0)) * f.magnitude + F * f.magnitude  # and the product with the magnitude
     assert (np.abs(y[:, 0::2] - np.cos(2 * np.pi * turn) * f.magnitude) <= tol).all()
     assert (np.abs(y[:, 1::2] - np.sin(2 * np.pi * turn) * f.magnitude) <= tol).all()
+
+
+# ---------------------------------------------------------------------------
+# tables far longer than their sequences
+# ---------------------------------------------------------------------------
+
+
+def long_table(batch, heads, dim, page, lens, each, *, dtype=BF, seed=0):
+    """A pool for `lens` rows a sequence, behind a table of `each` pages a sequence, no page in the rest of it."""
+    c, _ = make(batch, heads, dim, page, max(lens), dtype=dtype, seed=seed)
+    table = torch.full((batch, each), -1, dtype=torch.int32, device="cuda")
+    table[:, : c.pages_per_seq] = c.page_table
+    d = PagedKVCache(c.k_pages, c.v_pages, table, c.counts, weight=c.weight, pos=c.pos)
+    d.counts[:] = torch.tensor(lens)
+    return d, twin(d)
+
+
+@pytest.mark.parametrize("budget", [100, 40, 198])  # moved by a kernel of their own, on the spot, a few rows
+def test_evict_behind_a_long_table(budget):
+    """The workspace goes by the pool where the table reaches further; what is evicted does not change."""
+    lens = [200 - 7 * (i % 9) for i in range(40)]
+    c, t = long_table(40, 2, 64, 16, lens, 4096)
+    assert c.workspace.numel() < (1 << 16) + c.num_pages * 2 * 16 * 4
+    r = np.random.default_rng(2)
+    t.pos[:] = r.integers(0, 200, t.pos.shape)
+    t.weight[:] = np.round(r.standard_normal(t.weight.shape), 1).astype(np.float32)
+    c.pos.copy_(torch.tensor(t.pos))
+    c.weight.copy_(torch.tensor(t.weight))
+    for left in (budget, budget // 2):
+        c.evict(left, recent=10, sinks=2)
+        t.evict(left, 10, 2)
+        same_rows(c, t)
+    assert c.read_status() == 0
+
+
+def test_workspace_of_a_cache_without_weights():
+    c = PagedKVCache.allocate(8, 16, 2, 64, 64, 8192, track=False)
+    assert c.workspace.numel() <= 1 << 15
+    c.page_table[:, 0] = 3
+    c.counts[0] = 5
+    assert c.attend(rnd(64, 2, 64)).shape == (64, 2, 64) and c.read_status() == 0
