@@ -60,7 +60,11 @@ struct AttnParams {
   float2* part_ml;  // [2 n_ctas][8 NT]
   int2* row_info;   // [rows]: first partial slot (-1: done), last CTA
   float* row_lse;   // [rows][8 NT] log2 units, of the rows done in one piece
-  float* scores;    // [rows][capacity][score_pitch], log2 units (track)
+  // track: scores in log2 units, [score_units][kBlockRows][score_pitch], where a row's begin with
+  // its unit (see Walk)
+  float* scores;
+  int* row_unit;  // [rows]: or -1, when there are more units than scores
+  int score_units;
   int score_pitch;  // heads of a part, up to a power of two from 2 on
 };
 
@@ -335,6 +339,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
     long long incl = scan(own);
     for (int i = 0; i < kWarps; ++i) total += sh_sum[i];
     n = min((long long)gridDim.x, total);
+    // More rows than the pool has: pages that stand twice in the table, or none.
+    if (p.track && total > p.score_units && cta == 0 && tid == 0) report_status(p.c.status, PI05_DEV_BAD_INDEX);
     if (cta >= n) return;
     const long long lo = divide(cta * total, n), hi = divide((cta + 1) * total, n);
     long long before = 0;
@@ -420,9 +426,15 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
   for (int slot = 2 * (int)cta; have; slot |= 1) {
     const Segment s = next;
     const int heads = min(H, p.group - s.part * H), head0 = s.kvh * p.group + s.part * H;
-    if (!SHORT && s.tile0 == 0 && tid == 0) {
-      // the CTA that has the pair's last block
-      p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)divide(walk.pair_end * n - 1, total));
+    int unit = 0;  // the pair's first, where its scores go; all into the first, unread, if they have no room
+    if constexpr (!SHORT) {
+      const bool room = total <= p.score_units;
+      if (p.track && room) unit = (int)(walk.pair_end - (s.len + kBlockRows - 1) / kBlockRows - kBorder);
+      if (s.tile0 == 0 && tid == 0) {
+        // the CTA that has the pair's last block
+        p.row_info[s.row] = s.whole ? make_int2(-1, -1) : make_int2(slot, (int)divide(walk.pair_end * n - 1, total));
+        if (p.track) p.row_unit[s.row] = room ? unit : -1;
+      }
     }
     float o[KS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KS, NT, SHORT>::kPerSM)
         if (p.track) {
           const int h = nt * 8 + 2 * (lane & 3), r0 = ((s.tile0 + j) * kWarps + w) * kWarpRows + (lane >> 2);
           float* dst = SHORT ? my_scores + (r0 - s.tile0 * kBlockRows) * p.score_pitch + h
-                             : p.scores + ((size_t)s.row * p.c.capacity + r0) * p.score_pitch + h;
+                             : p.scores + ((size_t)unit * kBlockRows + r0) * p.score_pitch + h;
           auto score = [](bool counts, float x) { return counts && x == -INFINITY ? kLowest : x; };
           if (r0 < s.len && h < heads)
             *reinterpret_cast<float2*>(dst) = make_float2(score(live0, xs[0]), score(live0, xs[1]));
@@ -831,7 +843,9 @@ __global__ void __launch_bounds__(kFinishThreads) paged_track_kernel(const __gri
     }
     for (int part = 0; part < p.parts; ++part) {
       const int row = (int)blockIdx.x * p.parts + part, heads = min(H, p.group - part * H);
-      const float* from = p.scores + ((size_t)row * p.c.capacity + r0 + threadIdx.x) * P;
+      const int unit = p.row_unit[row];
+      if (unit < 0) return;
+      const float* from = p.scores + ((size_t)unit * kBlockRows + r0 + threadIdx.x) * P;
       __align__(16) float s[R][P];
       float lse[P];
 #pragma unroll
@@ -865,7 +879,8 @@ struct Plan {
   int nt, parts, ks, ctas, rows, score_pitch;
   int short_ctas;       // CTAs of a pair in the form without further kernels, or 0
   size_t short_scores;  // its shared memory for scores
-  size_t part_o, part_ml, row_info, row_lse, scores, bytes;
+  int score_units;
+  size_t part_o, part_ml, row_info, row_lse, row_unit, scores, bytes;
 };
 
 // Steps of 16 columns that there are kernels for: every even size up to 12 and 5, which
@@ -941,7 +956,16 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   s.part_ml = take(2 * (size_t)s.ctas * h * 8);
   s.row_info = take((size_t)s.rows * 8);
   s.row_lse = take((size_t)s.rows * h * 4);
-  s.scores = take(track ? (size_t)s.rows * capacity * s.score_pitch * 4 : 0);
+  // Scores for every row that the table reaches, or, beyond 64 MB, that the pool has (in blocks: a
+  // block begun and the border for each pair): whoever tracks has each row in one sequence alone.
+  // No less than for one pair that the table's reach fills.
+  const size_t unit_bytes = (size_t)kBlockRows * s.score_pitch * 4;
+  const long long pool = (((long long)c->num_pages * c->page_size) / kBlockRows + (1ll + kBorder) * c->batch) * c->n_kv_heads * s.parts;
+  const long long longest = blocks_of(capacity) + kBorder;
+  s.score_units = (int)std::min<long long>(
+      {longest * s.rows, std::max<long long>({pool, longest, (long long)((64 << 20) / unit_bytes)}), 0x7fffffff});
+  s.row_unit = take(track ? (size_t)s.rows * 4 : 0);
+  s.scores = take(track ? s.score_units * unit_bytes : 0);
   s.bytes = at;
   return s;
 }
@@ -1057,6 +1081,8 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
   p.row_info = reinterpret_cast<int2*>(sc + s.row_info);
   p.row_lse = reinterpret_cast<float*>(sc + s.row_lse);
   p.scores = reinterpret_cast<float*>(sc + s.scores);
+  p.row_unit = reinterpret_cast<int*>(sc + s.row_unit);
+  p.score_units = s.score_units;
   p.score_pitch = s.score_pitch;
   p.ctas = s.short_ctas;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

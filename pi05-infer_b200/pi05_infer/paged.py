@@ -554,8 +554,8 @@ class PagedKVCache:
         ``scale`` is ``head_dim ** -0.5`` if not given.  ``key_valid`` (bool or uint8 ``[batch, n]``):
         rows that are False are left out, whatever they hold; rows from ``n`` on count (a prompt's
         padding mask need not grow with the sequence).  ``track`` adds the probabilities to the
-        cache's ``weight`` (its scratch holds a score for every row there can be and query head, so a
-        table much longer than its sequences costs memory).  A sequence with no row gives zeros (lse
+        cache's ``weight`` (its scratch holds a score of every query head for each row that the table
+        reaches or, beyond 64 MB, that the pool has).  A sequence with no row gives zeros (lse
         ``-inf``); rows that count but all score ``-inf`` give NaN, as a softmax of them does.  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
         natural-log sums ``[batch, heads]``.
         """

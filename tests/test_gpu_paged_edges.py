@@ -12,7 +12,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 from paged_model import turns_of
-from test_gpu_paged import BF, F, FP, HF, check_rope, gen, make, np64, rnd, same_rows, twin, u
+from test_gpu_paged import BF, F, FP, HF, check_attend, check_rope, gen, make, np64, rnd, same_rows, twin, u
 
 from pi05_infer import PagedKVCache, RopeFrequencies, rope
 
@@ -436,3 +436,31 @@ def test_workspace_of_a_cache_without_weights():
     c.page_table[:, 0] = 3
     c.counts[0] = 5
     assert c.attend(rnd(64, 2, 64)).shape == (64, 2, 64) and c.read_status() == 0
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads", [(160, 8, 2), (100, 18, 1)])
+def test_attend_behind_a_long_table(batch, heads, kv_heads):
+    """Tracked: the scratch goes by the pool where the table reaches further; what is computed does not change."""
+    lens = [1 + (37 * i) % 300 for i in range(batch)]
+    lens[0] = 0
+    c, t = long_table(batch, kv_heads, 64, 16, lens, 8192)
+    valid = torch.rand(batch, 250, device="cuda", generator=gen(4)) > 0.2
+    need = c._need(heads, True)[0] - c._need(heads, False)[0]
+    assert need < (64 << 20) + (1 << 16) + batch * heads * 64
+    check_attend(c, t, rnd(batch, heads, 64, g=gen(1)), valid=valid, track=True)
+    assert c.read_status() == 0
+
+
+def test_attend_tracks_no_more_rows_than_the_pool_has():
+    """Pages that stand in several sequences (not allowed to a call that writes), so many that the scores have no
+    room: the weights stay, the status says so, and the output is that of a call that only reads."""
+    k, v = rnd(4, 1, 16, 64), rnd(4, 1, 16, 64)
+    weight = torch.rand(4, 1, 16, device="cuda")
+    table = torch.zeros(96, 8192, dtype=torch.int32, device="cuda")
+    counts = torch.full((2, 96), 16 * 8192, dtype=torch.int32, device="cuda")
+    c = PagedKVCache(k, v, table, counts, weight=weight, pos=torch.zeros(4, 1, 16, dtype=torch.int32, device="cuda"))
+    q, before = rnd(96, 2, 64), weight.clone()
+    want = c.attend(q)
+    assert c.read_status() == 0
+    assert torch.equal(c.attend(q, track=True), want) and torch.equal(weight, before)
+    assert c.read_status() == 0x20

@@ -1,5 +1,6 @@
 """CPU tests of the text-decoding operators' host side at its edges."""
 
+import ctypes
 import math
 from decimal import Decimal, localcontext
 
@@ -36,3 +37,23 @@ def test_table_is_rounded_once(rotary, base, scaling, factor, original):
         context.prec = 50
         for t, want in zip(paged._turns(exact), turns_of(rotary, base, scaling, factor, original), strict=True):
             assert abs(t - want * 2**64) <= Decimal("0.5000001")
+
+
+def test_sizes_go_by_the_pool():
+    """Scratch and workspace behind tables for 131072 rows, 256 sequences, 8 heads, over 65536 pages of 16 rows."""
+    def sizes(weight=16, **kw):
+        shape = dict(num_pages=65536, page_size=16, n_kv_heads=8, head_dim=128, batch=256, pages_per_seq=8192) | kw
+        c = paged.Pi05PagedCache(dtype=0, weight=weight, pos=weight, table_pitch=shape["pages_per_seq"], **shape)
+        at = ctypes.byref(c)
+        scratch = [paged._fn("pi05_paged_attention_scratch_bytes")(at, 32, track) for track in (0, 1)]
+        return paged._fn("pi05_paged_workspace_bytes")(at), scratch[1] - scratch[0]
+
+    slots = 65536 * 16 * 8
+    lists, scores = sizes()
+    assert 4 * slots <= lists < 4 * slots + (1 << 16)  # 34 MB; by the table it was 1.07 GB
+    assert 16 * slots <= scores < 16 * slots + 256 * 8 * 3 * 64 * 16 + (1 << 16)  # 138 MB; 4.3 GB
+    assert sizes(weight=None)[0] < 1 << 15
+    lists, scores = sizes(num_pages=64)  # small pools: never less than 64 MB where the table asks for more
+    assert lists < 1 << 17 and 60 << 20 < scores < 65 << 20
+    lists, scores = sizes(pages_per_seq=16, num_pages=1 << 20)  # short tables over a large pool: by the table
+    assert lists < 4 * 256 * 8 * 256 + (1 << 16) and scores < 16 * 256 * 8 * (256 + 128) + (1 << 16)
