@@ -464,3 +464,57 @@ def test_attend_tracks_no_more_rows_than_the_pool_has():
     assert c.read_status() == 0
     assert torch.equal(c.attend(q, track=True), want) and torch.equal(weight, before)
     assert c.read_status() == 0x20
+
+
+# ---------------------------------------------------------------------------
+# every kernel that the sizes choose
+# ---------------------------------------------------------------------------
+
+# batch, heads, kv_heads, dim, page, lens, pages a sequence that the table has room for
+KERNELS = [
+    # heads of 129 to 160 and of 161 to 192 columns: a cluster for each pair, then equal shares
+    (3, 4, 2, 136, 16, [0, 77, 300], 20), (3, 4, 2, 160, 16, [1, 130, 300], 20), (2, 3, 1, 176, 8, [65, 200], 30),
+    (2, 8, 1, 192, 24, [500, 3], 30),
+    (3, 4, 2, 136, 16, [0, 77, 900], 4096), (3, 4, 2, 160, 16, [1, 130, 900], 4096), (2, 3, 1, 176, 8, [65, 700], 4096),
+    (2, 8, 1, 192, 24, [1500, 3], 4096),
+    # 9 to 16 query heads of a key-value head: clusters, then equal shares
+    (2, 9, 1, 72, 16, [40, 333], 30), (2, 32, 2, 96, 16, [63, 200], 20), (2, 10, 1, 160, 16, [129, 64], 20),
+    (1, 16, 1, 192, 16, [250], 16),
+    (2, 9, 1, 72, 16, [40, 900], 4096), (2, 32, 2, 96, 16, [63, 700], 4096), (2, 10, 1, 160, 16, [129, 1000], 4096),
+    (2, 16, 1, 192, 16, [250, 1], 4096), (3, 30, 2, 256, 16, [700, 0, 65], 4096), (2, 12, 1, 200, 16, [128, 129], 4096),
+    (2, 13, 1, 64, 16, [900, 1], 4096), (2, 16, 1, 128, 16, [2000, 17], 4096),
+    # more than 16, in parts
+    (2, 17, 1, 72, 16, [40, 500], 64), (2, 34, 2, 96, 16, [63, 300], 64), (2, 33, 1, 160, 16, [129, 400], 64),
+    (1, 20, 1, 192, 16, [700], 64), (2, 48, 2, 256, 16, [1, 600], 64), (1, 24, 1, 128, 8, [3000], 400),
+    # one long sequence among many pairs: more chunks of it to track than CTAs that do
+    (256, 2, 1, 64, 16, [9001] + [3] * 255, 600), (130, 18, 2, 64, 16, [4300] + [(5 * i) % 9 for i in range(129)], 300),
+]
+
+
+def pooled(batch, heads, dim, page, lens, each, *, dtype=BF, seed=0):
+    """A cache with just the pages that `lens` rows take, in no order, behind a table of `each` pages a sequence."""
+    g = gen(seed)
+    used = [-(-n // page) for n in lens]
+    pages = sum(used) + 1
+    k, v = (rnd(pages, heads, page, dim, dtype=dtype, g=g) for _ in range(2))
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    table = torch.full((batch, each), -1, dtype=torch.int32)
+    for b, n in enumerate(used):
+        table[b, :n] = order[sum(used[:b]) : sum(used[:b]) + n]
+    c = PagedKVCache(k, v, table.cuda(), torch.tensor([lens, lens], dtype=torch.int32, device="cuda"),
+                     weight=torch.rand(pages, heads, page, device="cuda", generator=g),
+                     pos=torch.zeros(pages, heads, page, dtype=torch.int32, device="cuda"))
+    return c, twin(c)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", KERNELS, ids=lambda c: f"b{c[0]}h{c[1]}kv{c[2]}d{c[3]}n{max(c[5])}t{c[6]}")
+def test_attend_every_kernel(case, dtype):
+    batch, heads, kv_heads, dim, page, lens, each = case
+    c, t = pooled(batch, kv_heads, dim, page, lens, each, dtype=dtype)
+    g = gen(13)
+    q = rnd(batch, heads, dim, dtype=dtype, g=g, scale=2.0)
+    valid = torch.rand(batch, max(max(lens) - 2, 1), device="cuda", generator=g) > 0.3
+    check_attend(c, t, q)
+    check_attend(c, t, q, valid=valid, track=True)
+    assert c.read_status() == 0
