@@ -516,7 +516,8 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* args, 
  * out[b, h] = sum_r softmax_r(scale * q[b, h] . k[r]) v[r] over the counts[0][b] rows
  * of key-value head h / (n_q_heads / n_kv_heads), in the cache's type; statistics and
  * sums in fp32.  key_valid [batch, valid_rows] bytes with a row pitch (0 = masked row), or
- * NULL; rows from valid_rows on count.  What a masked row holds is not read.  A sequence
+ * NULL; rows from valid_rows on count.  It speaks of rows, which an eviction moves: a cache
+ * that evicts is to hold no padding.  What a masked row holds is not read.  A sequence
  * with no row left gives out = 0, lse = -inf; rows that count but all score -inf give
  * out = NaN (0 / 0), lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.
  * `track` adds each row's probability, summed over the query heads of its key-value head,
@@ -546,7 +547,8 @@ int pi05_paged_attention(const Pi05PagedCache* cache, const Pi05PagedAttention* 
  * positions (pos >= counts[1][b] - recent) and of positions below `sinks` only after
  * all others.  Rows that stay and lie below the budget keep their place; the holes
  * between them are filled, in order, by the ones that stay from above, with their
- * weight and pos.  Rows from the budget on are left as they are.  Needs `weight` and
+ * weight and pos (so that a key_valid made before no longer fits).  Rows from the budget
+ * on are left as they are.  Needs `weight` and
  * `pos`; budget >= 1, recent and sinks >= 0, recent + sinks <= budget. */
 int pi05_paged_evict(const Pi05PagedCache* cache, int budget, int recent, int sinks, void* stream);
 

@@ -553,7 +553,10 @@ class PagedKVCache:
 
         ``scale`` is ``head_dim ** -0.5`` if not given.  ``key_valid`` (bool or uint8 ``[batch, n]``):
         rows that are False are left out, whatever they hold; rows from ``n`` on count (a prompt's
-        padding mask need not grow with the sequence).  ``track`` adds the probabilities to the
+        padding mask need not grow with the sequence).  It speaks of rows, not of positions: once
+        :meth:`evict` has moved rows, a mask made before means other tokens, and no one mask can say
+        what each head holds.  A cache that evicts is to hold no padding: leave it out of
+        :meth:`append` with ``cu_tokens``.  ``track`` adds the probabilities to the
         cache's ``weight`` (its scratch holds a score of every query head for each row that the table
         reaches or, beyond 64 MB, that the pool has).  A sequence with no row gives zeros (lse
         ``-inf``); rows that count but all score ``-inf`` give NaN, as a softmax of them does.  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
@@ -606,7 +609,7 @@ class PagedKVCache:
         (ties: the lowest row first; NaN first of all), those of the ``recent`` newest positions and
         of the first ``sinks`` positions only after all others.  The holes below the budget are filled in
         order by the rows that stay from above it, so the rows of a head are in no order of age
-        afterwards: ``pos`` says which token a row is.
+        afterwards: ``pos`` says which token a row is, and a ``key_valid`` made before no longer fits.
         """
         if self.weight is None or self.pos is None:
             raise ValueError("this cache keeps no weights and positions: build it with weight= and pos=")

@@ -518,3 +518,34 @@ def test_attend_every_kernel(case, dtype):
     check_attend(c, t, q)
     check_attend(c, t, q, valid=valid, track=True)
     assert c.read_status() == 0
+
+
+# ---------------------------------------------------------------------------
+# padding and eviction
+# ---------------------------------------------------------------------------
+
+
+def test_padded_prompts_and_eviction():
+    """Left-padded prompts for a cache that evicts: their tokens alone are appended, and attended to without a mask;
+    until an eviction that is the same as all of them under the mask."""
+    batch, n, heads, dim, f = 3, 90, 8, 64, RopeFrequencies(64)
+    pad = [0, 25, 60]
+    g = gen(9)
+    k, v, q = rnd(batch, n, 2, dim, g=g), rnd(batch, n, 2, dim, g=g), rnd(batch, heads, dim, g=g)
+    valid = torch.arange(n, device="cuda")[None] >= torch.tensor(pad, device="cuda")[:, None]
+    padded, _ = make(batch, 2, dim, 16, 100)
+    padded.append(k.flatten(0, 1), v.flatten(0, 1), cu_tokens=torch.arange(4, dtype=torch.int32, device="cuda") * n)
+    c, _ = make(batch, 2, dim, 16, 100)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum([n - p for p in pad])]), dtype=torch.int32, device="cuda")
+    c.append(k[valid], v[valid], cu_tokens=cu)
+    both = padded.attend(q, key_valid=valid), check_attend(c, twin(c), q, track=True)
+    # the same sums in another order, each output within its own tolerance: two roundings, and fp32's
+    assert (np.abs(np64(both[0]) - np64(both[1])) <= 2 * u(BF) * np.abs(np64(both[1])) + 2.0**-12).all()
+    for step in range(3):
+        t = twin(c)
+        c.evict(40 - 5 * step, recent=8, sinks=2)
+        t.evict(40 - 5 * step, 8, 2)
+        same_rows(c, t)
+        check_attend(c, t, q, track=True)
+        q = c.append(rnd(batch, 2, dim, g=g), rnd(batch, 2, dim, g=g), q=q, freqs=f)
+    assert c.read_status() == 0
