@@ -177,46 +177,51 @@ def _cuda(device) -> torch.device:
 # ---------------------------------------------------------------------------
 
 
-_PI = Decimal("3.1415926535897932384626433832795028841971693993751")
+_ONE = 1 << 128
+_PER_RAD = 0x28be60db9391054a7f09d5f47d4d3770  # 2^128 / (2 pi): turns of a radian
 
 
 def _exact_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast, beta_slow):
-    """Rad per position of each pair, to 40 digits (a 64-bit float's 53 bits would show from position 10^8 on), and
+    """Rad per position of each pair, in units of 2^-128 (a 64-bit float's 53 bits would show from position 10^8 on), and
     the factor on cos and sin."""
+    base, factor = float(base), float(factor)
+    num, den = factor.as_integer_ratio()
     with localcontext() as context:
-        context.prec = 50
-        exact_base, exact_factor = Decimal(base), Decimal(factor)
-        if scaling == "ntk":
-            exact_base *= exact_factor ** (Decimal(rotary_dim) / (rotary_dim - 2))
-        ratio = exact_base ** (Decimal(-2) / rotary_dim)
-        inv_freq = [Decimal(1)]
-        while len(inv_freq) < rotary_dim // 2:
-            inv_freq.append(inv_freq[-1] * ratio)
-        if scaling == "linear":
-            return [f / exact_factor for f in inv_freq], 1.0
-        if scaling != "yarn":
-            return inv_freq, 1.0
+        context.prec = 40
+        ratio = Decimal(base) ** (Decimal(-2) / rotary_dim)
+        if scaling == "ntk":  # (base factor^(rotary_dim / (rotary_dim - 2)))^(-2 / rotary_dim)
+            ratio *= Decimal(factor) ** (Decimal(-2) / (rotary_dim - 2))
+        ratio = int(ratio * _ONE)
+    inv_freq = [_ONE]
+    while len(inv_freq) < rotary_dim // 2:
+        inv_freq.append(inv_freq[-1] * ratio >> 128)
+    if scaling == "linear":
+        return [f * den // num for f in inv_freq], 1.0
+    if scaling != "yarn":
+        return inv_freq, 1.0
 
-        def pair(turns):  # number (not whole) of the pair that turns so often within original_len
-            return rotary_dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
+    def pair(turns):  # number (not whole) of the pair that turns so often within original_len
+        return rotary_dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
-        width = max(Decimal(high - low), Decimal("0.001"))
-        ramp = [min(max((i - low) / width, Decimal(0)), Decimal(1)) for i in range(rotary_dim // 2)]
-        return [f / exact_factor * r + f * (1 - r) for f, r in zip(inv_freq, ramp)], 0.1 * math.log(factor) + 1.0
+    low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
+    scale, width = (1, high - low) if high > low else (1000, 1)  # at least a thousandth of a pair wide
+    ramp = [min(max((i - low) * scale, 0), width) for i in range(rotary_dim // 2)]
+    return [f * (r * den + (width - r) * num) // (width * num) for f, r in zip(inv_freq, ramp)], 0.1 * math.log(factor) + 1.0
+
+
+def _floats(inv_freq):
+    return [f / _ONE for f in inv_freq]
 
 
 def _pair_frequencies(*args):
     """As 64-bit floats."""
     inv_freq, magnitude = _exact_frequencies(*args)
-    return [float(f) for f in inv_freq], magnitude
+    return _floats(inv_freq), magnitude
 
 
 def _turns(inv_freq):
-    """Fractions of a turn per position in units of 2^-64 (below one half: every frequency is at most 1 rad)."""
-    with localcontext() as context:
-        context.prec = 50
-        return [round(Decimal(f) / (2 * _PI) * 2**64) for f in inv_freq]
+    """Fractions of a turn per position in units of 2^-64, rounded (below one half: every frequency is at most 1 rad)."""
+    return [((f if isinstance(f, int) else int(f * _ONE)) * _PER_RAD + (1 << 191)) >> 192 for f in inv_freq]
 
 
 class RopeFrequencies:
@@ -256,7 +261,7 @@ class RopeFrequencies:
             raise ValueError("'yarn' scaling needs original_len and beta_fast > beta_slow > 0")
         self.rotary_dim, self.layout = rotary_dim, layout
         exact, self.magnitude = _exact_frequencies(rotary_dim, base, scaling, factor, original_len, beta_fast, beta_slow)
-        self.inv_freq = [float(f) for f in exact]
+        self.inv_freq = _floats(exact)
         turns = _turns(exact)
         self.device = _cuda(device)
         self.turns = torch.tensor(turns, dtype=torch.int64).to(self.device)

@@ -4,6 +4,7 @@ import ctypes
 import math
 from decimal import Decimal, localcontext
 
+import numpy as np
 import pytest
 import torch
 
@@ -57,3 +58,9 @@ def test_sizes_go_by_the_pool():
     assert lists < 1 << 17 and 60 << 20 < scores < 65 << 20
     lists, scores = sizes(pages_per_seq=16, num_pages=1 << 20)  # short tables over a large pool: by the table
     assert lists < 4 * 256 * 8 * 256 + (1 << 16) and scores < 16 * 256 * 8 * (256 + 128) + (1 << 16)
+
+
+def test_frequencies_of_other_number_types():
+    want = paged._exact_frequencies(64, 500000.0, "ntk", 8.0, None, 32.0, 1.0)
+    for of in (int, np.float32, np.float64):
+        assert paged._exact_frequencies(64, of(500000), "ntk", of(8), None, 32.0, 1.0) == want
