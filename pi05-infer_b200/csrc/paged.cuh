@@ -253,7 +253,7 @@ struct Unit {
 // Values to a unit: as many as a word of 16, 8 or 4 bytes holds (or one) that divide the pairs' halves,
 // the head, every stride and every pointer.  `bytes`: of a value.  Single values cost an
 // instruction each: 32768 tokens of 32 heads of 72 (36 pairs, no multiple of the 8
-// values of 16 bytes) turn in 50 us with 8-byte words and took 160 with single values; the append of 16384
+// values of 16 bytes) turn in 51 us with 8-byte words and took 160 with single values; the append of 16384
 // tokens of 8 + 8 heads of 72 takes 30 instead of 93.
 template <class... P>
 int unit_values(int bytes, int rotary, bool interleaved, int dim, std::initializer_list<long long> strides,
@@ -267,6 +267,8 @@ int unit_values(int bytes, int rotary, bool interleaved, int dim, std::initializ
 }
 
 // ---- division by a number known at launch (n < 2^31) ------------------------
+// By a multiplication, after Granlund and Montgomery, "Division by invariant integers using
+// multiplication" (1994).
 struct FastDiv {
   uint32_t mul, shift, d;
   FastDiv() = default;

@@ -21,10 +21,14 @@
 // accumulators as with 16 padded query rows.  The probabilities enter the second product as
 // a sum of two numbers of the cache's 16-bit type (see halves()); m, l and o stay fp32.
 //
-// Measured: 2 x 131072 rows, 32 / 8 heads of 128: 157 us = 6.8 TB/s + 5 us for the join.
-// The same with 16-byte cp.async copies through registers' addresses: 190 us (430
-// instructions a tile, and 8 warps an SM are too few to hide them); with a bulk copy for
-// each row, issued one by one: 174 us with 12 warps, 206 us with 8.
+// Measured: 2 x 131072 rows, 32 / 8 heads of 128: 167 us with the join's 5 = 6.6 TB/s (with
+// one 16-bit number for a probability 166).  An earlier form with 16-byte cp.async copies
+// through registers' addresses took 190 us where TMA took 157 (430 instructions a tile, and 8
+// warps an SM are too few to hide them); with a bulk copy for each row, issued one by one, 174
+// with 12 warps, 206 with 8.  More than 8 query heads to a key-value head are the weak side:
+// with 256 columns one CTA of four warps has an SM, and its accumulators leave the registers (430
+// bytes): 54 x 16 pairs of 104 rows, 16 query heads each, 143 us for 92 MB; above 16 each part
+// reads the rows again (33 heads over 131072 rows of 128: 54 us for 67 MB).
 #include <algorithm>
 #include <type_traits>
 
@@ -929,11 +933,12 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   // The form without further kernels: up to 8 CTAs for each pair while two of them (one,
   // for heads over 128) have an SM to themselves, with 1024 rows each at most (512).  us a
   // call there / with equal shares (32 / 8 heads of 128, uniform lengths): 32 pairs of 1000
-  // rows 7.8 / 13.3, of 8000 26 / 30; 128 of 512 13 / 16, of 2000 28 / 29, of 1 to 2000 24 /
-  // 21; 120 of 512 rows of 256 columns 22 / 27.  Beyond, the longest sequence or the scores'
+  // rows 7.8 / 13.5, of 8000 26 / 31; 128 of 512 13 / 16, of 2000 28 / 30, of 1 to 2000 24 /
+  // 22; 120 of 512 rows of 256 columns 22 / 28.  Beyond, the longest sequence or the scores'
   // share of an SM decides: 320 pairs of 512 rows, tracked, 36 / 28; 384 of 1 to 1500 rows
-  // of 80 columns 30 / 25; 150 of 512 rows of 256 columns 41 / 29; 1600 of 512 rows of 64
-  // columns 44 / 42.
+  // of 80 columns 30 / 26; 150 of 512 rows of 256 columns 40 / 29; 1600 of 512 rows of 64
+  // columns 44 / 43.  All with tables of the longest sequence's length: the host knows the table's
+  // reach and not the lengths, so short sequences behind a long table go by the second figures.
   const bool narrow = s.ks <= 8;
   const long long pairs = (long long)c->batch * c->n_kv_heads, at_once = narrow ? 2 * kSMs : kSMs;
   int ctas = 8;

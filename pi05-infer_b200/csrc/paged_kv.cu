@@ -99,8 +99,8 @@ struct __align__(16) TokenRow {
 
 // ROT: with rotation.  Two kernels, since the registers of the one cost the other its
 // occupancy: with v's first batch held over the row search as well, the append of 16384
-// rotated tokens took 44 us instead of 37; without, that of 65536 plain ones 105 instead
-// of 93.
+// rotated tokens took 44 us instead of 37 (38 with the angles' quarter turns); without, that of
+// 65536 plain ones 105 instead of 93.
 template <class T, int V, int VC, bool ROT>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ Pages c,
                                                                 const __grid_constant__ AppendParams p) {
@@ -689,7 +689,8 @@ int append_run(const Pages& c, AppendParams p, cudaStream_t stream) {
                     p);
 }
 
-// The turned rows and the copied ones each take the widest word of their own.
+// The turned rows take the widest word that fits them; the copied ones (v, and k without rotation)
+// 16 bytes, or single values where that does not fit.
 template <class T, int V>
 int append_rotated(const Pages& c, const AppendParams& p, bool rows, cudaStream_t stream) {
   return rows ? append_run<T, V, 8, true>(c, p, stream) : append_run<T, V, 1, true>(c, p, stream);

@@ -99,7 +99,7 @@ int rope_run(const void* x, void* out, RopeParams p, cudaStream_t stream) {
   p.by_pairs = FastDiv(p.rotary / 2);
   // A few batches of loads for a CTA, but for tokens enough to fill the SMs.  The longer of
   // the two passes counts: with many tokens to a CTA, L2 has lost the sectors and lines that
-  // both touch before the second comes (32768 tokens of 32 heads of 80, 40 of them turned: 80
+  // both touch before the second comes (32768 tokens of 32 heads of 80, 40 of them turned: 81
   // us; by the turned part alone 137).
   const int fill = std::max(1, 4 * J * (kThreads / std::max(p.turned_lanes, p.passed_lanes)) / p.heads);
   p.per_cta = std::max(1, std::min({fill, p.tokens / (4 * kSMs), 48 * 1024 / (p.rotary / 2 * (int)sizeof(float2))}));
