@@ -965,7 +965,8 @@ Plan make_plan(const Pi05PagedCache* c, int q_heads, int track) {
   // block begun and the border for each pair): whoever tracks has each row in one sequence alone.
   // No less than for one pair that the table's reach fills.
   const size_t unit_bytes = (size_t)kBlockRows * s.score_pitch * 4;
-  const long long pool = (((long long)c->num_pages * c->page_size) / kBlockRows + (1ll + kBorder) * c->batch) * c->n_kv_heads * s.parts;
+  const long long pool = ((long long)c->num_pages * c->page_size / kBlockRows + (1ll + kBorder) * c->batch) *
+                         c->n_kv_heads * s.parts;
   const long long longest = blocks_of(capacity) + kBorder;
   s.score_units = (int)std::min<long long>(
       {longest * s.rows, std::max<long long>({pool, longest, (long long)((64 << 20) / unit_bytes)}), 0x7fffffff});

@@ -355,7 +355,8 @@ struct MoveList {
   int b, h;
   int32_t* dense;
   __device__ __forceinline__ MoveList(const Pages& pages, bool slots, int seq, int head)
-      : c(pages), by_slot(slots), b(seq), h(head), dense(pages.move_list + (size_t)(seq * pages.heads + head) * pages.capacity) {}
+      : c(pages), by_slot(slots), b(seq), h(head),
+        dense(pages.move_list + (size_t)(seq * pages.heads + head) * pages.capacity) {}
   __device__ __forceinline__ int32_t* at(int i) const {
     if (!by_slot) return dense + i;
     int line;
@@ -761,7 +762,8 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* a, voi
   const long long kt = stride_of(a->tokens, a->k_token_stride), kh = stride_of(c.heads, a->k_head_stride);
   const long long vt = stride_of(a->tokens, a->v_token_stride), vh = stride_of(c.heads, a->v_head_stride);
   const bool q = a->q != nullptr;
-  const long long qt = q ? stride_of(a->tokens, a->q_token_stride) : 0, qh = q ? stride_of(a->n_q_heads, a->q_head_stride) : 0;
+  const long long qt = q ? stride_of(a->tokens, a->q_token_stride) : 0;
+  const long long qh = q ? stride_of(a->n_q_heads, a->q_head_stride) : 0;
   for (long long stride : {kt, kh, vt, vh, qt, qh})
     if (stride < 0 || stride >= 1ll << 31) {
       set_last_error("paged_append: stride of %lld elements", stride);

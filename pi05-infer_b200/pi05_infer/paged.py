@@ -303,7 +303,8 @@ def _leaf_node(x: torch.Tensor):
 
     Torch makes it with the first graph that uses the leaf and keeps it as long as any lives; a backward
     pass waits for its stream, which a capture on another stream cannot (torch then breaks the capture off
-    and leaves its random generator in it).  So a captured call is refused while such a graph is alive.
+    and leaves its random generator in it).  So a captured call is refused while such a graph is alive;
+    torch does not say on which stream other operators made one.
     """
     node = torch.autograd.graph.get_gradient_edge(x).node
     stream = _raw_stream(x.get_device())
@@ -344,16 +345,17 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: RopeFrequencies, *, tr
     to ``positions`` ``[tokens]`` (int32 or int64, any sign).
 
     bf16, fp16 or fp32, fp32 math, one rounding.  Any token and head strides (a q|k|v row's q and k
-    heads in one call, say, or views that overlap); values of a head contiguous.  ``out`` may be ``x`` (in place), but not
-    overlap it otherwise.  ``transpose`` turns backwards.  Differentiable in ``x``, in reverse and
-    forward mode, when ``out`` is not given; a captured call with a leaf ``x`` is refused while a graph of it from another stream
-    is alive.
+    heads in one call, say, or views that overlap); values of a head contiguous.  ``out`` may be ``x``
+    (in place), but not overlap it otherwise, nor itself.  ``transpose`` turns backwards.
+    Differentiable in ``x``, in reverse and forward mode, when ``out`` is not given.  A captured call
+    with a leaf ``x`` is refused while a graph that this function made of it on another stream is
+    alive; drop graphs that other operators made of it before such a capture.
     """
     if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda or x.stride(2) != 1:
         raise ValueError("x must be a [tokens, heads, dim] CUDA tensor, bf16, fp16 or fp32, contiguous in dim")
     index, (tokens, _, dim) = x.get_device(), x.shape
-    if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype not in _POSITIONS or positions.get_device() != index or \
-            not positions.is_contiguous():
+    if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype not in _POSITIONS or \
+            positions.get_device() != index or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32 or int64 [tokens] on x's device")
     if freqs._index != index:
         raise ValueError(f"the frequencies are on {freqs.device}, x is on {x.device}")
@@ -564,8 +566,9 @@ class PagedKVCache:
         :meth:`append` with ``cu_tokens``.  ``track`` adds the probabilities to the
         cache's ``weight`` (its scratch holds a score of every query head for each row that the table
         reaches or, beyond 64 MB, that the pool has).  A sequence with no row gives zeros (lse
-        ``-inf``); rows that count but all score ``-inf`` give NaN, as a softmax of them does.  Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32
-        natural-log sums ``[batch, heads]``.
+        ``-inf``); rows that count but all score ``-inf`` give NaN, as a softmax of them does.
+        Returns ``out`` ``[batch, heads, head_dim]``, with ``return_lse`` also the fp32 natural-log
+        sums ``[batch, heads]``.
         """
         (batch, heads, dim), (q_token, q_head, _) = self._rows(q, "q", None)
         self._no_gradients((q, out, self.k_pages, self.v_pages, self.weight if track else None),
