@@ -521,7 +521,8 @@ int pi05_paged_append(const Pi05PagedCache* cache, const Pi05PagedAppend* args, 
  * with no row left gives out = 0, lse = -inf; rows that count but all score -inf give
  * out = NaN (0 / 0), lse = -inf.  lse (natural logarithm) [batch, n_q_heads] or NULL.
  * `track` adds each row's probability, summed over the query heads of its key-value head,
- * to the cache's `weight`.  q with strides, out dense [batch, n_q_heads, head_dim].
+ * to the cache's `weight` (which stays, with PI05_DEV_BAD_INDEX, where sequences share
+ * pages so often that the scratch cannot hold their scores).  q with strides, out dense [batch, n_q_heads, head_dim].
  * `scratch`: pi05_paged_attention_scratch_bytes() bytes (0 for a few short sequences),
  * 16-byte aligned, any content.
  * The result does not depend on the run: every sum has a fixed order. */
